@@ -5,7 +5,8 @@ cd "$(dirname "$0")"
 OUT=../libsuave_hip.so
 OBJ=../../build/obj
 mkdir -p "$OBJ"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function $SUAVE_EXTRA_FLAGS"
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops $SUAVE_EXTRA_FLAGS"
 pids=()
 for f in gemm decode loss wide embed latent optim sample frame head api; do
   [ -f $f.hip ] || continue
