@@ -262,6 +262,58 @@ int suave_elbo_joint_backward(const suave_plan* plan, const float* params, const
                               void* workspace, size_t workspace_bytes, void* stream, const suave_elbo_out_t* out,
                               float* grads, const suave_head_t* head, void* decoder_ready_event);
 
+/* ---- heads of many classes, orthogonalised updates, 8-bit serving ---------------------------------------------
+ * Element type of the matrices of the three operators below.  bf16 is the upper half of a binary32. */
+#define SUAVE_DTYPE_F32 0
+#define SUAVE_DTYPE_BF16 1
+
+/* Linear layer + class-weighted softmax cross entropy for heads beyond suave_head_step's 64 classes (heads.py:62-91 with
+ * F.cross_entropy; also the last layer of a head with hidden layers), with its gradients, without keeping the
+ * [n_rows, n_classes] logits: scratch grows with n_rows * n_classes / 8 bytes (statistics of 64-class strips) plus one
+ * piece of the logit gradient (at most 192 MiB, or 256 classes of it).
+ *   loss = sum_i w[y_i] (log sum_c exp l_ic - l_i,y_i) / weight_sum,   l = x weight^T + bias
+ * weight_sum = sum_i w[y_i], or *weight_sum if given (data parallelism: the GLOBAL batch).  targets[i] < 0 leaves row i
+ * out: it adds nothing anywhere, whatever x holds there, and its dx is zero; targets[i] >= n_classes makes the row's
+ * loss NaN and with it the mean and the gradients.  A batch with no weight has loss 0 and zero gradients.  bias may
+ * hold -inf (a class that is never predicted); other non-finite inputs make what they touch non-finite.
+ * F32: products of binary32 grade (two fp16 planes per operand and tensor scale; elements 2^28 times smaller than their
+ * tensor's largest lose relative accuracy).  BF16: fp32 accumulation, the logit gradient rounded to bf16 once.
+ * Outputs that are NULL are not computed.  dx / dweight have the type of x / weight and are overwritten, multiplied by
+ * loss_scale like dbias; *loss is overwritten, *loss_sum += loss * loss_rows.  Results do not depend on anything but the
+ * arguments (no atomics).  Strides in elements.  No output may overlap an input.  workspace: 256-byte aligned; one call at
+ * a time uses it. */
+typedef struct suave_linear_ce_t {
+  int32_t dtype;
+  int32_t n_classes;
+  int32_t dim;
+  int64_t n_rows;
+  const void* x;              /* [n_rows, ld_x] */
+  int64_t ld_x;
+  const void* weight;         /* [n_classes, ld_weight] */
+  int64_t ld_weight;
+  const float* bias;          /* [n_classes] or NULL */
+  const int32_t* targets;     /* [n_rows] */
+  const float* class_weight;  /* [n_classes] or NULL */
+  const float* weight_sum;    /* device scalar or NULL */
+  float loss_scale;
+  float loss_rows;
+  float* loss;                /* device scalar or NULL */
+  double* loss_sum;           /* device scalar or NULL */
+  float* row_loss;            /* [n_rows] or NULL: w[y] * cross entropy, not divided */
+  float* lse;                 /* [n_rows] or NULL: log sum exp of the logits */
+  void* dx;
+  int64_t ld_dx;
+  void* dweight;
+  int64_t ld_dweight;
+  float* dbias;
+  void* workspace;
+  size_t workspace_bytes;
+} suave_linear_ce_t;
+/* Bytes of workspace for a call with these fields (the pointers of weight and outputs count: which of them are NULL, and
+ * weight's alignment; workspace itself is not looked at). */
+int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes);
+int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
+
 /* Decoder.forward's per-column log-likelihoods at a GIVEN latent (decoder.py:333-379 as called by the reference's
  * decode-side code and tests): y_full = trunk(z), then every head scores the batch's cells with the row's
  * component as the assignment one-hot.  log_px / log_px_missing: [n, n_cols], laid out as the fields of that name in the ELBO output struct (either may

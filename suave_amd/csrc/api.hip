@@ -1433,6 +1433,15 @@ extern "C" int suave_elbo_joint_backward(const suave_plan* p, const float* param
                    static_cast<hipStream_t>(stream), out, grads, nullptr, static_cast<hipEvent_t>(decoder_ready_event), head);
 }
 
+extern "C" int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes) {
+  return suave::linear_ce_workspace(call, bytes);
+}
+
+extern "C" int suave_linear_ce(const suave_linear_ce_t* call, void* stream) {
+  suave::drop_stale_hip_error();
+  return suave::launch_linear_ce(call, static_cast<hipStream_t>(stream));
+}
+
 extern "C" int suave_encode(const suave_plan* p, const float* params, const suave_batch_t* batch,
                             float inv_temperature, void* workspace, size_t workspace_bytes, void* stream,
                             float* enc_out, float* post_mean, float* post_logvar, float* probs) {

@@ -296,4 +296,8 @@ size_t head_workspace_floats(int C, int D);
 int launch_head_loss(const suave_head_t& h, int D, const float* latent, int ld, int latent_by_row_id, const int32_t* row_index,
                      int64_t row_begin, int64_t n, float* dz, int ldz, float* logits_out, hipStream_t s);
 
+// ----- many-class head (lce.hip) --------------------------------------------------
+int linear_ce_workspace(const suave_linear_ce_t* h, size_t* bytes);
+int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s);
+
 }  // namespace suave

@@ -1,0 +1,799 @@
+// Linear layer + softmax cross entropy over many classes, with gradients, without keeping the [n, C] logits.
+//
+//   l_ic = x_i . W_c + b_c      lse_i = log sum_c exp l_ic      ce_i = w[y_i] (lse_i - l_i,y_i)      loss = sum ce / sum w[y]
+//   G_ic = s w[y_i] / sum w (exp(l_ic - lse_i) - [c = y_i])     dx = G W       dW = G^T x            db = sum_i G_i
+//
+// Two sweeps over the classes.  The first computes logit tiles on the matrix pipe and keeps of each 64-class strip of a row
+// its maximum and its sum of exponentials (8 bytes for 64 logits) and the target's logit; the strips of a row are then joined.
+// The second computes the tiles again, now against the known lse, and writes G for one piece of the classes at a time (bounded
+// scratch), which two products turn into dx (summed over the pieces in fp32) and dW.  8 n C D flops instead of 6: the price of
+// not keeping the logits.
+//
+// bf16 operands are multiplied as they are, G is rounded to bf16 for its two products (relative 2^-9 of each entry, below the
+// rounding of the bf16 results); db and every sum stay fp32.  fp32 operands are scaled by a power of two per tensor, cut into
+// two fp16 planes once per call (mma.h), G likewise: binary32's own accuracy on the fp16 pipe.
+//
+// Rows with a negative target are left out whatever they hold (x is copied with those rows zero); a target >= C makes its row's
+// loss NaN, and with it the mean and the gradients.  No atomics: partial sums are written out and added in a fixed order.
+#include <algorithm>
+#include <cmath>
+
+#include "kernels.h"
+#include "mma.h"
+
+namespace suave {
+
+namespace {
+
+using namespace mma;
+
+constexpr int kStrip = 64;          // classes of one (max, sum) pair
+constexpr int kClassPad = 256;      // bias and G are padded to whole tiles of classes
+constexpr int kAmaxBlocks = 256;    // partial maxima per tensor
+constexpr int kCUs = 256;
+constexpr size_t kPieceBytes = (size_t)192 << 20;  // G of one piece: what the 256 MB memory-side cache holds beside its operands
+
+struct Scalars {
+  float x_scale, w_scale;    // powers of two the planes were multiplied by (1 for bf16)
+  float g_unit;              // loss_scale * max|w| / total / kGScale: what one unit of the stored G is worth
+  float max_w;
+};
+
+// G is stored relative to the largest row weight (entries in [-1, 1]) times 2^14: fp16's hi plane is normal down to 2^-28
+__host__ __device__ constexpr float g_scale(bool planes) { return planes ? 16384.0f : 1.0f; }
+
+struct PackArgs {
+  const void* src[2];        // x, W
+  int64_t ld[2];             // elements
+  int64_t rows[2];
+  char* dst[2];              // null: not packed
+  int64_t dst_ld[2];         // bytes
+  int blocks0;               // blocks of tensor 0
+  int D, Dp;
+  const int32_t* targets;    // rows of tensor 0 with a negative target are zero
+  float* amax;               // [2][kAmaxBlocks]
+  Scalars* scal;
+  const float* bias;         // null: zero
+  float* bias_pad;           // [round_up(C, kClassPad)], -inf past C
+  int C, C_pad;
+};
+
+__device__ __forceinline__ float load_as_float(const float* p) { return *p; }
+__device__ __forceinline__ float load_as_float(const uint16_t* p) { return bf16_value(*p); }
+
+// largest finite |value| of x (rows that count) and W, in kAmaxBlocks partials each
+__global__ __launch_bounds__(256) void k_lce_amax(PackArgs a) {
+  __shared__ float part[4];
+  const int t = blockIdx.x >= kAmaxBlocks;
+  const float* src = static_cast<const float*>(a.src[t]);
+  const int64_t rows = a.rows[t], ld = a.ld[t];
+  const int b = blockIdx.x - t * kAmaxBlocks;
+  float m = 0.f;
+  // a wave per row piece: D may be anything from 1 on, so the flat element range is walked with 64-bit division-free steps
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (a.D >= 64) {
+    for (int64_t r = (int64_t)b * 4 + wave; r < rows; r += (int64_t)kAmaxBlocks * 4) {
+      if (t == 0 && a.targets[r] < 0) continue;
+      const float* p = src + r * ld;
+      for (int d = lane; d < a.D; d += 64) {
+        const float v = fabsf(p[d]);
+        if (v < INFINITY) m = fmaxf(m, v);
+      }
+    }
+  } else {  // narrow rows: lanes over rows
+    for (int64_t r = ((int64_t)b * 4 + wave) * 64 + lane; r < rows; r += (int64_t)kAmaxBlocks * 256) {
+      if (t == 0 && a.targets[r] < 0) continue;
+      const float* p = src + r * ld;
+      for (int d = 0; d < a.D; ++d) {
+        const float v = fabsf(p[d]);
+        if (v < INFINITY) m = fmaxf(m, v);
+      }
+    }
+  }
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if (lane == 0) part[wave] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) a.amax[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+// the power of two that brings amax into [2^13, 2^14) (products of two such and their sums stay far inside binary32)
+__device__ __forceinline__ float plane_scale(float amax) {
+  if (!(amax > 0.f)) return 1.0f;
+  int e;
+  (void)frexpf(amax, &e);  // amax = f 2^e, f in [1/2, 1)
+  return ldexpf(1.0f, min(14 - e, 120));
+}
+
+template <class T, bool PLANES>
+__global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
+  const int t = (int)blockIdx.x >= a.blocks0;
+  const int b = blockIdx.x - (t ? a.blocks0 : 0), nb = t ? (int)gridDim.x - a.blocks0 : a.blocks0;
+  float scale = 1.0f;
+  if constexpr (PLANES) {
+    __shared__ float sc;
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < 64) {
+      float m = 0.f;
+      for (int i = lane; i < kAmaxBlocks; i += 64) m = fmaxf(m, a.amax[t * kAmaxBlocks + i]);
+      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      if (lane == 0) sc = plane_scale(m);
+    }
+    __syncthreads();
+    scale = sc;
+  }
+  if (b == 0 && threadIdx.x == 0) (t ? a.scal->w_scale : a.scal->x_scale) = scale;
+  if (t) {
+    for (int64_t c = (int64_t)b * 256 + threadIdx.x; c < a.C_pad; c += (int64_t)nb * 256)
+      a.bias_pad[c] = c < a.C ? (a.bias ? a.bias[c] : 0.f) : -INFINITY;
+  }
+  if (a.dst[t] == nullptr) return;
+  const T* src = static_cast<const T*>(a.src[t]);
+  const int q = a.Dp / 8;  // 16-byte chunks of a row
+  const int64_t chunks = a.rows[t] * q, ld = a.ld[t];
+  for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
+    const int64_t r = e / q;
+    const int d0 = (int)(e - r * q) * 8;
+    const bool gone = t == 0 && a.targets[r] < 0;
+    const T* p = src + r * ld + d0;
+    uint16_t hi[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = !gone && d0 + i < a.D;
+      if constexpr (PLANES) {
+        planes(in ? load_as_float(p + i) * scale : 0.f, hi[i], lo[i]);
+      } else {
+        hi[i] = in ? p[i] : (T)0;
+      }
+    }
+    char* o = a.dst[t] + r * a.dst_ld[t] + d0 * 2;
+    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+    if constexpr (PLANES) *reinterpret_cast<uint4*>(o + (size_t)a.Dp * 2) = *reinterpret_cast<const uint4*>(lo);
+  }
+}
+
+struct LogitArgs {
+  const char* x; int64_t ldx;      // packed [n][..], bytes
+  const char* w; int64_t ldw;
+  uint32_t plane;                  // bytes hi -> lo in a row of x and W
+  int64_t n;
+  int C, D;
+  int c0, c1;                      // classes of this launch
+  int group;
+  const Scalars* scal;
+  const float* bias;               // padded
+  const int32_t* targets;
+  // first sweep
+  float2* strips;                  // [strip][n] (max, sum exp(l - max))
+  float* target_logit;             // [n]
+  // second sweep
+  const float2* row;               // (lse, row weight / max weight)
+  char* g; int64_t ldg; uint32_t g_plane;  // [n][c1 - c0 rounded up], bytes
+  float* db;                       // [row tiles of a wave][C_pad]
+  int64_t db_ld;
+};
+
+// One tile of logits; SWEEP 0: strip statistics, 1: G
+template <class T, int SWEEP>
+__global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tiles_m = (int)((a.n + T::BM - 1) / T::BM), tiles_n = (a.c1 - a.c0 + T::BN - 1) / T::BN;
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, a.group, tm, tn);
+  const int64_t m_base = (int64_t)tm * T::BM;
+  const int c_base = a.c0 + tn * T::BN;
+  const Operand A{a.x + m_base * a.ldx, (uint32_t)a.ldx, (int)min<int64_t>(T::BM, a.n - m_base), a.plane};
+  const Operand B{a.w + (int64_t)c_base * a.ldw, (uint32_t)a.ldw, a.C - c_base, a.plane};
+  typename T::acc_t acc[T::MI][T::NI];
+  T::run(lds, A, B, a.D, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int g = lane >> 4;
+  const float unit = 1.0f / (a.scal->x_scale * a.scal->w_scale);  // a power of two
+  const int cw = c_base + wn * (T::NI * 16);
+  float4 bias[T::NI];
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) bias[j] = *reinterpret_cast<const float4*>(a.bias + cw + 16 * j + 4 * g);
+  static_assert(T::NI * 16 == kStrip, "a wave owns one strip");
+  if constexpr (SWEEP == 0) {
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
+      const int y = m < a.n ? a.targets[m] : -1;
+      float v[T::NI][4], mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        const float* bj = reinterpret_cast<const float*>(&bias[j]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          v[j][u] = fmaf(acc[i][j][u], unit, bj[u]);
+          mx = fmaxf(mx, v[j][u]);
+          if (cw + 16 * j + 4 * g + u == y) a.target_logit[m] = v[j][u];
+        }
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float base = mx == -INFINITY ? 0.f : mx;  // a strip that is -inf throughout contributes exp(-inf) = 0
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += __expf(v[j][u] - base);
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if (g == 0 && m < a.n && cw < a.c1) a.strips[(int64_t)(cw / kStrip) * a.n + m] = make_float2(base, s);
+    }
+  } else {
+    constexpr bool P = T::NP == 2;
+    float cs[T::NI][4];
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) cs[j][u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
+      const bool in = m < a.n;
+      const int y = in ? a.targets[m] : -1;
+      const float2 rw = in ? a.row[m] : make_float2(0.f, 0.f);
+      char* grow = a.g + m * a.ldg + (int64_t)(cw - a.c0 + 4 * g) * 2;
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        const float* bj = reinterpret_cast<const float*>(&bias[j]);
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float l = fmaf(acc[i][j][u], unit, bj[u]);
+          float p = __expf(l - rw.x);
+          if (cw + 16 * j + 4 * g + u == y) p -= 1.0f;
+          const float gv = rw.y == 0.f ? 0.f : p * rw.y;  // a row without weight contributes nothing, whatever it holds
+          cs[j][u] += gv;
+          if constexpr (P) planes(gv * g_scale(true), hi[u], lo[u]);
+          else hi[u] = bf16_bits(gv);
+        }
+        if (in) {
+          *reinterpret_cast<uint2*>(grow + 32 * j) = *reinterpret_cast<const uint2*>(hi);
+          if constexpr (P) *reinterpret_cast<uint2*>(grow + 32 * j + a.g_plane) = *reinterpret_cast<const uint2*>(lo);
+        }
+      }
+    }
+    if (a.db != nullptr) {  // column sums over the wave's rows: lanes of equal g hold the same columns
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        float4 s;
+        float* sp = reinterpret_cast<float*>(&s);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float t = cs[j][u];
+#pragma unroll
+          for (int off = 8; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+          sp[u] = t;
+        }
+        if ((lane & 15) == 0) *reinterpret_cast<float4*>(a.db + (int64_t)(tm * T::WM + wm) * a.db_ld + cw + 16 * j + 4 * g) = s;
+      }
+    }
+  }
+}
+
+struct RowArgs {
+  const float2* strips; int n_strips;
+  int64_t n;
+  const int32_t* targets; int C;
+  const float* class_weight;
+  const float* target_logit;
+  float* row_loss;   // or null
+  float* lse_out;    // or null
+  float2* row;       // (lse, w)
+  double* part;      // [blocks][2]: sum of ce, sum of w over the block's rows
+  float* part_max;   // [blocks]
+  const float* weight_sum; float loss_scale, loss_rows; float gs;
+  float* loss; double* loss_sum; Scalars* scal;
+};
+
+// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights
+__global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
+  __shared__ float2 ms[64][17];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t m = (int64_t)blockIdx.x * 16 + r;
+  float mx = -INFINITY, s = 0.f;
+  if (m < a.n) {
+    for (int t0 = q; t0 < a.n_strips; t0 += 256) {  // four strips in flight
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = t0 + 64 * u < a.n_strips ? a.strips[(int64_t)(t0 + 64 * u) * a.n + m] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (v[u].y == 0.f) continue;  // nothing of the strip counts (all -inf); NaN goes on
+        const float nm = fmaxf(mx, v[u].x);
+        s = s * (mx == -INFINITY ? 0.f : __expf(mx - nm)) + v[u].y * __expf(v[u].x - nm);
+        mx = nm;
+      }
+    }
+  }
+  ms[q][r] = make_float2(mx, s);
+  __syncthreads();
+  double ce = 0.0, wsum = 0.0;
+  float wmax = 0.f;
+  if (threadIdx.x < 16 && m < a.n) {
+    float M = -INFINITY;
+    for (int k = 0; k < 64; ++k) M = fmaxf(M, ms[k][r].x);
+    float S = 0.f;
+    for (int k = 0; k < 64; ++k)
+      if (ms[k][r].y != 0.f) S += ms[k][r].y * __expf(ms[k][r].x - M);
+    const float lse = S == 0.f ? -INFINITY : M + logf(S);
+    const int y = a.targets[m];
+    float w = 0.f, l = 0.f;
+    if (y >= a.C) {
+      w = l = NAN;
+    } else if (y >= 0) {
+      w = a.class_weight ? a.class_weight[y] : 1.0f;
+      l = w == 0.f ? 0.f : w * (lse - a.target_logit[m]);
+    }
+    if (a.row_loss) a.row_loss[m] = l;
+    if (a.lse_out) a.lse_out[m] = lse;
+    a.row[m] = make_float2(lse, w);
+    ce = l;
+    wsum = w;
+    wmax = fabsf(w);
+  }
+  if (threadIdx.x < 64) {
+    for (int off = 8; off > 0; off >>= 1) {
+      ce += __shfl_xor(ce, off, 64);
+      wsum += __shfl_xor(wsum, off, 64);
+      wmax = fmaxf(wmax, __shfl_xor(wmax, off, 64));
+    }
+    if (threadIdx.x == 0) {
+      a.part[2 * blockIdx.x] = ce;
+      a.part[2 * blockIdx.x + 1] = wsum;
+      a.part_max[blockIdx.x] = wmax;
+    }
+  }
+}
+
+__global__ __launch_bounds__(1024) void k_lce_total(RowArgs a, int n_part) {
+  __shared__ double sce[16], sw[16];
+  __shared__ float sm[16];
+  double ce = 0.0, w = 0.0;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n_part; i += 1024) {
+    ce += a.part[2 * i];
+    w += a.part[2 * i + 1];
+    m = fmaxf(m, a.part_max[i]);
+  }
+  for (int off = 32; off > 0; off >>= 1) {
+    ce += __shfl_xor(ce, off, 64);
+    w += __shfl_xor(w, off, 64);
+    m = fmaxf(m, __shfl_xor(m, off, 64));
+  }
+  if ((threadIdx.x & 63) == 0) { sce[threadIdx.x >> 6] = ce; sw[threadIdx.x >> 6] = w; sm[threadIdx.x >> 6] = m; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    ce = w = 0.0;
+    m = 0.f;
+    for (int k = 0; k < 16; ++k) { ce += sce[k]; w += sw[k]; m = fmaxf(m, sm[k]); }
+    const double total = a.weight_sum ? (double)*a.weight_sum : w;
+    const double loss = total == 0.0 ? 0.0 : ce / total;  // (NaN stays NaN)
+    if (a.loss) *a.loss = (float)loss;
+    if (a.loss_sum) *a.loss_sum += loss * (double)a.loss_rows;
+    const bool none = total == 0.0;
+    a.scal->max_w = m;
+    a.scal->g_unit = none ? 0.f : (float)((double)a.loss_scale * (double)m / total) / a.gs;
+  }
+}
+
+// row weights relative to the largest: G's entries then lie in [-1, 1] whatever the scale of the class weights
+__global__ __launch_bounds__(256) void k_lce_relative(float2* row, int64_t n, const Scalars* scal) {
+  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (m < n) row[m].y = scal->max_w > 0.f ? row[m].y / scal->max_w : row[m].y;
+}
+
+struct GradArgs {
+  const char* a; int64_t lda; uint32_t a_plane;
+  const char* b; int64_t ldb; uint32_t b_plane;
+  int64_t M;
+  int N, K, splits, group;     // split s takes K range [s, s + 1) * round_up(ceil(K / splits), 64)
+  float* slab; int64_t slab_stride; int ld_slab;  // fp32 [splits][M][ld_slab]; null: out is written
+  int accumulate;              // add to what the slab holds (an earlier piece of the classes)
+  void* out; int64_t ld_out;   // T_out [M][N]
+  int out_bf16, out_vec;       // out_vec: rows may be stored four elements at a time
+  const Scalars* scal;
+  int which;                   // 0: dx (the classes' operand is W), 1: dW (x)
+};
+
+__device__ __forceinline__ float grad_factor(const Scalars* s, int which) { return s->g_unit / (which ? s->x_scale : s->w_scale); }
+
+__device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4], int n_valid, int bf16, int vec) {
+  if (bf16) {
+    uint16_t* o = static_cast<uint16_t*>(out) + at;
+    uint16_t h[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) h[u] = bf16_bits(v[u]);
+    if (vec && n_valid >= 4) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(h);
+    else
+      for (int u = 0; u < 4; ++u)
+        if (u < n_valid) o[u] = h[u];
+  } else {
+    float* o = static_cast<float*>(out) + at;
+    if (vec && n_valid >= 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      for (int u = 0; u < 4; ++u)
+        if (u < n_valid) o[u] = v[u];
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void k_lce_grad(GradArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tiles_m = (int)((a.M + T::BM - 1) / T::BM), tiles_n = (a.N + T::BN - 1) / T::BN;
+  const int per = tiles_m * tiles_n;
+  const int split = blockIdx.x / per;
+  int tm, tn;
+  tile_of(blockIdx.x - split * per, per, tiles_m, tiles_n, a.group, tm, tn);
+  const int64_t m_base = (int64_t)tm * T::BM;
+  const int n_base = tn * T::BN;
+  const int kper = ((a.K + a.splits - 1) / a.splits + 63) / 64 * 64;
+  const int k0 = min(split * kper, a.K), k1 = min(k0 + kper, a.K);
+  Operand A, B;
+  if (T::ACOL) A = Operand{a.a + (int64_t)k0 * a.lda + m_base * 2, (uint32_t)a.lda, (int)min<int64_t>((a.M - m_base + 7) / 8 * 16, 1 << 20), a.a_plane};
+  else A = Operand{a.a + m_base * a.lda + (int64_t)k0 * 2, (uint32_t)a.lda, (int)min<int64_t>(T::BM, a.M - m_base), a.a_plane};
+  if (T::BCOL) B = Operand{a.b + (int64_t)k0 * a.ldb + (int64_t)n_base * 2, (uint32_t)a.ldb, (a.N - n_base + 7) / 8 * 16, a.b_plane};
+  else B = Operand{a.b + (int64_t)n_base * a.ldb + (int64_t)k0 * 2, (uint32_t)a.ldb, a.N - n_base, a.b_plane};
+  typename T::acc_t acc[T::MI][T::NI];
+  T::run(lds, A, B, k1 - k0, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const float f = grad_factor(a.scal, a.which);
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i) {
+    const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
+    if (m >= a.M) continue;
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const int n = n_base + wn * (T::NI * 16) + 16 * j + 4 * (lane >> 4);
+      if (n >= a.N) continue;
+      if (a.slab) {
+        float4* o = reinterpret_cast<float4*>(a.slab + split * a.slab_stride + m * a.ld_slab + n);
+        float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        if (a.accumulate) {
+          const float4 p = *o;
+          v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+        }
+        *o = v;
+      } else {
+        const float v[4] = {acc[i][j][0] * f, acc[i][j][1] * f, acc[i][j][2] * f, acc[i][j][3] * f};
+        store4(a.out, m * a.ld_out + n, v, a.N - n, a.out_bf16, a.out_vec);
+      }
+    }
+  }
+}
+
+struct FinishArgs {  // out = factor * sum over the slabs, for dx and dW; db = unit * sum over the row tiles
+  const float* slab[2]; int n_slabs[2]; int64_t slab_stride[2]; int64_t rows[2]; int ld_slab; int N;
+  void* out[2]; int64_t ld_out[2]; int vec[2];
+  int out_bf16;
+  const float* db; int64_t db_ld; int db_rows, C;
+  float* dbias;
+  float gs;
+  int blk1, blk2;  // blocks [0, blk1) dx, [blk1, blk2) dW, [blk2, grid) db
+  const Scalars* scal;
+};
+
+__global__ __launch_bounds__(256) void k_lce_finish(FinishArgs a) {
+  if ((int)blockIdx.x >= a.blk2) {
+    const int c = ((int)blockIdx.x - a.blk2) * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    __shared__ float part[4][64];
+    float s = 0.f;
+    if (c < a.C)
+      for (int r = q; r < a.db_rows; r += 4) s += a.db[(int64_t)r * a.db_ld + c];
+    part[q][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (q == 0 && c < a.C) a.dbias[c] = (((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x]) * (a.scal->g_unit * a.gs);
+    return;
+  }
+  const int w = (int)blockIdx.x >= a.blk1;
+  const int64_t b = blockIdx.x - (w ? a.blk1 : 0), nb = w ? a.blk2 - a.blk1 : a.blk1;
+  const float f = grad_factor(a.scal, w);
+  const int q = a.ld_slab / 4;
+  for (int64_t e = b * 256 + threadIdx.x; e < a.rows[w] * q; e += nb * 256) {
+    const int64_t r = e / q;
+    const int n = (int)(e - r * q) * 4;
+    if (n >= a.N) continue;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < a.n_slabs[w]; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(a.slab[w] + k * a.slab_stride[w] + r * a.ld_slab + n);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+    store4(a.out[w], r * a.ld_out[w] + n, v, a.N - n, a.out_bf16, a.vec[w]);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+
+struct Layout {  // offsets into the workspace, bytes
+  size_t scal, amax, bias, xp, wp, strips, target, row, part, part_max, g, db, dx_slab, dw_slab, total;
+  int Dp, C_pad, n_strips, piece, pieces;
+  int dx_splits, dw_splits;
+  int64_t ldp, ldg;      // bytes
+  uint32_t plane, g_plane;
+  bool pack_w, dw_direct;
+  int big;               // tile size of the gradient products: 256, 128 or 64
+  int row_blocks, db_rows;
+  int tile_s, tile_g;    // LogitTile of the two sweeps (one per call: the db partials of all pieces have the same rows)
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile height and width of the logit products.  Up to 16 and 64 rows the tile is as low as the batch and 256 classes wide
+// (the weights stream past once; a taller tile would multiply rows that are not there); otherwise 256 x 256 with eight
+// waves once that gives every CU a tile, else 128 x 128 (two blocks per CU).
+enum LogitTile : int { kLow16, kLow64, kMid128, kBig256 };
+LogitTile logit_tile(int64_t n, int64_t classes) {
+  if (n <= 16) return kLow16;
+  if (n <= 64) return kLow64;
+  return ceil_div(n, 256) * ceil_div(classes, 256) >= kCUs ? kBig256 : kMid128;
+}
+
+// Splits of a product of M x N tiles over its K range: enough blocks for two per CU, at least 512 values of K each
+int splits_for(int64_t M, int64_t N, int64_t K, int tile) {
+  const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2 * kCUs, tiles), K / 512, 32}));
+}
+
+void make_layout(const suave_linear_ce_t& h, Layout& L) {
+  const bool f32 = h.dtype == SUAVE_DTYPE_F32;
+  const int np = f32 ? 2 : 1;
+  const bool grad = h.dx || h.dweight || h.dbias;
+  const int64_t n = std::max<int64_t>(h.n_rows, 1);
+  L.Dp = round_up(h.dim, 8);
+  L.C_pad = round_up(h.n_classes, kClassPad);
+  L.n_strips = (int)ceil_div(h.n_classes, kStrip);
+  L.ldp = (int64_t)L.Dp * 2 * np;
+  L.plane = (uint32_t)(L.Dp * 2);
+  L.pack_w = f32 || h.dim % 8 != 0 || h.ld_weight % 8 != 0 || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+  const int64_t per_class = n * 2 * np;
+  // (at most 2^20 classes: 256 rows of a piece lie within the 2^31 bytes a tile addresses)
+  const int64_t piece = std::min<int64_t>(1 << 20, std::max<int64_t>(kClassPad, (int64_t)(kPieceBytes / per_class) / kClassPad * kClassPad));
+  L.pieces = (int)ceil_div(L.C_pad, std::min<int64_t>(piece, L.C_pad));
+  L.piece = (int)(ceil_div(ceil_div(L.C_pad, L.pieces), kClassPad) * kClassPad);
+  L.pieces = (int)ceil_div(L.C_pad, L.piece);
+  L.ldg = (int64_t)L.piece * 2 * np;
+  L.g_plane = (uint32_t)(L.piece * 2);
+  const int64_t gt256 = ceil_div(std::min<int64_t>(L.piece, h.n_classes), 256) * ceil_div(h.dim, 256);
+  L.big = gt256 >= kCUs ? 256 : (n >= 256 || L.piece >= 1024) && h.dim > 64 ? 128 : 64;
+  const int cp = std::min(L.piece, (int)h.n_classes);
+  L.dx_splits = splits_for(n, h.dim, cp, std::min(L.big, 128));
+  L.dw_splits = L.pieces > 1 ? 1 : splits_for(cp, h.dim, n, L.big);
+  L.dw_direct = L.dw_splits == 1;
+  L.tile_s = logit_tile(n, h.n_classes);
+  L.tile_g = logit_tile(n, cp);
+  L.db_rows = L.tile_g == kBig256 ? (int)ceil_div(n, 256) * 2 : L.tile_g == kMid128 ? (int)ceil_div(n, 128) * 2 : 1;
+  L.row_blocks = (int)ceil_div(n, 16);
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
+  L.scal = take(sizeof(Scalars));
+  L.amax = take(sizeof(float) * 2 * kAmaxBlocks);
+  L.bias = take(sizeof(float) * L.C_pad);
+  L.xp = take((size_t)n * L.ldp);
+  L.wp = L.pack_w ? take((size_t)h.n_classes * L.ldp) : 0;
+  L.strips = take(sizeof(float2) * (size_t)L.n_strips * n);
+  L.target = take(sizeof(float) * n);
+  L.row = take(sizeof(float2) * n);
+  L.part = take(sizeof(double) * 2 * L.row_blocks);
+  L.part_max = take(sizeof(float) * L.row_blocks);
+  L.g = L.db = L.dx_slab = L.dw_slab = 0;
+  if (grad) {
+    L.g = take((size_t)n * L.ldg);
+    L.db = take(sizeof(float) * (size_t)L.db_rows * L.C_pad);
+    if (h.dx) L.dx_slab = take(sizeof(float) * (size_t)L.dx_splits * n * L.Dp);
+    if (h.dweight && !L.dw_direct) L.dw_slab = take(sizeof(float) * (size_t)L.dw_splits * h.n_classes * L.Dp);
+  }
+  L.total = o;
+}
+
+int check_args(const suave_linear_ce_t* h) {
+  SUAVE_REQUIRE(h != nullptr, "linear_ce: null argument");
+  SUAVE_REQUIRE(h->dtype == SUAVE_DTYPE_F32 || h->dtype == SUAVE_DTYPE_BF16, "linear_ce: dtype must be SUAVE_DTYPE_F32 or SUAVE_DTYPE_BF16");
+  SUAVE_REQUIRE(h->n_classes >= 1 && h->n_classes <= (1 << 24), "linear_ce: n_classes must be in 1..2^24");
+  SUAVE_REQUIRE(h->dim >= 1 && h->dim <= 32768, "linear_ce: dim must be in 1..32768");
+  SUAVE_REQUIRE(h->n_rows >= 0 && h->n_rows <= (1 << 24), "linear_ce: n_rows must be in 0..2^24");
+  SUAVE_REQUIRE(h->n_rows * h->n_classes <= ((int64_t)1 << 40), "linear_ce: n_rows * n_classes must be at most 2^40");
+  SUAVE_REQUIRE(h->ld_x >= h->dim && h->ld_weight >= h->dim, "linear_ce: a row stride is shorter than the row");
+  SUAVE_REQUIRE(h->ld_x <= (1 << 22) && h->ld_weight <= (1 << 22), "linear_ce: row strides of x and weight must be at most 2^22 elements");
+  SUAVE_REQUIRE(!h->dx || h->ld_dx >= h->dim, "linear_ce: ld_dx < dim");
+  SUAVE_REQUIRE(!h->dweight || h->ld_dweight >= h->dim, "linear_ce: ld_dweight < dim");
+  return 0;
+}
+
+template <class T>
+int launch_tile(const void* fn, int grid, void** args, hipStream_t s) {
+  if (T::kLds > 64 * 1024) SUAVE_CHECK_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
+  SUAVE_CHECK_HIP(hipLaunchKernel(fn, dim3(grid), dim3(T::kThreads), args, T::kLds, s));
+  return 0;
+}
+
+template <class T, int SWEEP>
+int launch_logits_tile(LogitArgs a, hipStream_t s) {
+  const int64_t grid = ceil_div(a.n, T::BM) * ceil_div(a.c1 - a.c0, T::BN);
+  a.group = 8;
+  void* args[] = {&a};
+  return launch_tile<T>(reinterpret_cast<const void*>(k_lce_logits<T, SWEEP>), (int)grid, args, s);
+}
+
+template <int TYPE, int NP, int SWEEP>
+int launch_logits(const LogitArgs& a, int tile, hipStream_t s) {
+  switch (tile) {
+    case kLow16: return launch_logits_tile<Tile<TYPE, NP, false, false, 16, 256, 1, 4, 2>, SWEEP>(a, s);
+    case kLow64: return launch_logits_tile<Tile<TYPE, NP, false, false, 64, 256, 1, 4, 2>, SWEEP>(a, s);
+    case kMid128: return launch_logits_tile<Tile<TYPE, NP, false, false, 128, 128, 2, 2, 2>, SWEEP>(a, s);
+    default: return launch_logits_tile<Tile<TYPE, NP, false, false, 256, 256, 2, 4, 2>, SWEEP>(a, s);
+  }
+}
+
+template <int TYPE, int NP, bool ACOL>
+int launch_grad(const GradArgs& g, int tile, hipStream_t s) {
+  GradArgs a = g;
+  a.group = 8;
+  void* args[] = {&a};
+  const int64_t grid = ceil_div(a.M, tile) * ceil_div(a.N, tile) * a.splits;
+  if (tile == 256) {
+    typedef Tile<TYPE, NP, ACOL, true, 256, 256, 2, 4, 2> T;
+    return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
+  } else if (tile == 128) {
+    typedef Tile<TYPE, NP, ACOL, true, 128, 128, 2, 2, 2> T;
+    return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
+  }
+  typedef Tile<TYPE, NP, ACOL, true, 64, 64, 2, 2, 2> T;
+  return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
+}
+
+template <int TYPE, int NP>
+int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
+  constexpr bool F = NP == 2;
+  const bool grad = h.dx || h.dweight || h.dbias;
+  const int64_t n = h.n_rows;
+  char* ws = static_cast<char*>(h.workspace);
+  Scalars* scal = reinterpret_cast<Scalars*>(ws + L.scal);
+  PackArgs p{};
+  p.src[0] = h.x; p.src[1] = h.weight; p.ld[0] = h.ld_x; p.ld[1] = h.ld_weight; p.rows[0] = n; p.rows[1] = h.n_classes;
+  p.dst[0] = ws + L.xp; p.dst[1] = L.pack_w ? ws + L.wp : nullptr; p.dst_ld[0] = p.dst_ld[1] = L.ldp;
+  p.D = h.dim; p.Dp = L.Dp; p.targets = h.targets; p.amax = reinterpret_cast<float*>(ws + L.amax); p.scal = scal;
+  p.bias = h.bias; p.bias_pad = reinterpret_cast<float*>(ws + L.bias); p.C = h.n_classes; p.C_pad = L.C_pad;
+  if (F) {
+    hipLaunchKernelGGL(k_lce_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, s, p);
+    SUAVE_CHECK_HIP(hipGetLastError());
+  }
+  p.blocks0 = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(n * (L.Dp / 8), 256), 1024));
+  const int64_t wblocks = L.pack_w ? ceil_div((int64_t)h.n_classes * (L.Dp / 8), 256) : ceil_div(L.C_pad, 256);
+  const int grid = p.blocks0 + (int)std::max<int64_t>(1, std::min<int64_t>(wblocks, 4096));
+  if (F) hipLaunchKernelGGL((k_lce_pack<float, true>), dim3(grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((k_lce_pack<uint16_t, false>), dim3(grid), dim3(256), 0, s, p);
+  SUAVE_CHECK_HIP(hipGetLastError());
+
+  LogitArgs a{};
+  a.x = ws + L.xp; a.ldx = L.ldp;
+  a.w = L.pack_w ? ws + L.wp : static_cast<const char*>(h.weight);
+  a.ldw = L.pack_w ? L.ldp : h.ld_weight * 2;
+  a.plane = L.plane; a.n = n; a.C = h.n_classes; a.D = h.dim; a.c0 = 0; a.c1 = h.n_classes; a.scal = scal;
+  a.bias = p.bias_pad; a.targets = h.targets;
+  a.strips = reinterpret_cast<float2*>(ws + L.strips);
+  a.target_logit = reinterpret_cast<float*>(ws + L.target);
+  a.row = reinterpret_cast<const float2*>(ws + L.row);
+  if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+
+  RowArgs r{};
+  r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
+  r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
+  r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part);
+  r.part_max = reinterpret_cast<float*>(ws + L.part_max); r.weight_sum = h.weight_sum; r.loss_scale = h.loss_scale;
+  r.loss_rows = h.loss_rows; r.gs = g_scale(F); r.loss = h.loss; r.loss_sum = h.loss_sum; r.scal = scal;
+  hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(1024), 0, s, r, L.row_blocks);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  if (!grad) return 0;
+  hipLaunchKernelGGL(k_lce_relative, dim3((int)ceil_div(n, 256)), dim3(256), 0, s, r.row, n, scal);
+  SUAVE_CHECK_HIP(hipGetLastError());
+
+  const bool bf = !F;
+  auto vec_ok = [&](const void* ptr, int64_t ld) {
+    return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) & (bf ? 7 : 15)) == 0;
+  };
+  a.g = ws + L.g; a.ldg = L.ldg; a.g_plane = L.g_plane;
+  a.db_ld = L.C_pad;
+  for (int piece = 0; piece < L.pieces; ++piece) {
+    a.c0 = piece * L.piece;
+    a.c1 = std::min(a.c0 + L.piece, (int)h.n_classes);
+    a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
+    if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
+    const int cp = a.c1 - a.c0;
+    if (h.dx) {
+      GradArgs g{};
+      g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
+      g.b = a.w + (int64_t)a.c0 * a.ldw; g.ldb = a.ldw; g.b_plane = L.plane;
+      g.M = n; g.N = h.dim; g.K = cp; g.splits = L.dx_splits;
+      g.slab = reinterpret_cast<float*>(ws + L.dx_slab); g.slab_stride = n * L.Dp; g.ld_slab = L.Dp; g.accumulate = piece > 0;
+      g.scal = scal; g.which = 0;
+      if (int rc = launch_grad<TYPE, NP, false>(g, std::min(L.big, 128), s)) return rc;
+    }
+    if (h.dweight) {
+      GradArgs g{};
+      g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
+      g.b = a.x; g.ldb = L.ldp; g.b_plane = L.plane;
+      g.M = cp; g.N = h.dim; g.K = (int)n; g.splits = L.dw_splits;
+      if (!L.dw_direct) {
+        g.slab = reinterpret_cast<float*>(ws + L.dw_slab); g.slab_stride = (int64_t)h.n_classes * L.Dp; g.ld_slab = L.Dp;
+      }
+      g.out = static_cast<char*>(h.dweight) + (int64_t)a.c0 * h.ld_dweight * (bf ? 2 : 4); g.ld_out = h.ld_dweight;
+      g.out_bf16 = bf; g.out_vec = vec_ok(h.dweight, h.ld_dweight);
+      g.scal = scal; g.which = 1;
+      if (int rc = launch_grad<TYPE, NP, true>(g, L.big, s)) return rc;
+    }
+  }
+  FinishArgs f{};
+  f.scal = scal; f.out_bf16 = bf; f.ld_slab = L.Dp; f.N = h.dim; f.gs = g_scale(F);
+  int blocks = 0;
+  if (h.dx) {
+    f.slab[0] = reinterpret_cast<float*>(ws + L.dx_slab); f.n_slabs[0] = L.dx_splits; f.slab_stride[0] = n * L.Dp; f.rows[0] = n;
+    f.out[0] = h.dx; f.ld_out[0] = h.ld_dx; f.vec[0] = vec_ok(h.dx, h.ld_dx);
+    blocks += (int)std::min<int64_t>(ceil_div(n * (L.Dp / 4), 256), 4096);
+  }
+  f.blk1 = blocks;
+  if (h.dweight && !L.dw_direct) {
+    f.slab[1] = reinterpret_cast<float*>(ws + L.dw_slab); f.n_slabs[1] = L.dw_splits; f.slab_stride[1] = (int64_t)h.n_classes * L.Dp;
+    f.rows[1] = h.n_classes; f.out[1] = h.dweight; f.ld_out[1] = h.ld_dweight; f.vec[1] = vec_ok(h.dweight, h.ld_dweight);
+    blocks += (int)std::min<int64_t>(ceil_div((int64_t)h.n_classes * (L.Dp / 4), 256), 4096);
+  }
+  f.blk2 = blocks;
+  if (h.dbias) {
+    f.db = reinterpret_cast<const float*>(ws + L.db); f.db_ld = L.C_pad; f.db_rows = L.db_rows; f.C = h.n_classes; f.dbias = h.dbias;
+    blocks += (int)ceil_div(h.n_classes, 64);
+  }
+  if (blocks > 0) {
+    hipLaunchKernelGGL(k_lce_finish, dim3(blocks), dim3(256), 0, s, f);
+    SUAVE_CHECK_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+
+int linear_ce_workspace(const suave_linear_ce_t* h, size_t* bytes) {
+  if (int rc = check_args(h)) return rc;
+  SUAVE_REQUIRE(bytes != nullptr, "linear_ce: bytes is null");
+  Layout L;
+  make_layout(*h, L);
+  *bytes = L.total;
+  return 0;
+}
+
+__global__ __launch_bounds__(256) void k_lce_empty(float* loss, float* dbias, int C, void* dweight, int64_t ld, int D, int bf16) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  if (t == 0 && loss) *loss = 0.f;
+  if (dbias)
+    for (int64_t c = t; c < C; c += step) dbias[c] = 0.f;
+  if (dweight)
+    for (int64_t e = t; e < (int64_t)C * D; e += step) {
+      const int64_t r = e / D, d = e - r * D;
+      if (bf16) static_cast<uint16_t*>(dweight)[r * ld + d] = 0;
+      else static_cast<float*>(dweight)[r * ld + d] = 0.f;
+    }
+}
+
+int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s) {
+  if (int rc = check_args(h)) return rc;
+  if (h->n_rows == 0) {  // an empty batch: loss 0, zero gradients
+    hipLaunchKernelGGL(k_lce_empty, dim3(256), dim3(256), 0, s, h->loss, h->dbias, h->n_classes, h->dweight, h->ld_dweight, h->dim,
+                       (int)(h->dtype == SUAVE_DTYPE_BF16));
+    SUAVE_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
+  SUAVE_REQUIRE(h->x && h->weight && h->targets, "linear_ce: x / weight / targets is null");
+  Layout L;
+  make_layout(*h, L);
+  SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_ce: workspace is null or not 256-byte aligned");
+  SUAVE_REQUIRE(h->workspace_bytes >= L.total, "linear_ce: workspace too small (suave_linear_ce_workspace_bytes)");
+  return h->dtype == SUAVE_DTYPE_F32 ? run_linear_ce<kF16, 2>(*h, L, s) : run_linear_ce<kBf16, 1>(*h, L, s);
+}
+
+}  // namespace suave

@@ -1,0 +1,131 @@
+"""Operators around a classifier with many classes, on device tensors: its loss and gradients without the logits
+(``linear_cross_entropy``), the orthogonalised update of hidden weight matrices (``orthogonalize``, ``muon_step``) and the
+8-bit integer product that serves the head (``quantize_rows``, ``linear_quantized``).
+
+Thin bindings of the C-ABI entry points of the same names (include/suave_hip.h): they check what the library cannot see
+(devices, dtypes, strides), run on the current stream of the tensors' device, take scratch from torch's allocator (so calls
+on different streams or in different captured graphs never share it) and never wait for the GPU.  No autograd: gradients are
+outputs.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Dict, Optional
+
+import torch
+
+from . import lib as _lib
+from .plan import LinearCeT
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # SUAVE_DTYPE_F32, SUAVE_DTYPE_BF16
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _need(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def _device_of(name: str, t: torch.Tensor) -> torch.device:
+    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise _lib.SuaveHipError(f"{name} must be on a GPU device (there is no CPU fallback)")
+    return t.device
+
+
+def _matrix(name: str, t: torch.Tensor, dev: torch.device, dtypes, shape=None) -> int:
+    """Checks a matrix whose rows are contiguous; returns its row stride in elements."""
+
+    _need(isinstance(t, torch.Tensor) and t.dim() == 2, f"{name} must be a matrix")
+    _need(t.device == dev, f"{name} must be on {dev}")
+    _need(t.dtype in dtypes, f"{name} must have one of the types {[str(d) for d in dtypes]}")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} must have the shape {shape}")
+    rows, cols = t.shape
+    _need(cols <= 1 or t.stride(1) == 1, f"{name}: the elements of a row must be contiguous")
+    ld = int(t.stride(0)) if rows > 1 else max(int(cols), 1)
+    _need(ld >= cols, f"{name}: rows must not overlap")
+    return ld
+
+
+def _vector(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype, n: int) -> None:
+    _need(isinstance(t, torch.Tensor) and t.dim() == 1 and int(t.shape[0]) == n, f"{name} must be a vector of {n} values")
+    _need(t.device == dev, f"{name} must be on {dev}")
+    _need(t.dtype == dtype, f"{name} must have the type {dtype}")
+    _need(n <= 1 or t.stride(0) == 1, f"{name} must be contiguous")
+
+
+def _scalar(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
+    _need(isinstance(t, torch.Tensor) and t.numel() == 1 and t.device == dev and t.dtype == dtype,
+          f"{name} must be one {dtype} value on {dev}")
+
+
+def _workspace(nbytes: int, dev: torch.device):
+    """(tensor, aligned address, bytes) of per-call scratch."""
+
+    ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)
+    base = (ws.data_ptr() + 255) // 256 * 256
+    return ws, base, nbytes
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                         class_weight: Optional[torch.Tensor] = None, weight_sum: Optional[torch.Tensor] = None,
+                         loss_scale: float = 1.0, grad: bool = True, dx: Optional[torch.Tensor] = None,
+                         dweight: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None,
+                         loss_sum: Optional[torch.Tensor] = None, loss_rows: float = 1.0) -> Dict[str, torch.Tensor]:
+    """Class-weighted softmax cross entropy of ``x @ weight.T + bias`` against ``targets`` and its gradients
+    (``suave_linear_ce``): what ``ClassificationHead.loss(linear(x), targets)`` and its backward give, without the
+    ``[rows, classes]`` logits.
+
+    ``x`` [rows, dim], ``weight`` [classes, dim]: float32 or bfloat16, rows contiguous, any row stride.  ``targets`` int32;
+    a negative one leaves its row out, one beyond the classes makes the loss NaN.  ``weight_sum`` (one float32 value on the
+    device) replaces the sum of the rows' class weights (data parallelism: that of the global batch).  Returns ``loss``
+    (float32 scalar), ``row_loss`` [rows] (weighted, not divided), ``lse`` [rows] and, with ``grad``, ``dx``, ``dweight``
+    (types of ``x`` / ``weight``) and ``dbias`` (float32), all multiplied by ``loss_scale``; buffers for them may be given.
+    ``loss_sum`` (float64) += loss * ``loss_rows``."""
+
+    dev = _device_of("x", x)
+    ld_x = _matrix("x", x, dev, tuple(_DTYPES))
+    n, d = int(x.shape[0]), int(x.shape[1])
+    ld_w = _matrix("weight", weight, dev, (x.dtype,))
+    c = int(weight.shape[0])
+    _need(int(weight.shape[1]) == d, f"weight must have {d} columns, as x")
+    _need(c >= 1 and d >= 1, "weight must have at least one row and one column")
+    _vector("targets", targets, dev, torch.int32, n)
+    if bias is not None:
+        _vector("bias", bias, dev, torch.float32, c)
+    if class_weight is not None:
+        _vector("class_weight", class_weight, dev, torch.float32, c)
+    if weight_sum is not None:
+        _scalar("weight_sum", weight_sum, dev, torch.float32)
+    if loss_sum is not None:
+        _scalar("loss_sum", loss_sum, dev, torch.float64)
+    with torch.cuda.device(dev):
+        out = {"loss": torch.empty((), dtype=torch.float32, device=dev),
+               "row_loss": torch.empty(n, dtype=torch.float32, device=dev), "lse": torch.empty(n, dtype=torch.float32, device=dev)}
+        h = LinearCeT()
+        if grad:
+            out["dx"] = torch.empty((n, d), dtype=x.dtype, device=dev) if dx is None else dx
+            out["dweight"] = torch.empty((c, d), dtype=x.dtype, device=dev) if dweight is None else dweight
+            out["dbias"] = torch.empty(c, dtype=torch.float32, device=dev) if dbias is None else dbias
+            h.ld_dx = _matrix("dx", out["dx"], dev, (x.dtype,), (n, d))
+            h.ld_dweight = _matrix("dweight", out["dweight"], dev, (x.dtype,), (c, d))
+            _vector("dbias", out["dbias"], dev, torch.float32, c)
+            h.dx, h.dweight, h.dbias = (out[k].data_ptr() for k in ("dx", "dweight", "dbias"))
+        else:
+            _need(dx is None and dweight is None and dbias is None, "gradient buffers are given, but grad is False")
+        h.dtype, h.n_classes, h.dim, h.n_rows = _DTYPES[x.dtype], c, d, n
+        h.x, h.ld_x, h.weight, h.ld_weight = x.data_ptr(), ld_x, weight.data_ptr(), ld_w
+        h.bias, h.targets, h.class_weight, h.weight_sum = _ptr(bias), targets.data_ptr(), _ptr(class_weight), _ptr(weight_sum)
+        h.loss_scale, h.loss_rows = float(loss_scale), float(loss_rows)
+        h.loss, h.loss_sum = out["loss"].data_ptr(), _ptr(loss_sum)
+        h.row_loss, h.lse = out["row_loss"].data_ptr(), out["lse"].data_ptr()
+        lib = _lib.load()
+        nbytes = C.c_size_t(0)
+        _lib.check(lib.suave_linear_ce_workspace_bytes(C.byref(h), C.byref(nbytes)), "suave_linear_ce_workspace_bytes")
+        ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
+        _lib.check(lib.suave_linear_ce(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_ce")
+    return out

@@ -74,6 +74,15 @@ class HeadT(C.Structure):  # suave_head_t
                 ("adam_v", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class LinearCeT(C.Structure):  # suave_linear_ce_t
+    _fields_ = [("dtype", C.c_int32), ("n_classes", C.c_int32), ("dim", C.c_int32), ("n_rows", C.c_int64), ("x", C.c_void_p),
+                ("ld_x", C.c_int64), ("weight", C.c_void_p), ("ld_weight", C.c_int64), ("bias", C.c_void_p),
+                ("targets", C.c_void_p), ("class_weight", C.c_void_p), ("weight_sum", C.c_void_p), ("loss_scale", C.c_float),
+                ("loss_rows", C.c_float), ("loss", C.c_void_p), ("loss_sum", C.c_void_p), ("row_loss", C.c_void_p),
+                ("lse", C.c_void_p), ("dx", C.c_void_p), ("ld_dx", C.c_int64), ("dweight", C.c_void_p),
+                ("ld_dweight", C.c_int64), ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 def _r4(x: int) -> int:
     return (x + 3) // 4 * 4
 
