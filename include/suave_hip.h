@@ -314,6 +314,37 @@ typedef struct suave_linear_ce_t {
 int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes);
 int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
 
+/* 8-bit rows with one scale each: scale[r] = max |x_r| / 127 (binary32), q[r, k] = x[r, k] / scale[r] rounded to the
+ * nearest integer, ties to even, exactly.  A row of zeros has scale 0; a row with an infinity or a NaN has a non-finite
+ * scale and q = 0.  q: 16-byte aligned, ld_q a multiple of 16; the bytes of a row from cols to the next multiple of 16
+ * are written as zero.  Strides in elements. */
+int suave_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,
+                        float* scale, void* stream);
+
+/* Serving form of a linear layer (the classifier's `linear`, heads.py:62-91): out[r, n] = s_r weight_scale[n]
+ * sum_k q[r, k] weight[n, k] + bias[n], where q, s are suave_quantize_rows of x, made in the call.  The sums are exact in
+ * 32 bits.  x and out have the type dtype; weight: 16-byte aligned, ld_weight a multiple of 16 (suave_quantize_rows of the
+ * layer's rows; the bytes of a row from n_in to the next multiple of 16 are read, and do not matter).
+ * A row of x with an infinity or a NaN gives NaN.  workspace: 256-byte aligned. */
+typedef struct suave_linear_quantized_t {
+  int32_t dtype;
+  int32_t n_out;
+  int32_t n_in;
+  int64_t n_rows;
+  const void* x;             /* [n_rows, ld_x] */
+  int64_t ld_x;
+  const int8_t* weight;      /* [n_out, ld_weight] */
+  int64_t ld_weight;
+  const float* weight_scale; /* [n_out] */
+  const float* bias;         /* [n_out] or NULL */
+  void* out;                 /* [n_rows, ld_out] */
+  int64_t ld_out;
+  void* workspace;
+  size_t workspace_bytes;
+} suave_linear_quantized_t;
+int suave_linear_quantized_workspace_bytes(const suave_linear_quantized_t* call, size_t* bytes);
+int suave_linear_quantized(const suave_linear_quantized_t* call, void* stream);
+
 /* Decoder.forward's per-column log-likelihoods at a GIVEN latent (decoder.py:333-379 as called by the reference's
  * decode-side code and tests): y_full = trunk(z), then every head scores the batch's cells with the row's
  * component as the assignment one-hot.  log_px / log_px_missing: [n, n_cols], laid out as the fields of that name in the ELBO output struct (either may

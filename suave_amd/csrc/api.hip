@@ -1442,6 +1442,21 @@ extern "C" int suave_linear_ce(const suave_linear_ce_t* call, void* stream) {
   return suave::launch_linear_ce(call, static_cast<hipStream_t>(stream));
 }
 
+extern "C" int suave_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,
+                                   float* scale, void* stream) {
+  suave::drop_stale_hip_error();
+  return suave::launch_quantize_rows(x, dtype, rows, cols, ld_x, q, ld_q, scale, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int suave_linear_quantized_workspace_bytes(const suave_linear_quantized_t* call, size_t* bytes) {
+  return suave::linear_quantized_workspace(call, bytes);
+}
+
+extern "C" int suave_linear_quantized(const suave_linear_quantized_t* call, void* stream) {
+  suave::drop_stale_hip_error();
+  return suave::launch_linear_quantized(call, static_cast<hipStream_t>(stream));
+}
+
 extern "C" int suave_encode(const suave_plan* p, const float* params, const suave_batch_t* batch,
                             float inv_temperature, void* workspace, size_t workspace_bytes, void* stream,
                             float* enc_out, float* post_mean, float* post_logvar, float* probs) {

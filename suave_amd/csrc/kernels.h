@@ -300,4 +300,10 @@ int launch_head_loss(const suave_head_t& h, int D, const float* latent, int ld, 
 int linear_ce_workspace(const suave_linear_ce_t* h, size_t* bytes);
 int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s);
 
+// ----- 8-bit integer product (quant.hip) ------------------------------------------
+int launch_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
+                         hipStream_t s);
+int linear_quantized_workspace(const suave_linear_quantized_t* h, size_t* bytes);
+int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s);
+
 }  // namespace suave

@@ -1,0 +1,358 @@
+// Matrix product in 8-bit integers with a scale per row of either operand (per token and per output channel): the serving
+// form of a linear layer.
+//
+//   s_r = max_k |x_rk| / 127     q_rk = rint(x_rk / s_r)     out_rn = s_r w_n sum_k q_rk Q_nk + b_n
+//
+// k_quantize_rows writes q and s.  The scale is the correctly rounded binary32 quotient and q the exact nearest integer of
+// x / s (ties to even): the quotient by the reciprocal decides except next to a half-integer, where the sign of the exactly
+// rounded x - (q +- 1/2) s does; so q does not depend on how the division is evaluated.  A row of zeros has scale 0, a row
+// that holds an infinity or a NaN gets that as its scale and q = 0: its outputs are NaN.
+//
+// The sums are exact int32 (127^2 * 2^17 < 2^31).  Two kernels, by the number of rows:
+//  * up to 64 rows the call is bound by reading Q once: k_linear_rows.  A block owns 64 channels, its four waves a quarter of
+//    K each; a wave loads the 16 x 64 byte fragments of Q straight into registers (no LDS: nothing is reused) and those of q
+//    through L2; the four partial sums meet in LDS.
+//  * above, the tile product of mma.h (K step 128, 256 x 256 or 128 x 128 tiles), bound by the matrix pipe.
+#include <algorithm>
+#include <cmath>
+
+#include "kernels.h"
+#include "mma.h"
+
+namespace suave {
+
+namespace {
+
+using namespace mma;
+
+struct QuantArgs {
+  const void* x;
+  int64_t ld;
+  int64_t rows;
+  int cols;
+  int8_t* q;
+  int64_t ldq;
+  float* scale;
+  int vec;  // rows may be read 16 bytes at a time
+};
+
+__device__ __forceinline__ int quantize_one(float x, float s, float inv) {
+  const float k = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
+  const float up = fmaf(-(k + 0.5f), s, x), down = fmaf(-(k - 0.5f), s, x);  // signs are exact: one rounding each
+  const int ki = (int)k;
+  const int odd = ki & 1;
+  int r = ki;
+  if (up > 0.f || (up == 0.f && odd)) r = ki + 1;
+  if (down < 0.f || (down == 0.f && odd)) r = ki - 1;
+  return min(max(r, -127), 127);
+}
+// scales next to or below binary32's smallest normal number: the reciprocal or the residuals above may leave the range
+__device__ __forceinline__ int quantize_tiny(float x, float s) {
+  if (!(s > 0.f)) return 0;
+  return (int)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0);
+}
+
+template <class T> __device__ __forceinline__ float as_float(T v);
+template <> __device__ __forceinline__ float as_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float as_float<uint16_t>(uint16_t v) { return bf16_value(v); }
+
+template <class T>
+__device__ __forceinline__ void load16(const T* row, int k0, int cols, int vec, float (&v)[16]) {  // zeros past the row
+  if (vec && k0 + 16 <= cols) {
+    constexpr int per = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / per; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row + k0 + i * per);
+      const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < per; ++j) v[i * per + j] = as_float<T>(t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = k0 + i < cols ? as_float<T>(row[k0 + i]) : 0.f;
+  }
+}
+
+// W waves share a row: 16 values per lane and pass; the first pass's values stay in registers, rows beyond are read twice
+template <class T, int W>
+__global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
+  __shared__ uint32_t part[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  const int t = (wave % W) * 64 + lane;
+  const bool in = r < a.rows;
+  const T* row = static_cast<const T*>(a.x) + (in ? r : 0) * a.ld;
+  float v[16];
+  load16<T>(row, t * 16, a.cols, a.vec, v);
+  // |x| as an integer: monotonic, infinity above every number and NaN above infinity, so neither is lost in the maximum
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int k0 = (t + W * 64) * 16; k0 < a.cols; k0 += W * 64 * 16) {
+    float u[16];
+    load16<T>(row, k0, a.cols, a.vec, u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(u[i]) & 0x7fffffffu);
+  }
+  for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+  if constexpr (W > 1) {
+    if (lane == 0) part[wave] = mx;
+    __syncthreads();
+    const int w0 = wave / W * W;
+#pragma unroll
+    for (int i = 0; i < W; ++i) mx = max(mx, part[w0 + i]);
+  }
+  if (!in) return;
+  const float s = __fdiv_rn(__uint_as_float(mx), 127.0f);
+  if (t == 0) a.scale[r] = s;
+  const bool finite = mx < 0x7f800000u, tiny = s < 1e-30f;
+  const float inv = 1.0f / s;
+  const int end = (a.cols + 15) / 16 * 16;
+  for (int k0 = t * 16; k0 < end; k0 += W * 64 * 16) {
+    if (k0 != t * 16) load16<T>(row, k0, a.cols, a.vec, v);
+    int8_t o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = (int8_t)(!finite ? 0 : tiny ? quantize_tiny(v[i], s) : quantize_one(v[i], s, inv));
+    *reinterpret_cast<uint4*>(a.q + r * a.ldq + k0) = *reinterpret_cast<const uint4*>(o);
+  }
+}
+
+struct ProductArgs {
+  const int8_t* x; int64_t ldx;   // quantised rows [M][ldx], zero from K to the next multiple of 16
+  const float* xs;
+  const int8_t* w; int64_t ldw;
+  const float* ws;
+  const float* bias;
+  int64_t M;
+  int N, K;
+  void* out; int64_t ld_out;
+  int bf16, vec;
+  int group;
+};
+
+__device__ __forceinline__ void store_out(const ProductArgs& a, int64_t m, int n, const float (&v)[4]) {
+  if (a.bf16) {
+    uint16_t* o = static_cast<uint16_t*>(a.out) + m * a.ld_out + n;
+    uint16_t h[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) h[u] = bf16_bits(v[u]);
+    if (a.vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(h);
+    else
+      for (int u = 0; u < 4; ++u)
+        if (n + u < a.N) o[u] = h[u];
+  } else {
+    float* o = static_cast<float*>(a.out) + m * a.ld_out + n;
+    if (a.vec && n + 4 <= a.N) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      for (int u = 0; u < 4; ++u)
+        if (n + u < a.N) o[u] = v[u];
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void k_linear_tile(ProductArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tiles_m = (int)((a.M + T::BM - 1) / T::BM), tiles_n = (a.N + T::BN - 1) / T::BN;
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, a.group, tm, tn);
+  const int64_t m_base = (int64_t)tm * T::BM;
+  const int n_base = tn * T::BN;
+  const Operand A{reinterpret_cast<const char*>(a.x) + m_base * a.ldx, (uint32_t)a.ldx, (int)min<int64_t>(T::BM, a.M - m_base), 0};
+  const Operand B{reinterpret_cast<const char*>(a.w) + (int64_t)n_base * a.ldw, (uint32_t)a.ldw, a.N - n_base, 0};
+  typename T::acc_t acc[T::MI][T::NI];
+  T::run(lds, A, B, a.K, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  float sw[T::NI][4], b[T::NI][4];
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int n = n_base + wn * (T::NI * 16) + 16 * j + 4 * (lane >> 4) + u;
+      sw[j][u] = n < a.N ? a.ws[n] : 0.f;
+      b[j][u] = n < a.N && a.bias ? a.bias[n] : 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i) {
+    const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
+    if (m >= a.M) continue;
+    const float sx = a.xs[m];
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const int n = n_base + wn * (T::NI * 16) + 16 * j + 4 * (lane >> 4);
+      if (n >= a.N) continue;
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = fmaf((float)acc[i][j][u], sx * sw[j][u], b[j][u]);
+      store_out(a, m, n, v);
+    }
+  }
+}
+
+constexpr int kRowChannels = 64;
+
+// MT x 16 rows at most, 64 channels per block
+template <int MT>
+__global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a) {
+  __shared__ int part[4][4][MT * 4 * 64];  // [wave][channel tile][MT x 4 accumulators x lane]
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * kRowChannels;
+  const int chunks = (a.K + 15) / 16;                     // 16-byte chunks of a row
+  const int steps = (chunks + 3) / 4;                     // 64 bytes of K each
+  const int per = (steps + 3) / 4;
+  const int s0 = min(wave * per, steps), s1 = min(s0 + per, steps);
+  const int8_t* wp[4];
+  const int8_t* xp[MT];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) wp[j] = a.w + (int64_t)min(n0 + 16 * j + r, a.N - 1) * a.ldw;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xp[i] = a.x + min<int64_t>(16 * i + r, a.M - 1) * a.ldx;
+  i32x4 acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  constexpr int U = MT == 1 ? 8 : 4;  // K steps in flight
+  for (int s = s0; s < s1; s += U) {
+    i32x4 w[U][4], x[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = (s + u) * 4 + g;
+      const bool in = s + u < s1 && c < chunks;           // past the row: q is taken as zero, so whatever Q gives does not count
+      const int64_t off = (int64_t)(in ? c : 0) * 16;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[u][j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp[j] + off));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        x[u][i] = *reinterpret_cast<const i32x4*>(xp[i] + off);
+        if (!in) x[u][i] = i32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mul<kI8>(w[u][j], x[u][i], acc[i][j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) part[wave][j][(i * 4 + u) * 64 + lane] = acc[i][j][u];
+  __syncthreads();
+  // wave j finishes channel tile j
+  const int n = n0 + 16 * wave + 4 * g;
+  if (n >= a.N) return;
+  float sw[4], b[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    sw[u] = n + u < a.N ? a.ws[n + u] : 0.f;
+    b[u] = n + u < a.N && a.bias ? a.bias[n + u] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = 16 * i + r;
+    if (m >= a.M) continue;
+    const float sx = a.xs[m];
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = (i * 4 + u) * 64 + lane;
+      const int sum = (part[0][wave][e] + part[1][wave][e]) + (part[2][wave][e] + part[3][wave][e]);
+      v[u] = fmaf((float)sum, sx * sw[u], b[u]);
+    }
+    store_out(a, m, n, v);
+  }
+}
+
+template <class T>
+int launch_tile(ProductArgs a, hipStream_t s) {
+  const int64_t grid = (a.M + T::BM - 1) / T::BM * ((a.N + T::BN - 1) / T::BN);
+  a.group = 8;
+  if (T::kLds > 64 * 1024)
+    SUAVE_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_tile<T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
+  hipLaunchKernelGGL(k_linear_tile<T>, dim3((unsigned)grid), dim3(T::kThreads), T::kLds, s, a);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <class T>
+void launch_quantize(const QuantArgs& a, hipStream_t s) {
+  // a wave per row up to 2048 columns (two passes of 1024), then four
+  if (a.cols <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_quantize_rows<T, 4>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+int check_call(const suave_linear_quantized_t* h) {
+  SUAVE_REQUIRE(h != nullptr, "linear_quantized: null argument");
+  SUAVE_REQUIRE(h->dtype == SUAVE_DTYPE_F32 || h->dtype == SUAVE_DTYPE_BF16, "linear_quantized: dtype must be SUAVE_DTYPE_F32 or SUAVE_DTYPE_BF16");
+  SUAVE_REQUIRE(h->n_rows >= 0 && h->n_rows <= (1 << 24), "linear_quantized: n_rows must be in 0..2^24");
+  SUAVE_REQUIRE(h->n_in >= 1 && h->n_in <= 131072, "linear_quantized: n_in must be in 1..131072 (exact 32-bit sums)");
+  SUAVE_REQUIRE(h->n_out >= 1 && h->n_out <= (1 << 24), "linear_quantized: n_out must be in 1..2^24");
+  SUAVE_REQUIRE(h->n_rows * h->n_out <= ((int64_t)1 << 40), "linear_quantized: n_rows * n_out must be at most 2^40");
+  SUAVE_REQUIRE(h->ld_x >= h->n_in && h->ld_out >= h->n_out, "linear_quantized: a row stride is shorter than the row");
+  SUAVE_REQUIRE(h->ld_weight >= h->n_in && h->ld_weight % 16 == 0 && h->ld_weight <= (1 << 22),
+                "linear_quantized: ld_weight must be a multiple of 16, at least n_in and at most 2^22");
+  return 0;
+}
+
+}  // namespace
+
+int launch_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
+                         hipStream_t s) {
+  SUAVE_REQUIRE(dtype == SUAVE_DTYPE_F32 || dtype == SUAVE_DTYPE_BF16, "quantize_rows: dtype must be SUAVE_DTYPE_F32 or SUAVE_DTYPE_BF16");
+  SUAVE_REQUIRE(rows >= 0 && rows <= (1 << 30), "quantize_rows: rows must be in 0..2^30");
+  SUAVE_REQUIRE(cols >= 1 && cols <= (1 << 24), "quantize_rows: cols must be in 1..2^24");
+  SUAVE_REQUIRE(ld_x >= cols, "quantize_rows: ld_x < cols");
+  SUAVE_REQUIRE(ld_q % 16 == 0 && ld_q >= cols, "quantize_rows: ld_q must be a multiple of 16 and at least cols");
+  if (rows == 0) return 0;
+  SUAVE_REQUIRE(x && q && scale, "quantize_rows: x / q / scale is null");
+  SUAVE_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0, "quantize_rows: q must be 16-byte aligned");
+  QuantArgs a{x, ld_x, rows, cols, q, ld_q, scale, 0};
+  const int es = dtype == SUAVE_DTYPE_BF16 ? 2 : 4;
+  a.vec = (ld_x * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  if (dtype == SUAVE_DTYPE_BF16) launch_quantize<uint16_t>(a, s);
+  else launch_quantize<float>(a, s);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+int linear_quantized_workspace(const suave_linear_quantized_t* h, size_t* bytes) {
+  if (int rc = check_call(h)) return rc;
+  SUAVE_REQUIRE(bytes != nullptr, "linear_quantized: bytes is null");
+  *bytes = up256((size_t)h->n_rows * round_up(h->n_in, 16)) + up256(sizeof(float) * h->n_rows);
+  return 0;
+}
+
+int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
+  size_t need = 0;
+  if (int rc = linear_quantized_workspace(h, &need)) return rc;
+  if (h->n_rows == 0) return 0;
+  SUAVE_REQUIRE(h->x && h->weight && h->weight_scale && h->out, "linear_quantized: x / weight / weight_scale / out is null");
+  SUAVE_REQUIRE((reinterpret_cast<uintptr_t>(h->weight) & 15) == 0, "linear_quantized: weight must be 16-byte aligned");
+  SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_quantized: workspace is null or not 256-byte aligned");
+  SUAVE_REQUIRE(h->workspace_bytes >= need, "linear_quantized: workspace too small (suave_linear_quantized_workspace_bytes)");
+  const int ldq = round_up(h->n_in, 16);
+  int8_t* q = static_cast<int8_t*>(h->workspace);
+  float* xs = reinterpret_cast<float*>(q + up256((size_t)h->n_rows * ldq));
+  if (int rc = launch_quantize_rows(h->x, h->dtype, h->n_rows, h->n_in, h->ld_x, q, ldq, xs, s)) return rc;
+  ProductArgs a{};
+  a.x = q; a.ldx = ldq; a.xs = xs; a.w = h->weight; a.ldw = h->ld_weight; a.ws = h->weight_scale; a.bias = h->bias;
+  a.M = h->n_rows; a.N = h->n_out; a.K = h->n_in; a.out = h->out; a.ld_out = h->ld_out; a.bf16 = h->dtype == SUAVE_DTYPE_BF16;
+  a.vec = h->ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(h->out) & (a.bf16 ? 7 : 15)) == 0;
+  const unsigned blocks = (unsigned)((h->n_out + kRowChannels - 1) / kRowChannels);
+  if (a.M <= 16) hipLaunchKernelGGL(k_linear_rows<1>, dim3(blocks), dim3(256), 0, s, a);
+  else if (a.M <= 32) hipLaunchKernelGGL(k_linear_rows<2>, dim3(blocks), dim3(256), 0, s, a);
+  else if (a.M <= 64) hipLaunchKernelGGL(k_linear_rows<4>, dim3(blocks), dim3(256), 0, s, a);
+  else if ((a.M + 255) / 256 * ((a.N + 255) / 256) >= 256) return launch_tile<Tile<kI8, 1, false, false, 256, 256, 2, 4, 2>>(a, s);
+  else return launch_tile<Tile<kI8, 1, false, false, 128, 128, 2, 2, 2>>(a, s);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+}  // namespace suave

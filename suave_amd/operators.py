@@ -11,12 +11,12 @@ outputs.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Optional
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import lib as _lib
-from .plan import LinearCeT
+from .plan import LinearCeT, LinearQuantizedT
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # SUAVE_DTYPE_F32, SUAVE_DTYPE_BF16
 
@@ -128,4 +128,59 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         _lib.check(lib.suave_linear_ce_workspace_bytes(C.byref(h), C.byref(nbytes)), "suave_linear_ce_workspace_bytes")
         ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
         _lib.check(lib.suave_linear_ce(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_ce")
+    return out
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x`` [rows, cols] (float32 / bfloat16) in 8 bits with one scale per row (``suave_quantize_rows``): ``(q, scale)``
+    with ``q`` int8 [rows, cols], the nearest integers of ``x / scale`` (rows start at multiples of 16 bytes), and ``scale``
+    float32 [rows] = max |x| / 127.  The form ``linear_quantized`` takes a layer's weight in."""
+
+    dev = _device_of("x", x)
+    ld = _matrix("x", x, dev, tuple(_DTYPES))
+    n, k = int(x.shape[0]), int(x.shape[1])
+    _need(k >= 1, "x must have at least one column")
+    with torch.cuda.device(dev):
+        q = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.int8, device=dev)
+        scale = torch.empty(n, dtype=torch.float32, device=dev)
+        _lib.check(_lib.load().suave_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], n, k, ld, q.data_ptr(), int(q.shape[1]),
+                                                   scale.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "suave_quantize_rows")
+    return q[:, :k], scale
+
+
+def linear_quantized(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ (weight * weight_scale[:, None]).T + bias`` with ``x`` quantised per row in the call and exact integer sums
+    (``suave_linear_quantized``).  ``x`` [rows, in] float32 / bfloat16 and the result [rows, out] of the same type;
+    ``weight`` int8 [out, in] and ``weight_scale`` float32 [out] as ``quantize_rows`` gives them: rows 16-byte aligned, a
+    row stride that is a multiple of 16."""
+
+    dev = _device_of("x", x)
+    ld = _matrix("x", x, dev, tuple(_DTYPES))
+    n, k = int(x.shape[0]), int(x.shape[1])
+    ldw = _matrix("weight", weight, dev, (torch.int8,))
+    c = int(weight.shape[0])
+    _need(int(weight.shape[1]) == k, f"weight must have {k} columns, as x")
+    _need(c >= 1 and k >= 1, "weight must have at least one row and one column")
+    if c == 1:
+        ldw = (k + 15) // 16 * 16
+    _need(ldw % 16 == 0 and weight.data_ptr() % 16 == 0, "weight: rows must start at multiples of 16 bytes (quantize_rows)")
+    held = weight.untyped_storage().nbytes() - weight.storage_offset()
+    _need(held >= (c - 1) * ldw + (k + 15) // 16 * 16, "weight: the last row must be held up to a multiple of 16 (quantize_rows)")
+    _vector("weight_scale", weight_scale, dev, torch.float32, c)
+    if bias is not None:
+        _vector("bias", bias, dev, torch.float32, c)
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty((n, c), dtype=x.dtype, device=dev)
+        h = LinearQuantizedT()
+        h.ld_out = _matrix("out", out, dev, (x.dtype,), (n, c))
+        h.dtype, h.n_out, h.n_in, h.n_rows = _DTYPES[x.dtype], c, k, n
+        h.x, h.ld_x, h.weight, h.ld_weight = x.data_ptr(), ld, weight.data_ptr(), ldw
+        h.weight_scale, h.bias, h.out = weight_scale.data_ptr(), _ptr(bias), out.data_ptr()
+        lib = _lib.load()
+        nbytes = C.c_size_t(0)
+        _lib.check(lib.suave_linear_quantized_workspace_bytes(C.byref(h), C.byref(nbytes)), "suave_linear_quantized_workspace_bytes")
+        ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
+        _lib.check(lib.suave_linear_quantized(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_quantized")
     return out

@@ -83,6 +83,13 @@ class LinearCeT(C.Structure):  # suave_linear_ce_t
                 ("ld_dweight", C.c_int64), ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class LinearQuantizedT(C.Structure):  # suave_linear_quantized_t
+    _fields_ = [("dtype", C.c_int32), ("n_out", C.c_int32), ("n_in", C.c_int32), ("n_rows", C.c_int64), ("x", C.c_void_p),
+                ("ld_x", C.c_int64), ("weight", C.c_void_p), ("ld_weight", C.c_int64), ("weight_scale", C.c_void_p),
+                ("bias", C.c_void_p), ("out", C.c_void_p), ("ld_out", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 def _r4(x: int) -> int:
     return (x + 3) // 4 * 4
 
