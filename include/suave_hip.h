@@ -345,6 +345,45 @@ typedef struct suave_linear_quantized_t {
 int suave_linear_quantized_workspace_bytes(const suave_linear_quantized_t* call, size_t* bytes);
 int suave_linear_quantized(const suave_linear_quantized_t* call, void* stream);
 
+/* Orthogonalisation of matrices by Newton-Schulz products: X = U / (|U|_F + eps), then `steps` times
+ * X <- (a I + b A + c A A) X with A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315), on the shorter side; after five steps
+ * the singular values of the result lie in about 0.7 .. 1.2 where U's were not negligible.  All matrices of the list go
+ * through the same launches.  in / out have the type dtype and may be the same matrix, otherwise they must not overlap;
+ * rows contiguous, strides in elements.  F32: binary32-grade products; BF16: fp16 products with fp32 sums.  A zero matrix
+ * gives zero; an infinity or a NaN makes its whole matrix NaN.  Sides at most 32768 (short) and 2^20 (long).  The list is
+ * host memory and is read before the call returns.  workspace: 256-byte aligned; one call at a time uses it. */
+typedef struct suave_ortho_matrix_t {
+  const void* in;
+  void* out;
+  int64_t ld_in;
+  int64_t ld_out;
+  int32_t rows;
+  int32_t cols;
+} suave_ortho_matrix_t;
+int suave_orthogonalize_workspace_bytes(const suave_ortho_matrix_t* matrices_host, int32_t n_matrices, int32_t dtype,
+                                        size_t* bytes);
+int suave_orthogonalize(const suave_ortho_matrix_t* matrices_host, int32_t n_matrices, int32_t dtype, int32_t steps, float eps,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* One Muon step on a list of float32 weight matrices (hidden layers; biases and the rest stay with suave_adam_step):
+ *   momentum <- mu momentum + grad;   U = nesterov ? grad + mu momentum : momentum
+ *   param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) orthogonalize(U)
+ * param and momentum are updated in place; no matrix of the list may overlap another. */
+typedef struct suave_muon_matrix_t {
+  float* param;
+  const float* grad;
+  float* momentum;
+  int64_t ld_param;
+  int64_t ld_grad;
+  int64_t ld_momentum;
+  int32_t rows;
+  int32_t cols;
+  float lr;
+} suave_muon_matrix_t;
+int suave_muon_workspace_bytes(const suave_muon_matrix_t* matrices_host, int32_t n_matrices, size_t* bytes);
+int suave_muon_step(const suave_muon_matrix_t* matrices_host, int32_t n_matrices, float momentum, int32_t nesterov,
+                    float weight_decay, int32_t steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Decoder.forward's per-column log-likelihoods at a GIVEN latent (decoder.py:333-379 as called by the reference's
  * decode-side code and tests): y_full = trunk(z), then every head scores the batch's cells with the row's
  * component as the assignment one-hot.  log_px / log_px_missing: [n, n_cols], laid out as the fields of that name in the ELBO output struct (either may

@@ -1457,6 +1457,26 @@ extern "C" int suave_linear_quantized(const suave_linear_quantized_t* call, void
   return suave::launch_linear_quantized(call, static_cast<hipStream_t>(stream));
 }
 
+extern "C" int suave_orthogonalize_workspace_bytes(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, size_t* bytes) {
+  return suave::orthogonalize_workspace(mats, n, dtype, bytes);
+}
+
+extern "C" int suave_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, int32_t steps, float eps, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  suave::drop_stale_hip_error();
+  return suave::launch_orthogonalize(mats, n, dtype, steps, eps, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int suave_muon_workspace_bytes(const suave_muon_matrix_t* mats, int32_t n, size_t* bytes) {
+  return suave::muon_workspace(mats, n, bytes);
+}
+
+extern "C" int suave_muon_step(const suave_muon_matrix_t* mats, int32_t n, float momentum, int32_t nesterov, float weight_decay, int32_t steps,
+                               float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  suave::drop_stale_hip_error();
+  return suave::launch_muon(mats, n, momentum, nesterov, weight_decay, steps, eps, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
 extern "C" int suave_encode(const suave_plan* p, const float* params, const suave_batch_t* batch,
                             float inv_temperature, void* workspace, size_t workspace_bytes, void* stream,
                             float* enc_out, float* post_mean, float* post_logvar, float* probs) {

@@ -8,7 +8,7 @@ mkdir -p "$OBJ"
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops $SUAVE_EXTRA_FLAGS"
 pids=()
-for f in gemm decode loss wide embed latent optim sample frame head lce quant api; do
+for f in gemm decode loss wide embed latent optim sample frame head lce quant ortho api; do
   [ -f $f.hip ] || continue
   stale=0  # an object is rebuilt when its source, ANY header here or under include/, or this script is newer
   for dep in $f.hip *.h ../../include/*.h build.sh; do
@@ -24,6 +24,6 @@ for f in gemm decode loss wide embed latent optim sample frame head lce quant ap
 done
 for p in "${pids[@]}"; do wait $p; done
 objs=""
-for f in gemm decode loss wide embed latent optim sample frame head lce quant api; do [ -f $OBJ/$f.o ] && objs="$objs $OBJ/$f.o"; done
+for f in gemm decode loss wide embed latent optim sample frame head lce quant ortho api; do [ -f $OBJ/$f.o ] && objs="$objs $OBJ/$f.o"; done
 hipcc --offload-arch=gfx950 -shared -fPIC $objs -o $OUT
 echo "built $(realpath $OUT)"

@@ -306,4 +306,12 @@ int launch_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t col
 int linear_quantized_workspace(const suave_linear_quantized_t* h, size_t* bytes);
 int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s);
 
+// ----- orthogonalised updates (ortho.hip) -----------------------------------------
+int orthogonalize_workspace(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, size_t* bytes);
+int launch_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, int32_t steps, float eps, void* ws, size_t ws_bytes,
+                         hipStream_t s);
+int muon_workspace(const suave_muon_matrix_t* mats, int32_t n, size_t* bytes);
+int launch_muon(const suave_muon_matrix_t* mats, int32_t n, float momentum, int nesterov, float weight_decay, int32_t steps, float eps, void* ws,
+                size_t ws_bytes, hipStream_t s);
+
 }  // namespace suave

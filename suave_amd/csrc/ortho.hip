@@ -1,0 +1,491 @@
+// Orthogonalised updates: Newton-Schulz products, and the Muon step built on them.
+//
+//   X_0 = U / (|U|_F + eps)      A = X X^T      B = a I + b A + c A A      X <- B X,     (a, b, c) = (3.4445, -4.7750, 2.0315)
+//
+// drives every singular value of U towards 1 (after five steps into about 0.7 .. 1.2) and keeps the singular vectors.  X is
+// kept in the orientation of U; A and B live on the short side, so a tall U uses A = X^T X and X <- X B.  A and B are
+// symmetric: only tiles on and above the diagonal are computed, the others are written as their mirror image, which takes a
+// step from 2 s^2 l + 2 s^3 + 2 s^2 l to s^2 l + s^3 + 2 s^2 l flops (s the short side, l the long one).  All matrices of a
+// call go through the same launches: three per step for the whole list.
+//
+// Arithmetic (mma.h).  fp32 matrices: every factor as two fp16 planes, which keeps binary32's accuracy -- the iteration
+// multiplies small singular directions, and rounding noise in them, by up to a^5 = 485.  bf16 matrices: one fp16 plane (11 bits;
+// the result is rounded to 8): a relative error of about 1.3e-3 where the rounding of the result is 1.7e-3.  Factors are stored times a power of two:
+// X times 2^(12 - e), A times 2^(12 - 2 e), B times 2^12, with 2^e the size of X (e = 0 unless |U|_F is below eps): entries of
+// X are at most about 1.3 in magnitude, and start at 1 / sqrt(rows cols), which 2^12 keeps clear of fp16's subnormals.
+#include <algorithm>
+#include <cmath>
+#include <utility>
+
+#include "kernels.h"
+#include "mma.h"
+
+namespace suave {
+
+namespace {
+
+using namespace mma;
+
+constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
+constexpr int kMaxMats = 24;      // matrices of one group of launches
+constexpr int kMaxSteps = 16;
+constexpr int kNormBlocks = 128;  // partial sums per matrix at most
+constexpr float kS = 4096.0f;
+
+struct Mat {
+  const void* in;       // U (orthogonalize) or the gradient (muon)
+  void* out;            // result or parameter
+  float* mom;           // muon: momentum
+  int64_t ld_in, ld_out, ld_mom;
+  char* x[2];           // planes of X, [rows][pitch]
+  char* a;              // [short][pitch_s]
+  char* b;
+  int rows, cols;
+  float lr;             // muon: learning rate times shape factor
+  float decay;          // muon: 1 - learning rate * weight decay
+};
+
+struct Group {
+  Mat m[kMaxMats];
+  int32_t begin[kMaxMats + 1];  // first block of each matrix in this launch
+  int n;
+  double* part;                 // [kMaxMats][kNormBlocks]
+  int32_t* exps;                // [kMaxMats][kMaxSteps + 1]: e of X_k
+  double eps;
+  float momentum;
+  int nesterov, muon, bf16, steps, k;  // k: the step
+};
+
+__device__ __forceinline__ int find_mat(const Group& g, int b) {
+  int i = 0;
+  while (i + 1 < g.n && b >= g.begin[i + 1]) ++i;
+  return i;
+}
+__host__ __device__ inline int pitch(int cols, int np) { return (cols + 7) / 8 * 8 * 2 * np; }  // bytes of a stored row
+
+__device__ __forceinline__ float in_value(const Group& g, const Mat& m, int64_t r, int c) {
+  if (g.bf16) return bf16_value(static_cast<const uint16_t*>(m.in)[r * m.ld_in + c]);
+  const float v = static_cast<const float*>(m.in)[r * m.ld_in + c];
+  if (!g.muon) return v;
+  const float mom = m.mom[r * m.ld_mom + c];  // already this step's
+  return g.nesterov ? fmaf(g.momentum, mom, v) : mom;
+}
+
+// partial sums of squares (double: neither overflow nor loss over 2^24 values); muon: the momentum first
+__global__ __launch_bounds__(256) void k_ortho_norm(Group g) {
+  const int i = find_mat(g, blockIdx.x);
+  const Mat& m = g.m[i];
+  const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
+  double s = 0.0;
+  const int64_t total = (int64_t)m.rows * m.cols;
+  for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < total; e += (int64_t)nb * 256) {
+    const int64_t r = e / m.cols;
+    const int c = (int)(e - r * m.cols);
+    if (g.muon) {
+      float* mp = m.mom + r * m.ld_mom + c;
+      *mp = fmaf(g.momentum, *mp, static_cast<const float*>(m.in)[r * m.ld_in + c]);
+    }
+    const double v = in_value(g, m, r, c);
+    s += v * v;
+  }
+  __shared__ double part[4];
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) g.part[i * kNormBlocks + b] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// X_0 in planes, pads zero; the sizes of X_0 .. X_steps
+template <int NP>
+__global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
+  const int i = find_mat(g, blockIdx.x);
+  const Mat& m = g.m[i];
+  const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
+  __shared__ double sc;
+  if (threadIdx.x < 64) {
+    double s = 0.0;
+    for (int k = threadIdx.x; k < kNormBlocks; k += 64) s += g.part[i * kNormBlocks + k];
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(s), full = norm + g.eps;
+      double f = norm / full;  // |X_0|_F
+      int e0 = 0;
+      for (int k = 0; k <= g.steps; ++k) {
+        int e = 0;
+        if (f > 0.0 && f < 1.0) { (void)frexp(f, &e); e = max(e, -100); }
+        if (!(e < 0)) e = 0;
+        if (k == 0) e0 = e;
+        if (b == 0) g.exps[i * (kMaxSteps + 1) + k] = e;
+        f *= (double)kNsA;
+      }
+      sc = isfinite(s) ? ldexp(1.0 / full, 12 - e0) : (double)NAN;  // anything not finite: the whole result is NaN
+    }
+  }
+  __syncthreads();
+  const double scale = sc;
+  const int cp = (m.cols + 7) / 8 * 8, q = cp / 8;
+  const int64_t chunks = (int64_t)m.rows * q;
+  const int pit = pitch(m.cols, NP);
+  for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
+    const int64_t r = e / q;
+    const int c0 = (int)(e - r * q) * 8;
+    uint16_t hi[8], lo[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float v = c0 + u < m.cols ? (float)((double)in_value(g, m, r, c0 + u) * scale) : 0.f;
+      if constexpr (NP == 2) planes(v, hi[u], lo[u]);
+      else hi[u] = f16_bits((_Float16)v);
+    }
+    char* o = m.x[0] + r * pit + c0 * 2;
+    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+    if constexpr (NP == 2) *reinterpret_cast<uint4*>(o + cp * 2) = *reinterpret_cast<const uint4*>(lo);
+  }
+}
+
+// stores four consecutive elements (n .. n + 3) of row m, elements past `cols` as zero; n < round_up(cols, 8)
+template <int NP>
+__device__ __forceinline__ void store_planes(char* base, int pit, int cols, int64_t m, int n, const float (&v)[4]) {
+  uint16_t hi[4], lo[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float x = n + u < cols ? v[u] : 0.f;
+    if constexpr (NP == 2) planes(x, hi[u], lo[u]);
+    else hi[u] = f16_bits((_Float16)x);
+  }
+  char* o = base + m * pit + n * 2;
+  *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(hi);
+  if constexpr (NP == 2) *reinterpret_cast<uint2*>(o + (cols + 7) / 8 * 16) = *reinterpret_cast<const uint2*>(lo);
+}
+// the mirror image: elements (n .. n + 3, m)
+template <int NP>
+__device__ __forceinline__ void store_mirror(char* base, int pit, int cols, int m, int n, const float (&v)[4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (n + u >= cols) continue;
+    char* o = base + (int64_t)(n + u) * pit + m * 2;
+    if constexpr (NP == 2) {
+      uint16_t hi, lo;
+      planes(v[u], hi, lo);
+      *reinterpret_cast<uint16_t*>(o) = hi;
+      *reinterpret_cast<uint16_t*>(o + (cols + 7) / 8 * 16) = lo;
+    } else {
+      *reinterpret_cast<uint16_t*>(o) = f16_bits((_Float16)v[u]);
+    }
+  }
+}
+
+// tile t of the T (T + 1) / 2 on and above the diagonal
+__device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
+  tm = 0;
+  while (t >= T - tm) { t -= T - tm; ++tm; }
+  tn = tm + t;
+}
+
+// POLY 0: A from X; 1: B from A
+template <int NP, int BM, int WM, int WN, int POLY>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN, 2> R;
+  typedef Tile<kF16, NP, true, true, BM, BM, WM, WN, 2> C;
+  const int i = find_mat(g, blockIdx.x);
+  const Mat& m = g.m[i];
+  const int s = min(m.rows, m.cols), T = (s + BM - 1) / BM;
+  const int ps = pitch(s, NP);
+  int tm, tn;
+  upper_tile(blockIdx.x - g.begin[i], T, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BM;
+  f32x4 acc[R::MI][R::NI];
+  if (POLY) {
+    const uint32_t plane = (s + 7) / 8 * 16;
+    R::run(lds, Operand{m.a + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane}, Operand{m.a + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane}, s, acc);
+  } else {
+    const int px = pitch(m.cols, NP);
+    const uint32_t plane = (m.cols + 7) / 8 * 16;
+    const char* x = m.x[g.k & 1];
+    if (m.rows <= m.cols)
+      R::run(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, s - m0, plane}, Operand{x + (int64_t)n0 * px, (uint32_t)px, s - n0, plane}, m.cols, acc);
+    else
+      C::run(lds, Operand{x + m0 * 2, (uint32_t)px, (s - m0 + 7) / 8 * 16, plane}, Operand{x + n0 * 2, (uint32_t)px, (s - n0 + 7) / 8 * 16, plane}, m.rows, acc);
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  const int e = g.exps[i * (kMaxSteps + 1) + g.k];
+  const float fb = ldexpf(kNsB, 2 * e), fc = ldexpf(kNsC, max(4 * e - 12, -126));
+  const int sp = (s + 7) / 8 * 8;
+#pragma unroll
+  for (int mi = 0; mi < R::MI; ++mi) {
+    const int r = m0 + wm * (R::MI * 16) + 16 * mi + (lane & 15);
+    if (r >= s) continue;
+#pragma unroll
+    for (int j = 0; j < R::NI; ++j) {
+      const int n = n0 + wn * (R::NI * 16) + 16 * j + 4 * (lane >> 4);
+      if (n >= sp) continue;
+      float v[4];
+      if (POLY) {
+        uint16_t hi[4], lo[4];
+        const char* o = m.a + (int64_t)r * ps + n * 2;
+        *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<const uint2*>(o);
+        if (NP == 2) *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(o + sp * 2);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float av = (float)__builtin_bit_cast(_Float16, hi[u]);
+          if (NP == 2) av += (float)__builtin_bit_cast(_Float16, lo[u]);
+          v[u] = fmaf(fc, acc[mi][j][u], fb * av) + (r == n + u ? kNsA * kS : 0.f);
+        }
+        store_planes<NP>(m.b, ps, s, r, n, v);
+        if (tm != tn) store_mirror<NP>(m.b, ps, s, r, n, v);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = acc[mi][j][u] * (1.0f / kS);
+        store_planes<NP>(m.a, ps, s, r, n, v);
+        if (tm != tn) store_mirror<NP>(m.a, ps, s, r, n, v);
+      }
+    }
+  }
+}
+
+// X <- B X (wide) or X B (tall); the last step writes the result or takes the step on the parameter
+template <int NP, int BM, int WM, int WN, bool LAST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_update(Group g) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  typedef Tile<kF16, NP, false, true, BM, BM, WM, WN, 2> W;
+  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN, 2> H;
+  const int i = find_mat(g, blockIdx.x);
+  const Mat& m = g.m[i];
+  const int s = min(m.rows, m.cols);
+  const int ps = pitch(s, NP), px = pitch(m.cols, NP);
+  const uint32_t plane_s = (s + 7) / 8 * 16, plane_x = (m.cols + 7) / 8 * 16;
+  const int tiles_m = (m.rows + BM - 1) / BM, tiles_n = (m.cols + BM - 1) / BM;
+  int tm, tn;
+  tile_of(blockIdx.x - g.begin[i], tiles_m * tiles_n, tiles_m, tiles_n, 8, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BM;
+  const char* x = m.x[g.k & 1];
+  f32x4 acc[W::MI][W::NI];
+  if (m.rows <= m.cols)
+    W::run(lds, Operand{m.b + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane_s}, Operand{x + (int64_t)n0 * 2, (uint32_t)px, (m.cols - n0 + 7) / 8 * 16, plane_x}, s, acc);
+  else
+    H::run(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  const int e = g.exps[i * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[i * (kMaxSteps + 1) + g.k + 1];
+  const float f = ldexpf(1.0f, max(e - e1 - 12, -126));
+  const int cp = (m.cols + 7) / 8 * 8;
+#pragma unroll
+  for (int mi = 0; mi < W::MI; ++mi) {
+    const int r = m0 + wm * (W::MI * 16) + 16 * mi + (lane & 15);
+    if (r >= m.rows) continue;
+#pragma unroll
+    for (int j = 0; j < W::NI; ++j) {
+      const int n = n0 + wn * (W::NI * 16) + 16 * j + 4 * (lane >> 4);
+      if (n >= (LAST ? m.cols : cp)) continue;
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = acc[mi][j][u] * f;
+      if constexpr (!LAST) {
+        store_planes<NP>(m.x[(g.k & 1) ^ 1], px, m.cols, r, n, v);
+      } else if (g.bf16) {
+        uint16_t* o = static_cast<uint16_t*>(m.out) + (int64_t)r * m.ld_out + n;
+        for (int u = 0; u < 4; ++u)
+          if (n + u < m.cols) o[u] = bf16_bits(v[u]);
+      } else {
+        float* o = static_cast<float*>(m.out) + (int64_t)r * m.ld_out + n;
+        for (int u = 0; u < 4; ++u)
+          if (n + u < m.cols) o[u] = g.muon ? fmaf(-m.lr, v[u], o[u] * m.decay) : v[u];
+      }
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+size_t mat_bytes(int rows, int cols, int np) {
+  const int s = std::min(rows, cols);
+  return 2 * up256((size_t)rows * pitch(cols, np)) + 2 * up256((size_t)s * pitch(s, np));
+}
+size_t head_bytes() { return up256(sizeof(double) * kMaxMats * kNormBlocks) + up256(sizeof(int32_t) * kMaxMats * (kMaxSteps + 1)); }
+
+// Matrices of a call go through the launches in groups of kMaxMats; the groups use the same workspace one after the other
+template <class F>
+size_t workspace_bytes(int n, int np, F shape) {
+  size_t most = 0;
+  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
+    size_t b = 0;
+    for (int i = g0; i < std::min(n, g0 + kMaxMats); ++i) b += mat_bytes(shape(i).first, shape(i).second, np);
+    most = std::max(most, b);
+  }
+  return head_bytes() + most;
+}
+
+int64_t sym_tiles(const Group& g, int bm) {
+  int64_t t = 0;
+  for (int i = 0; i < g.n; ++i) {
+    const int64_t T = ceil_div(std::min(g.m[i].rows, g.m[i].cols), bm);
+    t += T * (T + 1) / 2;
+  }
+  return t;
+}
+int64_t all_tiles(const Group& g, int bm) {
+  int64_t t = 0;
+  for (int i = 0; i < g.n; ++i) t += ceil_div(g.m[i].rows, bm) * ceil_div(g.m[i].cols, bm);
+  return t;
+}
+// the largest tile that still gives most CUs work
+template <class F>
+int pick_tile(const Group& g, F tiles) {
+  if (tiles(g, 256) >= 200) return 256;
+  if (tiles(g, 128) >= 200) return 128;
+  return 64;
+}
+
+template <class K>
+int launch(K kernel, Group& g, int grid, int threads, int lds, hipStream_t s) {
+  if (lds > 64 * 1024) SUAVE_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, g);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <class F>
+int set_begin(Group& g, F blocks) {
+  int64_t b = 0;
+  for (int i = 0; i < g.n; ++i) {
+    g.begin[i] = (int32_t)b;
+    b += blocks(g.m[i]);
+  }
+  g.begin[g.n] = (int32_t)b;
+  return (int)b;
+}
+
+template <int NP, int POLY>
+int launch_sym(Group& g, hipStream_t s) {
+  const int bm = pick_tile(g, sym_tiles);
+  const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), bm); return T * (T + 1) / 2; });
+  if (bm == 256) return launch(k_ortho_sym<NP, 256, 2, 4, POLY>, g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4, 2>::kLds, s);
+  if (bm == 128) return launch(k_ortho_sym<NP, 128, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2, 2>::kLds, s);
+  return launch(k_ortho_sym<NP, 64, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2, 2>::kLds, s);
+}
+template <int NP, bool LAST>
+int launch_update(Group& g, hipStream_t s) {
+  const int bm = pick_tile(g, all_tiles);
+  const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, bm) * ceil_div(m.cols, bm); });
+  if (bm == 256) return launch(k_ortho_update<NP, 256, 2, 4, LAST>, g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4, 2>::kLds, s);
+  if (bm == 128) return launch(k_ortho_update<NP, 128, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2, 2>::kLds, s);
+  return launch(k_ortho_update<NP, 64, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2, 2>::kLds, s);
+}
+
+template <int NP>
+int run_group(Group& g, char* ws, hipStream_t s) {
+  g.part = reinterpret_cast<double*>(ws);
+  g.exps = reinterpret_cast<int32_t*>(ws + up256(sizeof(double) * kMaxMats * kNormBlocks));
+  char* at = ws + head_bytes();
+  for (int i = 0; i < g.n; ++i) {
+    Mat& m = g.m[i];
+    const int sh = std::min(m.rows, m.cols);
+    for (int k = 0; k < 2; ++k) { m.x[k] = at; at += up256((size_t)m.rows * pitch(m.cols, NP)); }
+    m.a = at; at += up256((size_t)sh * pitch(sh, NP));
+    m.b = at; at += up256((size_t)sh * pitch(sh, NP));
+  }
+  // every partial of a matrix is written: kNormBlocks blocks whatever its size
+  int grid = set_begin(g, [](const Mat&) { return (int64_t)kNormBlocks; });
+  hipLaunchKernelGGL(k_ortho_norm, dim3(grid), dim3(256), 0, s, g);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  grid = set_begin(g, [](const Mat& m) { return std::min<int64_t>(1024, std::max<int64_t>(1, ceil_div((int64_t)m.rows * ((m.cols + 7) / 8), 256))); });
+  hipLaunchKernelGGL(k_ortho_pack<NP>, dim3(grid), dim3(256), 0, s, g);
+  SUAVE_CHECK_HIP(hipGetLastError());
+  for (g.k = 0; g.k < g.steps; ++g.k) {
+    if (int rc = launch_sym<NP, 0>(g, s)) return rc;
+    if (int rc = launch_sym<NP, 1>(g, s)) return rc;
+    if (int rc = g.k + 1 < g.steps ? launch_update<NP, false>(g, s) : launch_update<NP, true>(g, s)) return rc;
+  }
+  return 0;
+}
+
+int check_dims(int32_t rows, int32_t cols) {
+  SUAVE_REQUIRE(rows >= 1 && cols >= 1, "orthogonalize: a matrix needs at least one row and one column");
+  SUAVE_REQUIRE(std::min(rows, cols) <= 32768 && std::max(rows, cols) <= (1 << 20), "orthogonalize: the sides of a matrix must be at most 32768 (short) and 2^20 (long)");
+  return 0;
+}
+int check_run(int32_t n, int32_t steps, float eps, const void* ws, size_t bytes, size_t need) {
+  SUAVE_REQUIRE(n >= 0, "orthogonalize: negative number of matrices");
+  SUAVE_REQUIRE(steps >= 1 && steps <= kMaxSteps, "orthogonalize: steps must be in 1..16");
+  SUAVE_REQUIRE(eps > 0.f && std::isfinite(eps), "orthogonalize: eps must be positive");
+  SUAVE_REQUIRE(n == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 255) == 0), "orthogonalize: workspace is null or not 256-byte aligned");
+  SUAVE_REQUIRE(bytes >= need || n == 0, "orthogonalize: workspace too small");
+  return 0;
+}
+
+}  // namespace
+
+int orthogonalize_workspace(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, size_t* bytes) {
+  SUAVE_REQUIRE(dtype == SUAVE_DTYPE_F32 || dtype == SUAVE_DTYPE_BF16, "orthogonalize: dtype must be SUAVE_DTYPE_F32 or SUAVE_DTYPE_BF16");
+  SUAVE_REQUIRE(n >= 0 && (n == 0 || mats) && bytes, "orthogonalize: null argument");
+  for (int i = 0; i < n; ++i)
+    if (int rc = check_dims(mats[i].rows, mats[i].cols)) return rc;
+  *bytes = workspace_bytes(n, dtype == SUAVE_DTYPE_F32 ? 2 : 1, [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); });
+  return 0;
+}
+
+int launch_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dtype, int32_t steps, float eps, void* ws, size_t ws_bytes, hipStream_t s) {
+  size_t need = 0;
+  if (int rc = orthogonalize_workspace(mats, n, dtype, &need)) return rc;
+  if (int rc = check_run(n, steps, eps, ws, ws_bytes, need)) return rc;
+  for (int i = 0; i < n; ++i) {
+    SUAVE_REQUIRE(mats[i].in && mats[i].out, "orthogonalize: a matrix is null");
+    SUAVE_REQUIRE(mats[i].ld_in >= mats[i].cols && mats[i].ld_out >= mats[i].cols, "orthogonalize: a row stride is shorter than the row");
+  }
+  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
+    Group g{};
+    g.n = std::min(kMaxMats, n - g0);
+    for (int i = 0; i < g.n; ++i) {
+      const suave_ortho_matrix_t& h = mats[g0 + i];
+      Mat& m = g.m[i];
+      m.in = h.in; m.out = h.out; m.ld_in = h.ld_in; m.ld_out = h.ld_out; m.rows = h.rows; m.cols = h.cols;
+    }
+    g.eps = eps; g.steps = steps; g.bf16 = dtype == SUAVE_DTYPE_BF16;
+    if (int rc = g.bf16 ? run_group<1>(g, static_cast<char*>(ws), s) : run_group<2>(g, static_cast<char*>(ws), s)) return rc;
+  }
+  return 0;
+}
+
+int muon_workspace(const suave_muon_matrix_t* mats, int32_t n, size_t* bytes) {
+  SUAVE_REQUIRE(n >= 0 && (n == 0 || mats) && bytes, "muon_step: null argument");
+  for (int i = 0; i < n; ++i)
+    if (int rc = check_dims(mats[i].rows, mats[i].cols)) return rc;
+  *bytes = workspace_bytes(n, 2, [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); });
+  return 0;
+}
+
+int launch_muon(const suave_muon_matrix_t* mats, int32_t n, float momentum, int nesterov, float weight_decay, int32_t steps, float eps, void* ws,
+                size_t ws_bytes, hipStream_t s) {
+  size_t need = 0;
+  if (int rc = muon_workspace(mats, n, &need)) return rc;
+  if (int rc = check_run(n, steps, eps, ws, ws_bytes, need)) return rc;
+  SUAVE_REQUIRE(momentum >= 0.f && momentum < 1.f, "muon_step: momentum must be in [0, 1)");
+  SUAVE_REQUIRE(weight_decay >= 0.f && std::isfinite(weight_decay), "muon_step: weight_decay must not be negative");
+  for (int i = 0; i < n; ++i) {
+    const suave_muon_matrix_t& h = mats[i];
+    SUAVE_REQUIRE(h.param && h.grad && h.momentum, "muon_step: param / grad / momentum is null");
+    SUAVE_REQUIRE(h.ld_param >= h.cols && h.ld_grad >= h.cols && h.ld_momentum >= h.cols, "muon_step: a row stride is shorter than the row");
+    SUAVE_REQUIRE(std::isfinite(h.lr) && h.lr >= 0.f, "muon_step: lr must not be negative");
+  }
+  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
+    Group g{};
+    g.n = std::min(kMaxMats, n - g0);
+    for (int i = 0; i < g.n; ++i) {
+      const suave_muon_matrix_t& h = mats[g0 + i];
+      Mat& m = g.m[i];
+      m.in = h.grad; m.out = h.param; m.mom = h.momentum; m.ld_in = h.ld_grad; m.ld_out = h.ld_param; m.ld_mom = h.ld_momentum;
+      m.rows = h.rows; m.cols = h.cols;
+      m.lr = (float)((double)h.lr * std::sqrt(std::max(1.0, (double)h.rows / h.cols)));
+      m.decay = (float)(1.0 - (double)h.lr * weight_decay);
+    }
+    g.eps = eps; g.steps = steps; g.muon = 1; g.momentum = momentum; g.nesterov = nesterov;
+    if (int rc = run_group<2>(g, static_cast<char*>(ws), s)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace suave

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-from .plan import BatchT, ColT, ElboOutT, HeadT, LinearCeT, LinearQuantizedT, ModelT, NoiseT
+from .plan import BatchT, ColT, ElboOutT, HeadT, LinearCeT, LinearQuantizedT, ModelT, MuonMatrixT, NoiseT, OrthoMatrixT
 
 # SUAVE_HIP_LIB points at another build of the same library (tuning builds under build/); default: the in-tree one
 _LIB_PATH = os.environ.get("SUAVE_HIP_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsuave_hip.so")
@@ -29,6 +29,10 @@ EXPORTS = (
     "suave_elbo_joint_backward",
     "suave_linear_ce_workspace_bytes",
     "suave_linear_ce",
+    "suave_orthogonalize_workspace_bytes",
+    "suave_orthogonalize",
+    "suave_muon_workspace_bytes",
+    "suave_muon_step",
     "suave_quantize_rows",
     "suave_linear_quantized_workspace_bytes",
     "suave_linear_quantized",
@@ -106,6 +110,10 @@ def load():
     lib.suave_quantize_rows.argtypes = [vp, i32, i64, i32, i64, vp, i64, vp, vp]
     lib.suave_linear_quantized_workspace_bytes.argtypes = [C.POINTER(LinearQuantizedT), C.POINTER(sz)]
     lib.suave_linear_quantized.argtypes = [C.POINTER(LinearQuantizedT), vp]
+    lib.suave_orthogonalize_workspace_bytes.argtypes = [C.POINTER(OrthoMatrixT), i32, i32, C.POINTER(sz)]
+    lib.suave_orthogonalize.argtypes = [C.POINTER(OrthoMatrixT), i32, i32, i32, f32, vp, sz, vp]
+    lib.suave_muon_workspace_bytes.argtypes = [C.POINTER(MuonMatrixT), i32, C.POINTER(sz)]
+    lib.suave_muon_step.argtypes = [C.POINTER(MuonMatrixT), i32, f32, i32, f32, i32, f32, vp, sz, vp]
     lib.suave_adam_step.argtypes = [vp, vp, vp, vp, C.POINTER(i32), C.POINTER(f32), i32, i64, f32, f32, f32, vp]
     lib.suave_encode.argtypes = [vp, vp, C.POINTER(BatchT), f32, vp, sz, vp, vp, vp, vp, vp]
     lib.suave_encode_hard.argtypes = [vp, vp, C.POINTER(BatchT), f32, vp, sz, vp, vp, vp]

@@ -11,12 +11,12 @@ outputs.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import lib as _lib
-from .plan import LinearCeT, LinearQuantizedT
+from .plan import LinearCeT, LinearQuantizedT, MuonMatrixT, OrthoMatrixT
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # SUAVE_DTYPE_F32, SUAVE_DTYPE_BF16
 
@@ -129,6 +129,70 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
         _lib.check(lib.suave_linear_ce(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_ce")
     return out
+
+
+def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, eps: float = 1e-7,
+                  out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+    """Newton-Schulz orthogonalisation of a list of matrices at once (``suave_orthogonalize``): float32 or bfloat16 (one type
+    for the list), rows contiguous, any row stride; ``out`` may be the matrices themselves.  ``steps`` times
+    ``X <- (a I + b X X^T + c (X X^T)^2) X`` from ``X = U / (|U|_F + eps)``."""
+
+    matrices = list(matrices)
+    if not matrices:
+        return []
+    dev = _device_of("matrices[0]", matrices[0])
+    dt = matrices[0].dtype
+    _need(dt in _DTYPES, f"matrices must have one of the types {[str(d) for d in _DTYPES]}")
+    lds = [_matrix(f"matrices[{i}]", t, dev, (dt,)) for i, t in enumerate(matrices)]
+    _need(all(t.numel() > 0 for t in matrices), "a matrix needs at least one row and one column")
+    with torch.cuda.device(dev):
+        if out is None:
+            out = [torch.empty(t.shape, dtype=dt, device=dev) for t in matrices]
+        out = list(out)
+        _need(len(out) == len(matrices), "out must have one matrix for each")
+        arr = (OrthoMatrixT * len(matrices))()
+        for i, (a, t, o) in enumerate(zip(arr, matrices, out)):
+            a.ld_out = _matrix(f"out[{i}]", o, dev, (dt,), t.shape)
+            a.in_, a.out, a.ld_in, a.rows, a.cols = t.data_ptr(), o.data_ptr(), lds[i], int(t.shape[0]), int(t.shape[1])
+        lib = _lib.load()
+        nbytes = C.c_size_t(0)
+        _lib.check(lib.suave_orthogonalize_workspace_bytes(arr, len(matrices), _DTYPES[dt], C.byref(nbytes)),
+                   "suave_orthogonalize_workspace_bytes")
+        ws, base, nb = _workspace(int(nbytes.value), dev)
+        _lib.check(lib.suave_orthogonalize(arr, len(matrices), _DTYPES[dt], int(steps), float(eps), base, nb,
+                                           torch.cuda.current_stream(dev).cuda_stream), "suave_orthogonalize")
+    return out
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], *, lr,
+              momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7) -> None:
+    """One Muon step in place on a list of float32 weight matrices (``suave_muon_step``): ``momentum`` averaging, the
+    orthogonalised update of each matrix, ``param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O``.  ``lr``: a
+    number, or one for each matrix.  ``momenta`` start as zeros.  Rows contiguous, any row stride (views of a flat buffer)."""
+
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    n = len(params)
+    _need(len(grads) == n and len(momenta) == n, "params, grads and momenta must have the same length")
+    lrs = [float(lr)] * n if not isinstance(lr, (list, tuple)) else [float(v) for v in lr]
+    _need(len(lrs) == n, "lr must be a number or one for each matrix")
+    if not n:
+        return
+    dev = _device_of("params[0]", params[0])
+    f32 = (torch.float32,)
+    arr = (MuonMatrixT * n)()
+    for i, (a, p, g, m) in enumerate(zip(arr, params, grads, momenta)):
+        a.ld_param = _matrix(f"params[{i}]", p, dev, f32)
+        _need(p.numel() > 0, "a matrix needs at least one row and one column")
+        a.ld_grad, a.ld_momentum = _matrix(f"grads[{i}]", g, dev, f32, p.shape), _matrix(f"momenta[{i}]", m, dev, f32, p.shape)
+        a.param, a.grad, a.momentum = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        a.rows, a.cols, a.lr = int(p.shape[0]), int(p.shape[1]), lrs[i]
+    with torch.cuda.device(dev):
+        lib = _lib.load()
+        nbytes = C.c_size_t(0)
+        _lib.check(lib.suave_muon_workspace_bytes(arr, n, C.byref(nbytes)), "suave_muon_workspace_bytes")
+        ws, base, nb = _workspace(int(nbytes.value), dev)
+        _lib.check(lib.suave_muon_step(arr, n, float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps), base, nb,
+                                       torch.cuda.current_stream(dev).cuda_stream), "suave_muon_step")
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

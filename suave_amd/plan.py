@@ -90,6 +90,16 @@ class LinearQuantizedT(C.Structure):  # suave_linear_quantized_t
                 ("workspace_bytes", C.c_size_t)]
 
 
+class OrthoMatrixT(C.Structure):  # suave_ortho_matrix_t
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("ld_in", C.c_int64), ("ld_out", C.c_int64), ("rows", C.c_int32),
+                ("cols", C.c_int32)]
+
+
+class MuonMatrixT(C.Structure):  # suave_muon_matrix_t
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p), ("ld_param", C.c_int64),
+                ("ld_grad", C.c_int64), ("ld_momentum", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32), ("lr", C.c_float)]
+
+
 def _r4(x: int) -> int:
     return (x + 3) // 4 * 4
 
