@@ -623,10 +623,10 @@ int launch_logits_tile(LogitArgs a, hipStream_t s) {
 template <int TYPE, int NP, int SWEEP>
 int launch_logits(const LogitArgs& a, int tile, hipStream_t s) {
   switch (tile) {
-    case kLow16: return launch_logits_tile<Tile<TYPE, NP, false, false, 16, 256, 1, 4, 2>, SWEEP>(a, s);
-    case kLow64: return launch_logits_tile<Tile<TYPE, NP, false, false, 64, 256, 1, 4, 2>, SWEEP>(a, s);
-    case kMid128: return launch_logits_tile<Tile<TYPE, NP, false, false, 128, 128, 2, 2, 2>, SWEEP>(a, s);
-    default: return launch_logits_tile<Tile<TYPE, NP, false, false, 256, 256, 2, 4, 2>, SWEEP>(a, s);
+    case kLow16: return launch_logits_tile<Tile<TYPE, NP, false, false, 16, 256, 1, 4>, SWEEP>(a, s);
+    case kLow64: return launch_logits_tile<Tile<TYPE, NP, false, false, 64, 256, 1, 4>, SWEEP>(a, s);
+    case kMid128: return launch_logits_tile<Tile<TYPE, NP, false, false, 128, 128, 2, 2>, SWEEP>(a, s);
+    default: return launch_logits_tile<Tile<TYPE, NP, false, false, 256, 256, 2, 4>, SWEEP>(a, s);
   }
 }
 
@@ -637,13 +637,13 @@ int launch_grad(const GradArgs& g, int tile, hipStream_t s) {
   void* args[] = {&a};
   const int64_t grid = ceil_div(a.M, tile) * ceil_div(a.N, tile) * a.splits;
   if (tile == 256) {
-    typedef Tile<TYPE, NP, ACOL, true, 256, 256, 2, 4, 2> T;
+    typedef Tile<TYPE, NP, ACOL, true, 256, 256, 2, 4> T;
     return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
   } else if (tile == 128) {
-    typedef Tile<TYPE, NP, ACOL, true, 128, 128, 2, 2, 2> T;
+    typedef Tile<TYPE, NP, ACOL, true, 128, 128, 2, 2> T;
     return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
   }
-  typedef Tile<TYPE, NP, ACOL, true, 64, 64, 2, 2, 2> T;
+  typedef Tile<TYPE, NP, ACOL, true, 64, 64, 2, 2> T;
   return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
 }
 

@@ -11,11 +11,16 @@
 // way out of LDS by ds_read_b64_tr_b16: 16 lanes read 4 k-rows x 16 columns, lane i gets column i.
 //
 // A K step is 128 bytes per row whatever the type: 64 bf16 / fp16, 32 values in two planes, 128 int8.  Tiles go from
-// global memory to LDS directly (buffer_load ... lds, 16 bytes per lane), ST - 1 steps ahead.  The DMA writes lane i
+// global memory to LDS directly (buffer_load ... lds, 16 bytes per lane), into two slots.  The DMA writes lane i
 // at base + 16 i, so the bank swizzle is a permutation of the SOURCE chunks: row form slot s of row r holds chunk
 // s ^ (r & 7); column form slot s of k-row r holds chunk s ^ (2 (r & 3) [^ 8 ((r >> 3) & 1)]).  Chunks past the edge of an
 // operand along K read as zero (an offset beyond the buffer resource's range), rows past the edge are clamped to the
 // last one (their products are never written).
+//
+// What it reaches (256 x 256 tile, eight waves, 8192 x 8192 x 4096, stores of the fp32 result included): bf16 1200 TFLOP/s, int8 1950,
+// two fp16 planes 1510 of their three products; a library product reaches 1400 / 2160 / 1490 on this card.  Matrix pipe busy 61 %
+// (bf16) and 69 % (planes) of the cycles at the 2.0 - 2.2 GHz it runs at under this load; the rest is the feed: without the
+// transfers the bf16 loop runs at 1530, with every transfer hitting L2 at 1280.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -55,9 +60,24 @@ __device__ __forceinline__ const char* uniform_ptr(const char* p) {
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-__device__ __forceinline__ void dma16(const char* base, uint32_t voff, char* lds) {
+__device__ __forceinline__ i32x4 resource(const char* base) {  // raw buffer of 2^31 bytes from base
+  const uint64_t v = reinterpret_cast<uint64_t>(base);
+  return i32x4{(int)(uint32_t)v, (int)((uint32_t)(v >> 32) & 0xffffu), (int)0x80000000u, 0x00020000};
+}
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_char*)p);
+}
+// 16 bytes per lane from base + voff to LDS at lds + 16 lane.
+__device__ __forceinline__ void dma16_scheduled(const char* base, uint32_t voff, char* lds) {
   __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)0x80000000u, 0x00020000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds_char*)lds, 16, voff, 0, 0, 0);
+}
+// The same, written as an instruction because the compiler, which would
+// otherwise know of the transfer, waits for ALL transfers before any transposed LDS read (8192 x 8192 x 4096 bf16 with a
+// column-form operand: 569 us, against 457 us).  It has no result register; callers wait by vmcnt and a barrier before the LDS is read.
+// The wait states cover m0 and a resource that a vector instruction has just written.
+__device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "m0");
 }
 
 // The staging of one operand: EXT rows (row form) or columns (column form) of a tile, NP planes, by NW waves.
@@ -132,9 +152,9 @@ __device__ __forceinline__ typename Acc<TYPE>::type mul(i32x4 a, i32x4 b, typena
 
 // A block of WM x WN waves computes BM x BN; a wave MI x NI fragments of 16 x 16.  Lane layout of acc[mi][ni]:
 // m = wave_m0 + 16 mi + (lane & 15), n = wave_n0 + 16 ni + 4 (lane >> 4) + j: four consecutive n per lane.
-template <int TYPE_, int NP_, bool ACOL_, bool BCOL_, int BM_, int BN_, int WM_, int WN_, int ST_>
+template <int TYPE_, int NP_, bool ACOL_, bool BCOL_, int BM_, int BN_, int WM_, int WN_>
 struct Tile {
-  static constexpr int TYPE = TYPE_, NP = NP_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int TYPE = TYPE_, NP = NP_, BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr bool ACOL = ACOL_, BCOL = BCOL_;
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
@@ -144,79 +164,106 @@ struct Tile {
   typedef typename Acc<TYPE>::type acc_t;
   static constexpr int kStepK = SA::kStepK;
   static constexpr int kStepBytes = SA::kBytes + SB::kBytes;
-  static constexpr int kLds = ST * kStepBytes;
-  // DMA instructions a wave has in flight per step (waves that issue fewer simply wait for less)
-  static constexpr int kPerStep = SA::kPer + SB::kPer;
+  static constexpr int kLds = 2 * kStepBytes;
+  static constexpr int kPerStep = SA::kPer + SB::kPer;  // DMA instructions of a wave and step
   static constexpr bool kEven = SA::kInstr % (WM * WN) == 0 && SB::kInstr % (WM * WN) == 0;
 
-  static __device__ __forceinline__ void load(const Operand& A, const Operand& B, const char* pa, const char* pb, char* lds, int wave, int lane,
-                                              const uint32_t (&oa)[SA::kPer], const uint32_t (&ob)[SB::kPer], int kleft) {
-    const bool full = kleft >= kStepK;
-#pragma unroll
-    for (int i = 0; i < SA::kPer; ++i) {
-      if (SA::kInstr % (WM * WN) != 0 && i * WM * WN + wave >= SA::kInstr) break;
-      dma16(pa, full ? oa[i] : SA::offset(A, i, wave, lane, kleft), lds + (i * WM * WN + wave) * 1024);
+  // DMA instruction i (of kPerStep) of this wave
+  template <int I>
+  static __device__ __forceinline__ void dma(i32x4 ra, i32x4 rb, uint32_t lds, int wave, const uint32_t (&oa)[SA::kPer], const uint32_t (&ob)[SB::kPer]) {
+    if constexpr (I < SA::kPer) {
+      if (SA::kInstr % (WM * WN) == 0 || I * WM * WN + wave < SA::kInstr) dma16(ra, oa[I], lds + (I * WM * WN + wave) * 1024);
+    } else if constexpr (I < kPerStep) {
+      constexpr int J = I - SA::kPer;
+      if (SB::kInstr % (WM * WN) == 0 || J * WM * WN + wave < SB::kInstr) dma16(rb, ob[J], lds + SA::kBytes + (J * WM * WN + wave) * 1024);
     }
-#pragma unroll
-    for (int i = 0; i < SB::kPer; ++i) {
-      if (SB::kInstr % (WM * WN) != 0 && i * WM * WN + wave >= SB::kInstr) break;
-      dma16(pb, full ? ob[i] : SB::offset(B, i, wave, lane, kleft), lds + SA::kBytes + (i * WM * WN + wave) * 1024);
+  }
+  template <int I0, int I1>
+  static __device__ __forceinline__ void dmas(i32x4 ra, i32x4 rb, uint32_t lds, int wave, const uint32_t (&oa)[SA::kPer], const uint32_t (&ob)[SB::kPer]) {
+    if constexpr (I0 < I1) {
+      dma<I0>(ra, rb, lds, wave, oa, ob);
+      dmas<I0 + 1, I1>(ra, rb, lds, wave, oa, ob);
     }
+  }
+  static __device__ __forceinline__ void offsets(const Operand& A, const Operand& B, int wave, int lane, int kleft, uint32_t (&oa)[SA::kPer],
+                                                 uint32_t (&ob)[SB::kPer]) {
+#pragma unroll
+    for (int i = 0; i < SA::kPer; ++i) oa[i] = SA::offset(A, i, wave, lane, kleft);
+#pragma unroll
+    for (int i = 0; i < SB::kPer; ++i) ob[i] = SB::offset(B, i, wave, lane, kleft);
   }
 
-  template <int N, int PER>
-  static __device__ __forceinline__ void schedule() {  // N times: PER matrix instructions, one LDS read
-    if constexpr (N > 0) {
-      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      schedule<N - 1, PER>();
+  struct Frags { i32x4 b[NI], a[MI]; };
+  // fragment q of a half step (one plane: kk the half, two planes: kk the plane): B's NI first, then A's MI
+  static __device__ __forceinline__ void read(const char* lds, int wm, int wn, int kk, int lane, int q, Frags& f) {
+    if (q < NI) f.b[q] = fragment<TYPE, NP, BCOL, BN>(lds + SA::kBytes, wn * (NI * 16) + 16 * q, kk, lane);
+    else f.a[q - NI] = fragment<TYPE, NP, ACOL, BM>(lds, wm * (MI * 16) + 16 * (q - NI), kk, lane);
+  }
+  static __device__ __forceinline__ void read_all(const char* lds, int wm, int wn, int kk, int lane, Frags& f) {
+#pragma unroll
+    for (int q = 0; q < NI + MI; ++q) read(lds, wm, wn, kk, lane, q, f);
+  }
+
+  // Half a step: the products of `now`, while the other half (or the next step's first) is read into `then` and, if DMA, a step's
+  // DMA is issued.  A wave issues in order: DMA instructions in a row fill the address unit's queue and hold up the products
+  // behind them, and a fragment read right before its products is waited for.  So each of the MI groups of products is followed
+  // by its share of both, and the compiler may not move them across (8192 x 8192 x 4096 bf16: transfers in a row and one barrier
+  // in front of each step 490 us, this 450 us; the transfers in front of the products 456 us).
+  template <int I, bool DMA>
+  static __device__ __forceinline__ void half(const char* lds, int wm, int wn, int kk, int lane, const Frags& now, Frags& then, acc_t (&acc)[MI][NI],
+                                              i32x4 ra, i32x4 rb, uint32_t slot, int wave, const uint32_t (&oa)[SA::kPer], const uint32_t (&ob)[SB::kPer]) {
+    if constexpr (I < MI) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[I][j] = mul<TYPE>(now.b[j], now.a[I], acc[I][j]);
+#pragma unroll
+      for (int q = (I * (NI + MI) + MI - 1) / MI; q < ((I + 1) * (NI + MI) + MI - 1) / MI; ++q) read(lds, wm, wn, kk, lane, q, then);
+      if constexpr (DMA) dmas<I * kPerStep / MI, (I + 1) * kPerStep / MI>(ra, rb, slot, wave, oa, ob);
+      __builtin_amdgcn_sched_barrier(0);
+      half<I + 1, DMA>(lds, wm, wn, kk, lane, now, then, acc, ra, rb, slot, wave, oa, ob);
     }
   }
-  static __device__ __forceinline__ void step(const char* lds, int wm, int wn, int lane, acc_t (&acc)[MI][NI]) {
-    const char* la = lds;
-    const char* lb = lds + SA::kBytes;
-    const int m0 = wm * (MI * 16), n0 = wn * (NI * 16);
-    if constexpr (NP == 1) {
+  // Two planes: a step's fragments (row form chunks 0..3 hi, 4..7 lo; column form k-rows 0..31 hi, 32..63 lo), three products
+  // for each pair.  The transfers of the next step are placed by the compiler: the reads of this step all come first or
+  // between its products, so nothing waits for a transfer before the next turn.
+  static __device__ __forceinline__ void planes_load(const char* pa, const char* pb, char* lds, int wave, const uint32_t (&oa)[SA::kPer],
+                                                     const uint32_t (&ob)[SB::kPer]) {
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        i32x4 b[NI], a[MI];
+    for (int i = 0; i < SA::kPer; ++i)
+      if (SA::kInstr % (WM * WN) == 0 || i * WM * WN + wave < SA::kInstr) dma16_scheduled(pa, oa[i], lds + (i * WM * WN + wave) * 1024);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) b[j] = fragment<TYPE, NP, BCOL, BN>(lb, n0 + 16 * j, kk, lane);
+    for (int i = 0; i < SB::kPer; ++i)
+      if (SB::kInstr % (WM * WN) == 0 || i * WM * WN + wave < SB::kInstr)
+        dma16_scheduled(pb, ob[i], lds + SA::kBytes + (i * WM * WN + wave) * 1024);
+  }
+  static __device__ __forceinline__ void planes_step(const char* lds, int wm, int wn, int lane, acc_t (&acc)[MI][NI]) {
+    Frags h, l;
+    read_all(lds, wm, wn, 0, lane, h);
+    read_all(lds, wm, wn, 1, lane, l);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) a[i] = fragment<TYPE, NP, ACOL, BM>(la, m0 + 16 * i, kk, lane);
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(b[j], a[i], acc[i][j]);
-      }
-      // issue order: the first sub-step's B fragments and two A fragments, then one fragment read behind every few
-      // products (left alone the compiler waits for each A fragment right before its products: 4096^3 bf16 132 -> 116 us,
-      // int8 71 -> 64 us; the two-plane form has three products per fragment pair and gains nothing)
-      constexpr int ra = ACOL ? 2 : 1, rb = BCOL ? 2 : 1;
-      constexpr int head = NI * rb + (MI > 1 ? 2 : 1) * ra, rest = 2 * (NI * rb + MI * ra) - head, mf = 2 * MI * NI;
-      constexpr int per = (mf - 4) / rest > 1 ? (mf - 4) / rest : 1;
-      __builtin_amdgcn_sched_group_barrier(0x100, head, 0);
-      schedule<rest, per>();
-      __builtin_amdgcn_sched_group_barrier(0x008, mf, 0);
-    } else {  // kk is the plane: row form chunks 0..3 hi, 4..7 lo; column form k-rows 0..31 hi, 32..63 lo
-      i32x4 bh[NI], bl[NI];
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        bh[j] = fragment<TYPE, NP, BCOL, BN>(lb, n0 + 16 * j, 0, lane);
-        bl[j] = fragment<TYPE, NP, BCOL, BN>(lb, n0 + 16 * j, 1, lane);
+        acc[i][j] = mul<TYPE>(l.b[j], h.a[i], acc[i][j]);
+        acc[i][j] = mul<TYPE>(h.b[j], l.a[i], acc[i][j]);
+        acc[i][j] = mul<TYPE>(h.b[j], h.a[i], acc[i][j]);
       }
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const i32x4 ah = fragment<TYPE, NP, ACOL, BM>(la, m0 + 16 * i, 0, lane);
-        const i32x4 al = fragment<TYPE, NP, ACOL, BM>(la, m0 + 16 * i, 1, lane);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          acc[i][j] = mul<TYPE>(bl[j], ah, acc[i][j]);
-          acc[i][j] = mul<TYPE>(bh[j], al, acc[i][j]);
-          acc[i][j] = mul<TYPE>(bh[j], ah, acc[i][j]);
-        }
-      }
+  }
+  // issue order of a planes step: B's and the first two A fragments, then the other reads and the transfers spread evenly
+  // between the products
+  template <int I, int M, int D, int V>
+  static __device__ __forceinline__ void spread() {
+    if constexpr (I < M) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if constexpr ((I + 1) * D / M > I * D / M) __builtin_amdgcn_sched_group_barrier(0x100, (I + 1) * D / M - I * D / M, 0);
+      if constexpr ((I + 1) * V / M > I * V / M) __builtin_amdgcn_sched_group_barrier(0x010, (I + 1) * V / M - I * V / M, 0);
+      spread<I + 1, M, D, V>();
     }
+  }
+  static __device__ __forceinline__ void turn() {  // this wave's DMA has landed and its LDS reads are done; then everybody's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // K elements from the operands' bases.  Every thread of the block takes part; lds: kLds bytes, 16-byte aligned.
@@ -227,38 +274,78 @@ struct Tile {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+    const int steps = (K + kStepK - 1) / kStepK;
+    if (steps == 0) return;
     uint32_t oa[SA::kPer], ob[SB::kPer];
-#pragma unroll
-    for (int i = 0; i < SA::kPer; ++i) oa[i] = SA::offset(A, i, wave, lane, kStepK);
-#pragma unroll
-    for (int i = 0; i < SB::kPer; ++i) ob[i] = SB::offset(B, i, wave, lane, kStepK);
+    offsets(A, B, wave, lane, steps > 1 ? kStepK : K, oa, ob);
     const char* pa = uniform_ptr(A.base);
     const char* pb = uniform_ptr(B.base);
     const uint64_t da = SA::advance(A), db = SB::advance(B);
-    const int steps = (K + kStepK - 1) / kStepK;
-    int issued = 0;
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-      if (s < steps) {
-        load(A, B, pa, pb, lds + s * kStepBytes, wave, lane, oa, ob, K - s * kStepK);
-        pa += da; pb += db; ++issued;
+    const uint32_t slot0 = lds_offset(lds);
+    int s = 0;
+    if constexpr (NP == 1) {
+      dmas<0, kPerStep>(resource(pa), resource(pb), slot0, wave, oa, ob);
+      // The slot of step s is free as soon as every wave holds its second half in registers, so there is ONE barrier per step,
+      // in the middle of its products: behind it the DMA of step s + 2 starts and the first half of step s + 1 is read while
+      // the second half of step s is multiplied.  No product waits for LDS, and a DMA has a whole step to land.
+      if (steps > 1) {
+        pa += da; pb += db;
+        if (steps == 2) offsets(A, B, wave, lane, K - kStepK, oa, ob);
+        dmas<0, kPerStep>(resource(pa), resource(pb), slot0 + kStepBytes, wave, oa, ob);
       }
-    }
-    for (int s = 0; s < steps; ++s) {
-      // step s has landed when at most the steps issued behind it are still in flight
-      if (ST == 2 || !kEven || s + ST - 1 > steps) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      else if constexpr (ST == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPerStep) : "memory");
-      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kPerStep) : "memory");
+      if (kEven && steps > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPerStep) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (issued < steps) {  // into the slot that step s - 1 has left (all waves are past it: the barrier above)
-        load(A, B, pa, pb, lds + (issued % ST) * kStepBytes, wave, lane, oa, ob, K - issued * kStepK);
-        pa += da; pb += db; ++issued;
+      Frags f0, f1;
+      read_all(lds, wm, wn, 0, lane, f0);
+      __builtin_amdgcn_sched_barrier(0);
+      for (; s < steps - 3; ++s) {
+        half<0, false>(lds + (s & 1) * kStepBytes, wm, wn, 1, lane, f0, f1, acc, i32x4{}, i32x4{}, 0, wave, oa, ob);
+        turn();
+        pa += da; pb += db;
+        half<0, true>(lds + (~s & 1) * kStepBytes, wm, wn, 0, lane, f1, f0, acc, resource(pa), resource(pb), slot0 + (s & 1) * kStepBytes, wave, oa, ob);
       }
-      step(lds + (s % ST) * kStepBytes, wm, wn, lane, acc);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the slot are done before the next barrier
+      for (; s < steps - 1; ++s) {  // the last step may be short: its chunks past K are masked
+        half<0, false>(lds + (s & 1) * kStepBytes, wm, wn, 1, lane, f0, f1, acc, i32x4{}, i32x4{}, 0, wave, oa, ob);
+        turn();
+        if (s + 2 < steps) {
+          pa += da; pb += db;
+          offsets(A, B, wave, lane, K - (s + 2) * kStepK, oa, ob);
+          dmas<0, kPerStep>(resource(pa), resource(pb), slot0 + (s & 1) * kStepBytes, wave, oa, ob);
+        }
+        half<0, false>(lds + (~s & 1) * kStepBytes, wm, wn, 0, lane, f1, f0, acc, i32x4{}, i32x4{}, 0, wave, oa, ob);
+      }
+      half<0, false>(lds + (s & 1) * kStepBytes, wm, wn, 1, lane, f0, f1, acc, i32x4{}, i32x4{}, 0, wave, oa, ob);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(f1.b[j], f1.a[i], acc[i][j]);
+    } else {
+      planes_load(pa, pb, lds, wave, oa, ob);
+      constexpr int da_reads = 2 * MI * (ACOL ? 2 : 1), db_reads = 2 * NI * (BCOL ? 2 : 1), first = db_reads + da_reads / MI * (MI > 1 ? 2 : 1);
+      for (; s < steps - 2; ++s) {
+        turn();
+        pa += da; pb += db;
+        planes_step(lds + (s & 1) * kStepBytes, wm, wn, lane, acc);
+        planes_load(pa, pb, lds + (~s & 1) * kStepBytes, wave, oa, ob);
+        __builtin_amdgcn_sched_group_barrier(0x100, first, 0);
+        spread<0, 3 * MI * NI, da_reads + db_reads - first, kEven ? kPerStep : 0>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      for (; s < steps; ++s) {  // the last step may be short: its chunks past K are masked
+        turn();
+        if (s + 1 < steps) {
+          pa += da; pb += db;
+          offsets(A, B, wave, lane, K - (s + 1) * kStepK, oa, ob);
+          planes_load(pa, pb, lds + (~s & 1) * kStepBytes, wave, oa, ob);
+        }
+        planes_step(lds + (s & 1) * kStepBytes, wm, wn, lane, acc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // the caller may reuse the LDS
     asm volatile("" ::: "memory");
   }
 };

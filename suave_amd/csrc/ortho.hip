@@ -185,8 +185,8 @@ __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
 template <int NP, int BM, int WM, int WN, int POLY>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN, 2> R;
-  typedef Tile<kF16, NP, true, true, BM, BM, WM, WN, 2> C;
+  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> R;
+  typedef Tile<kF16, NP, true, true, BM, BM, WM, WN> C;
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int s = min(m.rows, m.cols), T = (s + BM - 1) / BM;
@@ -248,8 +248,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
 template <int NP, int BM, int WM, int WN, bool LAST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_update(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  typedef Tile<kF16, NP, false, true, BM, BM, WM, WN, 2> W;
-  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN, 2> H;
+  typedef Tile<kF16, NP, false, true, BM, BM, WM, WN> W;
+  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> H;
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int s = min(m.rows, m.cols);
@@ -363,17 +363,17 @@ template <int NP, int POLY>
 int launch_sym(Group& g, hipStream_t s) {
   const int bm = pick_tile(g, sym_tiles);
   const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), bm); return T * (T + 1) / 2; });
-  if (bm == 256) return launch(k_ortho_sym<NP, 256, 2, 4, POLY>, g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4, 2>::kLds, s);
-  if (bm == 128) return launch(k_ortho_sym<NP, 128, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2, 2>::kLds, s);
-  return launch(k_ortho_sym<NP, 64, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2, 2>::kLds, s);
+  if (bm == 256) return launch(k_ortho_sym<NP, 256, 2, 4, POLY>, g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4>::kLds, s);
+  if (bm == 128) return launch(k_ortho_sym<NP, 128, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2>::kLds, s);
+  return launch(k_ortho_sym<NP, 64, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2>::kLds, s);
 }
 template <int NP, bool LAST>
 int launch_update(Group& g, hipStream_t s) {
   const int bm = pick_tile(g, all_tiles);
   const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, bm) * ceil_div(m.cols, bm); });
-  if (bm == 256) return launch(k_ortho_update<NP, 256, 2, 4, LAST>, g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4, 2>::kLds, s);
-  if (bm == 128) return launch(k_ortho_update<NP, 128, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2, 2>::kLds, s);
-  return launch(k_ortho_update<NP, 64, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2, 2>::kLds, s);
+  if (bm == 256) return launch(k_ortho_update<NP, 256, 2, 4, LAST>, g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4>::kLds, s);
+  if (bm == 128) return launch(k_ortho_update<NP, 128, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2>::kLds, s);
+  return launch(k_ortho_update<NP, 64, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2>::kLds, s);
 }
 
 template <int NP>

@@ -349,8 +349,8 @@ int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
   if (a.M <= 16) hipLaunchKernelGGL(k_linear_rows<1>, dim3(blocks), dim3(256), 0, s, a);
   else if (a.M <= 32) hipLaunchKernelGGL(k_linear_rows<2>, dim3(blocks), dim3(256), 0, s, a);
   else if (a.M <= 64) hipLaunchKernelGGL(k_linear_rows<4>, dim3(blocks), dim3(256), 0, s, a);
-  else if ((a.M + 255) / 256 * ((a.N + 255) / 256) >= 256) return launch_tile<Tile<kI8, 1, false, false, 256, 256, 2, 4, 2>>(a, s);
-  else return launch_tile<Tile<kI8, 1, false, false, 128, 128, 2, 2, 2>>(a, s);
+  else if ((a.M + 255) / 256 * ((a.N + 255) / 256) >= 256) return launch_tile<Tile<kI8, 1, false, false, 256, 256, 2, 4>>(a, s);
+  else return launch_tile<Tile<kI8, 1, false, false, 128, 128, 2, 2>>(a, s);
   SUAVE_CHECK_HIP(hipGetLastError());
   return 0;
 }
