@@ -20,6 +20,7 @@
 
 #include "kernels.h"
 #include "mma.h"
+#include "tiles.h"
 
 namespace suave {
 
@@ -29,14 +30,15 @@ using namespace mma;
 
 constexpr int kStrip = 64;          // classes of one (max, sum) pair
 constexpr int kClassPad = 256;      // bias and G are padded to whole tiles of classes
-constexpr int kAmaxBlocks = 256;    // partial maxima per tensor
-constexpr int kCUs = 256;
+constexpr int kAmaxBlocks = 512;    // partial maxima per tensor
+constexpr int64_t kScanElems = 65536;  // x and W together: up to here every packing block finds the maximum itself (a launch less)
 constexpr size_t kPieceBytes = (size_t)192 << 20;  // G of one piece: what the 256 MB memory-side cache holds beside its operands
 
 struct Scalars {
   float x_scale, w_scale;    // powers of two the planes were multiplied by (1 for bf16)
-  float g_unit;              // loss_scale * max|w| / total / kGScale: what one unit of the stored G is worth
-  float max_w;
+  float g_unit;              // loss_scale * max_w / total / g_scale: what one unit of the stored G is worth
+  float max_w;               // largest |class weight| (1 for bf16 and without class weights): G is stored relative to it
+  uint32_t ticket;           // blocks of k_lce_rows that have written their partial sums
 };
 
 // G is stored relative to the largest row weight (entries in [-1, 1]) times 2^14: fp16's hi plane is normal down to 2^-28
@@ -51,7 +53,9 @@ struct PackArgs {
   int blocks0;               // blocks of tensor 0
   int D, Dp;
   const int32_t* targets;    // rows of tensor 0 with a negative target are zero
-  float* amax;               // [2][kAmaxBlocks]
+  float* amax;               // [3][kAmaxBlocks]: x, W, class weights
+  int scan;                  // no k_lce_amax launch: the blocks look for the maxima themselves
+  const float* class_weight;
   Scalars* scal;
   const float* bias;         // null: zero
   float* bias_pad;           // [round_up(C, kClassPad)], -inf past C
@@ -61,39 +65,71 @@ struct PackArgs {
 __device__ __forceinline__ float load_as_float(const float* p) { return *p; }
 __device__ __forceinline__ float load_as_float(const uint16_t* p) { return bf16_value(*p); }
 
-// largest finite |value| of x (rows that count) and W, in kAmaxBlocks partials each
-__global__ __launch_bounds__(256) void k_lce_amax(PackArgs a) {
-  __shared__ float part[4];
-  const int t = blockIdx.x >= kAmaxBlocks;
+__device__ __forceinline__ float finite_abs(float v) {
+  v = fabsf(v);
+  return v < INFINITY ? v : 0.f;  // (a NaN compares false)
+}
+
+// largest finite |value| of rows first, first + step, ...: of x (rows that count) or W, this thread's share
+__device__ __forceinline__ float scan_rows(const PackArgs& a, int t, int64_t first, int64_t step) {
   const float* src = static_cast<const float*>(a.src[t]);
   const int64_t rows = a.rows[t], ld = a.ld[t];
-  const int b = blockIdx.x - t * kAmaxBlocks;
   float m = 0.f;
-  // a wave per row piece: D may be anything from 1 on, so the flat element range is walked with 64-bit division-free steps
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (a.D >= 64) {
-    for (int64_t r = (int64_t)b * 4 + wave; r < rows; r += (int64_t)kAmaxBlocks * 4) {
-      if (t == 0 && a.targets[r] < 0) continue;
-      const float* p = src + r * ld;
-      for (int d = lane; d < a.D; d += 64) {
-        const float v = fabsf(p[d]);
-        if (v < INFINITY) m = fmaxf(m, v);
-      }
+  if (t == 1 && ld == a.D && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {  // one flat array: `first` / `step` are threads
+    const int64_t total = rows * ld, quads = total / 4;
+    const float4* p = reinterpret_cast<const float4*>(src);
+    int64_t e = first;
+    for (; e + 3 * step < quads; e += 4 * step) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = p[e + u * step];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)), fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
     }
-  } else {  // narrow rows: lanes over rows
-    for (int64_t r = ((int64_t)b * 4 + wave) * 64 + lane; r < rows; r += (int64_t)kAmaxBlocks * 256) {
+    for (; e < quads; e += step) {
+      const float4 v = p[e];
+      m = fmaxf(m, fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
+    }
+    if (first < total - 4 * quads) m = fmaxf(m, finite_abs(src[4 * quads + first]));
+    return m;
+  }
+  if (a.D >= 64) {  // a wave per row
+    const int lane = (int)(first & 63);
+    for (int64_t r = first >> 6; r < rows; r += step >> 6) {
       if (t == 0 && a.targets[r] < 0) continue;
       const float* p = src + r * ld;
-      for (int d = 0; d < a.D; ++d) {
-        const float v = fabsf(p[d]);
-        if (v < INFINITY) m = fmaxf(m, v);
-      }
+      for (int d = lane; d < a.D; d += 64) m = fmaxf(m, finite_abs(p[d]));
+    }
+  } else {  // narrow rows: a thread per row
+    for (int64_t r = first; r < rows; r += step) {
+      if (t == 0 && a.targets[r] < 0) continue;
+      const float* p = src + r * ld;
+      for (int d = 0; d < a.D; ++d) m = fmaxf(m, finite_abs(p[d]));
     }
   }
+  return m;
+}
+__device__ __forceinline__ float block_max(float m, float* part) {  // 256 threads; every thread gets the maximum
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if (lane == 0) part[wave] = m;
   __syncthreads();
-  if (threadIdx.x == 0) a.amax[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+__global__ __launch_bounds__(256) void k_lce_amax(PackArgs a) {
+  __shared__ float part[4];
+  const int t = (int)blockIdx.x >= kAmaxBlocks, b = blockIdx.x - t * kAmaxBlocks;
+  const int64_t first = (int64_t)b * 256 + threadIdx.x, step = (int64_t)kAmaxBlocks * 256;
+  const float m = block_max(scan_rows(a, t, first, step), part);
+  if (threadIdx.x == 0) a.amax[blockIdx.x] = m;
+  if (t == 0) {
+    float w = 0.f;
+    if (a.class_weight)
+      for (int64_t c = first; c < a.C; c += step) w = fmaxf(w, finite_abs(a.class_weight[c]));
+    w = block_max(w, part);
+    if (threadIdx.x == 0) a.amax[2 * kAmaxBlocks + b] = w;
+  }
 }
 
 // the power of two that brings amax into [2^13, 2^14) (products of two such and their sums stay far inside binary32)
@@ -108,20 +144,33 @@ template <class T, bool PLANES>
 __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
   const int t = (int)blockIdx.x >= a.blocks0;
   const int b = blockIdx.x - (t ? a.blocks0 : 0), nb = t ? (int)gridDim.x - a.blocks0 : a.blocks0;
-  float scale = 1.0f;
+  float scale = 1.0f, max_w = 1.0f;
   if constexpr (PLANES) {
-    __shared__ float sc;
-    const int lane = threadIdx.x & 63;
-    if (threadIdx.x < 64) {
-      float m = 0.f;
-      for (int i = lane; i < kAmaxBlocks; i += 64) m = fmaxf(m, a.amax[t * kAmaxBlocks + i]);
-      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      if (lane == 0) sc = plane_scale(m);
+    __shared__ float part[4];
+    float m = 0.f, w = 0.f;
+    if (a.scan) {
+      m = scan_rows(a, t, threadIdx.x, 256);
+      if (t == 0 && a.class_weight)
+        for (int c = threadIdx.x; c < a.C; c += 256) w = fmaxf(w, finite_abs(a.class_weight[c]));
+    } else {
+      for (int i = threadIdx.x; i < kAmaxBlocks; i += 256) {
+        m = fmaxf(m, a.amax[t * kAmaxBlocks + i]);
+        w = fmaxf(w, a.amax[2 * kAmaxBlocks + i]);
+      }
     }
-    __syncthreads();
-    scale = sc;
+    scale = plane_scale(block_max(m, part));
+    w = block_max(w, part);
+    max_w = a.class_weight && w > 0.f ? w : 1.0f;
   }
-  if (b == 0 && threadIdx.x == 0) (t ? a.scal->w_scale : a.scal->x_scale) = scale;
+  if (b == 0 && threadIdx.x == 0) {
+    if (t == 0) {
+      a.scal->x_scale = scale;
+      a.scal->max_w = max_w;
+      a.scal->ticket = 0;
+    } else {
+      a.scal->w_scale = scale;
+    }
+  }
   if (t) {
     for (int64_t c = (int64_t)b * 256 + threadIdx.x; c < a.C_pad; c += (int64_t)nb * 256)
       a.bias_pad[c] = c < a.C ? (a.bias ? a.bias[c] : 0.f) : -INFINITY;
@@ -166,7 +215,7 @@ struct LogitArgs {
   float2* strips;                  // [strip][n] (max, sum exp(l - max))
   float* target_logit;             // [n]
   // second sweep
-  const float2* row;               // (lse, row weight / max weight)
+  const float2* row;               // (lse, row weight / largest class weight)
   char* g; int64_t ldg; uint32_t g_plane;  // [n][c1 - c0 rounded up], bytes
   float* db;                       // [row tiles of a wave][C_pad]
   int64_t db_ld;
@@ -282,26 +331,29 @@ struct RowArgs {
   const float* target_logit;
   float* row_loss;   // or null
   float* lse_out;    // or null
-  float2* row;       // (lse, w)
+  float2* row;       // (lse, w / max_w)
   double* part;      // [blocks][2]: sum of ce, sum of w over the block's rows
-  float* part_max;   // [blocks]
   const float* weight_sum; float loss_scale, loss_rows; float gs;
   float* loss; double* loss_sum; Scalars* scal;
 };
 
-// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights
+// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights; the block that is done
+// last adds up the partial sums of all blocks, in their order
 __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
   __shared__ float2 ms[64][17];
+  __shared__ double sce[16], sw[16];
+  __shared__ int last;
   const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int64_t m = (int64_t)blockIdx.x * 16 + r;
   float mx = -INFINITY, s = 0.f;
   if (m < a.n) {
-    for (int t0 = q; t0 < a.n_strips; t0 += 256) {  // four strips in flight
-      float2 v[4];
+    constexpr int U = 8;  // strips in flight
+    for (int t0 = q; t0 < a.n_strips; t0 += 64 * U) {
+      float2 v[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = t0 + 64 * u < a.n_strips ? a.strips[(int64_t)(t0 + 64 * u) * a.n + m] : make_float2(-INFINITY, 0.f);
+      for (int u = 0; u < U; ++u) v[u] = t0 + 64 * u < a.n_strips ? a.strips[(int64_t)(t0 + 64 * u) * a.n + m] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
         if (v[u].y == 0.f) continue;  // nothing of the strip counts (all -inf); NaN goes on
         const float nm = fmaxf(mx, v[u].x);
         s = s * (mx == -INFINITY ? 0.f : __expf(mx - nm)) + v[u].y * __expf(v[u].x - nm);
@@ -311,79 +363,70 @@ __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
   }
   ms[q][r] = make_float2(mx, s);
   __syncthreads();
-  double ce = 0.0, wsum = 0.0;
-  float wmax = 0.f;
-  if (threadIdx.x < 16 && m < a.n) {
-    float M = -INFINITY;
-    for (int k = 0; k < 64; ++k) M = fmaxf(M, ms[k][r].x);
-    float S = 0.f;
-    for (int k = 0; k < 64; ++k)
-      if (ms[k][r].y != 0.f) S += ms[k][r].y * __expf(ms[k][r].x - M);
-    const float lse = S == 0.f ? -INFINITY : M + logf(S);
-    const int y = a.targets[m];
-    float w = 0.f, l = 0.f;
-    if (y >= a.C) {
-      w = l = NAN;
-    } else if (y >= 0) {
-      w = a.class_weight ? a.class_weight[y] : 1.0f;
-      l = w == 0.f ? 0.f : w * (lse - a.target_logit[m]);
+  if (threadIdx.x < 64) {  // four lanes per row, 16 groups each
+    const int part = threadIdx.x >> 4;
+    float M = -INFINITY, S = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) M = fmaxf(M, ms[part * 16 + k][r].x);
+    M = fmaxf(M, __shfl_xor(M, 16, 64));
+    M = fmaxf(M, __shfl_xor(M, 32, 64));
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (ms[part * 16 + k][r].y != 0.f) S += ms[part * 16 + k][r].y * __expf(ms[part * 16 + k][r].x - M);
+    S += __shfl_xor(S, 16, 64);
+    S += __shfl_xor(S, 32, 64);
+    double ce = 0.0, wsum = 0.0;
+    if (part == 0 && m < a.n) {
+      const float lse = S == 0.f ? -INFINITY : M + logf(S);
+      const int y = a.targets[m];
+      float w = 0.f, l = 0.f;
+      if (y >= a.C) {
+        w = l = NAN;
+      } else if (y >= 0) {
+        w = a.class_weight ? a.class_weight[y] : 1.0f;
+        l = w == 0.f ? 0.f : w * (lse - a.target_logit[m]);
+      }
+      if (a.row_loss) a.row_loss[m] = l;
+      if (a.lse_out) a.lse_out[m] = lse;
+      a.row[m] = make_float2(lse, w / a.scal->max_w);
+      ce = l;
+      wsum = w;
     }
-    if (a.row_loss) a.row_loss[m] = l;
-    if (a.lse_out) a.lse_out[m] = lse;
-    a.row[m] = make_float2(lse, w);
-    ce = l;
-    wsum = w;
-    wmax = fabsf(w);
-  }
-  if (threadIdx.x < 64) {
     for (int off = 8; off > 0; off >>= 1) {
       ce += __shfl_xor(ce, off, 64);
       wsum += __shfl_xor(wsum, off, 64);
-      wmax = fmaxf(wmax, __shfl_xor(wmax, off, 64));
     }
     if (threadIdx.x == 0) {
       a.part[2 * blockIdx.x] = ce;
       a.part[2 * blockIdx.x + 1] = wsum;
-      a.part_max[blockIdx.x] = wmax;
+      // the partial sums are visible to the whole device before the ticket is, and to the last block behind it
+      last = __hip_atomic_fetch_add(&a.scal->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
     }
   }
-}
-
-__global__ __launch_bounds__(1024) void k_lce_total(RowArgs a, int n_part) {
-  __shared__ double sce[16], sw[16];
-  __shared__ float sm[16];
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double ce = 0.0, w = 0.0;
-  float m = 0.f;
-  for (int i = threadIdx.x; i < n_part; i += 1024) {
-    ce += a.part[2 * i];
-    w += a.part[2 * i + 1];
-    m = fmaxf(m, a.part_max[i]);
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) {
+    ce += __hip_atomic_load(&a.part[2 * i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    w += __hip_atomic_load(&a.part[2 * i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   for (int off = 32; off > 0; off >>= 1) {
     ce += __shfl_xor(ce, off, 64);
     w += __shfl_xor(w, off, 64);
-    m = fmaxf(m, __shfl_xor(m, off, 64));
   }
-  if ((threadIdx.x & 63) == 0) { sce[threadIdx.x >> 6] = ce; sw[threadIdx.x >> 6] = w; sm[threadIdx.x >> 6] = m; }
+  if ((threadIdx.x & 63) == 0) { sce[threadIdx.x >> 6] = ce; sw[threadIdx.x >> 6] = w; }
   __syncthreads();
   if (threadIdx.x == 0) {
     ce = w = 0.0;
-    m = 0.f;
-    for (int k = 0; k < 16; ++k) { ce += sce[k]; w += sw[k]; m = fmaxf(m, sm[k]); }
+    for (int k = 0; k < 16; ++k) { ce += sce[k]; w += sw[k]; }
     const double total = a.weight_sum ? (double)*a.weight_sum : w;
-    const double loss = total == 0.0 ? 0.0 : ce / total;  // (NaN stays NaN)
+    const bool none = total == 0.0;  // (NaN stays NaN)
+    const double loss = none ? 0.0 : ce / total;
     if (a.loss) *a.loss = (float)loss;
     if (a.loss_sum) *a.loss_sum += loss * (double)a.loss_rows;
-    const bool none = total == 0.0;
-    a.scal->max_w = m;
-    a.scal->g_unit = none ? 0.f : (float)((double)a.loss_scale * (double)m / total) / a.gs;
+    a.scal->g_unit = none ? 0.f : (float)((double)a.loss_scale * (double)a.scal->max_w / total / (double)a.gs);
   }
-}
-
-// row weights relative to the largest: G's entries then lie in [-1, 1] whatever the scale of the class weights
-__global__ __launch_bounds__(256) void k_lce_relative(float2* row, int64_t n, const Scalars* scal) {
-  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (m < n) row[m].y = scal->max_w > 0.f ? row[m].y / scal->max_w : row[m].y;
 }
 
 struct GradArgs {
@@ -421,13 +464,12 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads, 2) void k_lce_grad(GradArgs a) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
+__device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* lds) {
   const int tiles_m = (int)((a.M + T::BM - 1) / T::BM), tiles_n = (a.N + T::BN - 1) / T::BN;
   const int per = tiles_m * tiles_n;
-  const int split = blockIdx.x / per;
+  const int split = block / per;
   int tm, tn;
-  tile_of(blockIdx.x - split * per, per, tiles_m, tiles_n, a.group, tm, tn);
+  tile_of(block - split * per, per, tiles_m, tiles_n, a.group, tm, tn);
   const int64_t m_base = (int64_t)tm * T::BM;
   const int n_base = tn * T::BN;
   const int kper = ((a.K + a.splits - 1) / a.splits + 63) / 64 * 64;
@@ -464,6 +506,14 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_grad(GradArgs a) {
       }
     }
   }
+}
+
+// dx and dW of one piece of the classes in one launch: they only share G
+template <class TX, class TW>
+__global__ __launch_bounds__(TX::kThreads, 2) void k_lce_grads(GradArgs dx, GradArgs dw, int dx_blocks) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  if ((int)blockIdx.x < dx_blocks) grad_tile<TX>(dx, blockIdx.x, lds);
+  else grad_tile<TW>(dw, blockIdx.x - dx_blocks, lds);
 }
 
 struct FinishArgs {  // out = factor * sum over the slabs, for dx and dW; db = unit * sum over the row tiles
@@ -510,19 +560,18 @@ __global__ __launch_bounds__(256) void k_lce_finish(FinishArgs a) {
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 struct Layout {  // offsets into the workspace, bytes
-  size_t scal, amax, bias, xp, wp, strips, target, row, part, part_max, g, db, dx_slab, dw_slab, total;
+  size_t scal, amax, bias, xp, wp, strips, target, row, part, g, db, dx_slab, dw_slab, total;
   int Dp, C_pad, n_strips, piece, pieces;
   int dx_splits, dw_splits;
   int64_t ldp, ldg;      // bytes
   uint32_t plane, g_plane;
   bool pack_w, dw_direct;
-  int big;               // tile size of the gradient products: 256, 128 or 64
+  TileId grad_tile;
   int row_blocks, db_rows;
   int tile_s, tile_g;    // LogitTile of the two sweeps (one per call: the db partials of all pieces have the same rows)
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile height and width of the logit products.  Up to 16 and 64 rows the tile is as low as the batch and 256 classes wide
 // (the weights stream past once; a taller tile would multiply rows that are not there); otherwise 256 x 256 with eight
@@ -534,10 +583,28 @@ LogitTile logit_tile(int64_t n, int64_t classes) {
   return ceil_div(n, 256) * ceil_div(classes, 256) >= kCUs ? kBig256 : kMid128;
 }
 
-// Splits of a product of M x N tiles over its K range: enough blocks for two per CU, at least 512 values of K each
-int splits_for(int64_t M, int64_t N, int64_t K, int tile) {
-  const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2 * kCUs, tiles), K / 512, 32}));
+// Tile and K splits of the two gradient products of a piece.  A split takes whole multiples of 64 values of K, so a product of
+// K values has at most K / 64 of them; dW is not split when the classes come in several pieces (its rows are then plenty).
+void pick_grad(int64_t n, int cp, int dim, int planes, bool dx, bool dw, bool one_piece, Layout& L) {
+  double best = 1e30;
+  const int step = planes == 2 ? 32 : 64;
+  for (int t = 0; t < kTileIds; ++t) {
+    Work w[2];
+    int count = 0, at_dx = -1, at_dw = -1;
+    if (dx) { at_dx = count; w[count++] = {ceil_div(n, kTileM[t]) * ceil_div(dim, kTileN[t]), ceil_div(cp, step), 4.0 * n * dim}; }
+    if (dw) { at_dw = count; w[count++] = {ceil_div(cp, kTileM[t]) * ceil_div(dim, kTileN[t]), ceil_div(n, step), 4.0 * cp * dim}; }
+    for (int sx = 1; sx <= (dx ? 32 : 1); sx *= 2) {
+      if (sx > 1 && sx * 64 > cp) break;
+      for (int sw = 1; sw <= (dw && one_piece ? 32 : 1); sw *= 2) {
+        if (sw > 1 && sw * 64 > n) break;
+        int split[2] = {1, 1};
+        if (at_dx >= 0) split[at_dx] = sx;
+        if (at_dw >= 0) split[at_dw] = sw;
+        const double us = estimate_us((TileId)t, planes, w, split, count);
+        if (us < best * 0.98) { best = us; L.grad_tile = (TileId)t; L.dx_splits = sx; L.dw_splits = sw; }
+      }
+    }
+  }
 }
 
 void make_layout(const suave_linear_ce_t& h, Layout& L) {
@@ -559,11 +626,10 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.pieces = (int)ceil_div(L.C_pad, L.piece);
   L.ldg = (int64_t)L.piece * 2 * np;
   L.g_plane = (uint32_t)(L.piece * 2);
-  const int64_t gt256 = ceil_div(std::min<int64_t>(L.piece, h.n_classes), 256) * ceil_div(h.dim, 256);
-  L.big = gt256 >= kCUs ? 256 : (n >= 256 || L.piece >= 1024) && h.dim > 64 ? 128 : 64;
   const int cp = std::min(L.piece, (int)h.n_classes);
-  L.dx_splits = splits_for(n, h.dim, cp, std::min(L.big, 128));
-  L.dw_splits = L.pieces > 1 ? 1 : splits_for(cp, h.dim, n, L.big);
+  L.grad_tile = kT64;
+  L.dx_splits = L.dw_splits = 1;
+  if (h.dx || h.dweight) pick_grad(n, cp, h.dim, np, h.dx != nullptr, h.dweight != nullptr, L.pieces == 1, L);
   L.dw_direct = L.dw_splits == 1;
   L.tile_s = logit_tile(n, h.n_classes);
   L.tile_g = logit_tile(n, cp);
@@ -572,7 +638,7 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
   L.scal = take(sizeof(Scalars));
-  L.amax = take(sizeof(float) * 2 * kAmaxBlocks);
+  L.amax = take(sizeof(float) * 3 * kAmaxBlocks);
   L.bias = take(sizeof(float) * L.C_pad);
   L.xp = take((size_t)n * L.ldp);
   L.wp = L.pack_w ? take((size_t)h.n_classes * L.ldp) : 0;
@@ -580,7 +646,6 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.target = take(sizeof(float) * n);
   L.row = take(sizeof(float2) * n);
   L.part = take(sizeof(double) * 2 * L.row_blocks);
-  L.part_max = take(sizeof(float) * L.row_blocks);
   L.g = L.db = L.dx_slab = L.dw_slab = 0;
   if (grad) {
     L.g = take((size_t)n * L.ldg);
@@ -630,21 +695,24 @@ int launch_logits(const LogitArgs& a, int tile, hipStream_t s) {
   }
 }
 
-template <int TYPE, int NP, bool ACOL>
-int launch_grad(const GradArgs& g, int tile, hipStream_t s) {
-  GradArgs a = g;
-  a.group = 8;
-  void* args[] = {&a};
-  const int64_t grid = ceil_div(a.M, tile) * ceil_div(a.N, tile) * a.splits;
-  if (tile == 256) {
-    typedef Tile<TYPE, NP, ACOL, true, 256, 256, 2, 4> T;
-    return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
-  } else if (tile == 128) {
-    typedef Tile<TYPE, NP, ACOL, true, 128, 128, 2, 2> T;
-    return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
+template <int TYPE, int NP, int BM, int BN, int WM, int WN>
+int launch_grads_tile(GradArgs dx, GradArgs dw, hipStream_t s) {
+  typedef Tile<TYPE, NP, false, true, BM, BN, WM, WN> X;
+  typedef Tile<TYPE, NP, true, true, BM, BN, WM, WN> W;
+  dx.group = dw.group = 8;
+  int dx_blocks = (int)(ceil_div(dx.M, BM) * ceil_div(dx.N, BN) * dx.splits);  // (M = 0: not wanted)
+  const int blocks = dx_blocks + (int)(ceil_div(dw.M, BM) * ceil_div(dw.N, BN) * dw.splits);
+  void* args[] = {&dx, &dw, &dx_blocks};
+  return launch_tile<X>(reinterpret_cast<const void*>(k_lce_grads<X, W>), blocks, args, s);
+}
+template <int TYPE, int NP>
+int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, hipStream_t s) {
+  switch (tile) {
+    case kT64: return launch_grads_tile<TYPE, NP, 64, 64, 2, 2>(dx, dw, s);
+    case kT64x128: return launch_grads_tile<TYPE, NP, 64, 128, 2, 2>(dx, dw, s);
+    case kT128: return launch_grads_tile<TYPE, NP, 128, 128, 2, 2>(dx, dw, s);
+    default: return launch_grads_tile<TYPE, NP, 256, 256, 2, 4>(dx, dw, s);
   }
-  typedef Tile<TYPE, NP, ACOL, true, 64, 64, 2, 2> T;
-  return launch_tile<T>(reinterpret_cast<const void*>(k_lce_grad<T>), (int)grid, args, s);
 }
 
 template <int TYPE, int NP>
@@ -658,8 +726,10 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   p.src[0] = h.x; p.src[1] = h.weight; p.ld[0] = h.ld_x; p.ld[1] = h.ld_weight; p.rows[0] = n; p.rows[1] = h.n_classes;
   p.dst[0] = ws + L.xp; p.dst[1] = L.pack_w ? ws + L.wp : nullptr; p.dst_ld[0] = p.dst_ld[1] = L.ldp;
   p.D = h.dim; p.Dp = L.Dp; p.targets = h.targets; p.amax = reinterpret_cast<float*>(ws + L.amax); p.scal = scal;
+  p.class_weight = F ? h.class_weight : nullptr;
+  p.scan = (n + h.n_classes) * h.dim <= kScanElems;
   p.bias = h.bias; p.bias_pad = reinterpret_cast<float*>(ws + L.bias); p.C = h.n_classes; p.C_pad = L.C_pad;
-  if (F) {
+  if (F && !p.scan) {
     hipLaunchKernelGGL(k_lce_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, s, p);
     SUAVE_CHECK_HIP(hipGetLastError());
   }
@@ -685,15 +755,11 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
   r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
   r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part);
-  r.part_max = reinterpret_cast<float*>(ws + L.part_max); r.weight_sum = h.weight_sum; r.loss_scale = h.loss_scale;
+  r.weight_sum = h.weight_sum; r.loss_scale = h.loss_scale;
   r.loss_rows = h.loss_rows; r.gs = g_scale(F); r.loss = h.loss; r.loss_sum = h.loss_sum; r.scal = scal;
   hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
   SUAVE_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(1024), 0, s, r, L.row_blocks);
-  SUAVE_CHECK_HIP(hipGetLastError());
   if (!grad) return 0;
-  hipLaunchKernelGGL(k_lce_relative, dim3((int)ceil_div(n, 256)), dim3(256), 0, s, r.row, n, scal);
-  SUAVE_CHECK_HIP(hipGetLastError());
 
   const bool bf = !F;
   auto vec_ok = [&](const void* ptr, int64_t ld) {
@@ -707,17 +773,17 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
     if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
     const int cp = a.c1 - a.c0;
+    GradArgs gx{}, gw{};
     if (h.dx) {
-      GradArgs g{};
+      GradArgs& g = gx;
       g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
       g.b = a.w + (int64_t)a.c0 * a.ldw; g.ldb = a.ldw; g.b_plane = L.plane;
       g.M = n; g.N = h.dim; g.K = cp; g.splits = L.dx_splits;
       g.slab = reinterpret_cast<float*>(ws + L.dx_slab); g.slab_stride = n * L.Dp; g.ld_slab = L.Dp; g.accumulate = piece > 0;
       g.scal = scal; g.which = 0;
-      if (int rc = launch_grad<TYPE, NP, false>(g, std::min(L.big, 128), s)) return rc;
     }
     if (h.dweight) {
-      GradArgs g{};
+      GradArgs& g = gw;
       g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
       g.b = a.x; g.ldb = L.ldp; g.b_plane = L.plane;
       g.M = cp; g.N = h.dim; g.K = (int)n; g.splits = L.dw_splits;
@@ -727,8 +793,9 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
       g.out = static_cast<char*>(h.dweight) + (int64_t)a.c0 * h.ld_dweight * (bf ? 2 : 4); g.ld_out = h.ld_dweight;
       g.out_bf16 = bf; g.out_vec = vec_ok(h.dweight, h.ld_dweight);
       g.scal = scal; g.which = 1;
-      if (int rc = launch_grad<TYPE, NP, true>(g, L.big, s)) return rc;
     }
+    if (h.dx || h.dweight)
+      if (int rc = launch_grads<TYPE, NP>(gx, gw, L.grad_tile, s)) return rc;
   }
   FinishArgs f{};
   f.scal = scal; f.out_bf16 = bf; f.ld_slab = L.Dp; f.N = h.dim; f.gs = g_scale(F);

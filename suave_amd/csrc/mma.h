@@ -75,9 +75,12 @@ __device__ __forceinline__ void dma16_scheduled(const char* base, uint32_t voff,
 // The same, written as an instruction because the compiler, which would
 // otherwise know of the transfer, waits for ALL transfers before any transposed LDS read (8192 x 8192 x 4096 bf16 with a
 // column-form operand: 569 us, against 457 us).  It has no result register; callers wait by vmcnt and a barrier before the LDS is read.
-// The wait states cover m0 and a resource that a vector instruction has just written.
+// The wait states cover m0 and a resource that a vector instruction has just written; m0 is given back as it was.
 __device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "m0");
+  uint32_t keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "s"(lds), "v"(voff), "s"(rsrc));
 }
 
 // The staging of one operand: EXT rows (row form) or columns (column form) of a tile, NP planes, by NW waves.
