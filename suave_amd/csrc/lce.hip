@@ -670,10 +670,10 @@ int check_args(const suave_linear_ce_t* h) {
   return 0;
 }
 
-template <class T>
-int launch_tile(const void* fn, int grid, void** args, hipStream_t s) {
-  if (T::kLds > 64 * 1024) SUAVE_CHECK_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
-  SUAVE_CHECK_HIP(hipLaunchKernel(fn, dim3(grid), dim3(T::kThreads), args, T::kLds, s));
+// `done`: per kernel, a static of the caller (allow_lds)
+int launch_tile(const void* fn, int grid, int threads, int lds, void** args, std::atomic<uint64_t>& done, hipStream_t s) {
+  SUAVE_CHECK_HIP(allow_lds(fn, lds, done));
+  SUAVE_CHECK_HIP(hipLaunchKernel(fn, dim3(grid), dim3(threads), args, lds, s));
   return 0;
 }
 
@@ -682,7 +682,8 @@ int launch_logits_tile(LogitArgs a, hipStream_t s) {
   const int64_t grid = ceil_div(a.n, T::BM) * ceil_div(a.c1 - a.c0, T::BN);
   a.group = 8;
   void* args[] = {&a};
-  return launch_tile<T>(reinterpret_cast<const void*>(k_lce_logits<T, SWEEP>), (int)grid, args, s);
+  static std::atomic<uint64_t> done{0};
+  return launch_tile(reinterpret_cast<const void*>(k_lce_logits<T, SWEEP>), (int)grid, T::kThreads, T::kLds, args, done, s);
 }
 
 template <int TYPE, int NP, int SWEEP>
@@ -703,7 +704,8 @@ int launch_grads_tile(GradArgs dx, GradArgs dw, hipStream_t s) {
   int dx_blocks = (int)(ceil_div(dx.M, BM) * ceil_div(dx.N, BN) * dx.splits);  // (M = 0: not wanted)
   const int blocks = dx_blocks + (int)(ceil_div(dw.M, BM) * ceil_div(dw.N, BN) * dw.splits);
   void* args[] = {&dx, &dw, &dx_blocks};
-  return launch_tile<X>(reinterpret_cast<const void*>(k_lce_grads<X, W>), blocks, args, s);
+  static std::atomic<uint64_t> done{0};
+  return launch_tile(reinterpret_cast<const void*>(k_lce_grads<X, W>), blocks, X::kThreads, X::kLds, args, done, s);
 }
 template <int TYPE, int NP>
 int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, hipStream_t s) {

@@ -25,6 +25,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace suave {
 namespace mma {
 
@@ -375,6 +377,18 @@ __device__ __forceinline__ void planes(float x, uint16_t& hi, uint16_t& lo) {
   const float r = x - (float)h;
   hi = f16_bits(h);
   lo = __builtin_isinf((float)h) ? 0 : f16_bits((_Float16)r);
+}
+
+// Dynamic LDS beyond 64 KB has to be allowed once per kernel and device; `done` is the caller's record for one kernel.
+inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  if (bytes <= 64 * 1024) return hipSuccess;
+  int dev = 0;
+  if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return hipSuccess;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 }  // namespace mma

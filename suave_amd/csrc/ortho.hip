@@ -340,9 +340,10 @@ int pick_tile(const Group& g, F tiles) {
   return 64;
 }
 
-template <class K>
-int launch(K kernel, Group& g, int grid, int threads, int lds, hipStream_t s) {
-  if (lds > 64 * 1024) SUAVE_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+template <auto kernel>
+int launch(Group& g, int grid, int threads, int lds, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  SUAVE_CHECK_HIP(allow_lds(reinterpret_cast<const void*>(kernel), lds, done));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
   return 0;
@@ -363,17 +364,17 @@ template <int NP, int POLY>
 int launch_sym(Group& g, hipStream_t s) {
   const int bm = pick_tile(g, sym_tiles);
   const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), bm); return T * (T + 1) / 2; });
-  if (bm == 256) return launch(k_ortho_sym<NP, 256, 2, 4, POLY>, g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4>::kLds, s);
-  if (bm == 128) return launch(k_ortho_sym<NP, 128, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2>::kLds, s);
-  return launch(k_ortho_sym<NP, 64, 2, 2, POLY>, g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2>::kLds, s);
+  if (bm == 256) return launch<k_ortho_sym<NP, 256, 2, 4, POLY>>(g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4>::kLds, s);
+  if (bm == 128) return launch<k_ortho_sym<NP, 128, 2, 2, POLY>>(g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2>::kLds, s);
+  return launch<k_ortho_sym<NP, 64, 2, 2, POLY>>(g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2>::kLds, s);
 }
 template <int NP, bool LAST>
 int launch_update(Group& g, hipStream_t s) {
   const int bm = pick_tile(g, all_tiles);
   const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, bm) * ceil_div(m.cols, bm); });
-  if (bm == 256) return launch(k_ortho_update<NP, 256, 2, 4, LAST>, g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4>::kLds, s);
-  if (bm == 128) return launch(k_ortho_update<NP, 128, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2>::kLds, s);
-  return launch(k_ortho_update<NP, 64, 2, 2, LAST>, g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2>::kLds, s);
+  if (bm == 256) return launch<k_ortho_update<NP, 256, 2, 4, LAST>>(g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4>::kLds, s);
+  if (bm == 128) return launch<k_ortho_update<NP, 128, 2, 2, LAST>>(g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2>::kLds, s);
+  return launch<k_ortho_update<NP, 64, 2, 2, LAST>>(g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2>::kLds, s);
 }
 
 template <int NP>

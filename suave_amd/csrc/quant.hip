@@ -272,8 +272,8 @@ template <class T>
 int launch_tile(ProductArgs a, hipStream_t s) {
   const int64_t grid = (a.M + T::BM - 1) / T::BM * ((a.N + T::BN - 1) / T::BN);
   a.group = 8;
-  if (T::kLds > 64 * 1024)
-    SUAVE_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_tile<T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds));
+  static std::atomic<uint64_t> done{0};
+  SUAVE_CHECK_HIP(allow_lds(reinterpret_cast<const void*>(k_linear_tile<T>), T::kLds, done));
   hipLaunchKernelGGL(k_linear_tile<T>, dim3((unsigned)grid), dim3(T::kThreads), T::kLds, s, a);
   SUAVE_CHECK_HIP(hipGetLastError());
   return 0;

@@ -10,6 +10,7 @@ outputs.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -25,14 +26,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _need(cond: bool, msg: str) -> None:
-    if not cond:
-        raise ValueError(msg)
-
-
+# The checks below run on every call of operators that take ten microseconds: they build a message only when they fail.
 def _device_of(name: str, t: torch.Tensor) -> torch.device:
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if not t.is_cuda:
         raise _lib.SuaveHipError(f"{name} must be on a GPU device (there is no CPU fallback)")
     return t.device
 
@@ -40,35 +38,63 @@ def _device_of(name: str, t: torch.Tensor) -> torch.device:
 def _matrix(name: str, t: torch.Tensor, dev: torch.device, dtypes, shape=None) -> int:
     """Checks a matrix whose rows are contiguous; returns its row stride in elements."""
 
-    _need(isinstance(t, torch.Tensor) and t.dim() == 2, f"{name} must be a matrix")
-    _need(t.device == dev, f"{name} must be on {dev}")
-    _need(t.dtype in dtypes, f"{name} must have one of the types {[str(d) for d in dtypes]}")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} must have the shape {shape}")
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must have one of the types {[str(d) for d in dtypes]}")
     rows, cols = t.shape
-    _need(cols <= 1 or t.stride(1) == 1, f"{name}: the elements of a row must be contiguous")
-    ld = int(t.stride(0)) if rows > 1 else max(int(cols), 1)
-    _need(ld >= cols, f"{name}: rows must not overlap")
-    return ld
+    if shape is not None and (rows, cols) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}")
+    s0, s1 = t.stride()
+    if s1 != 1 and cols > 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous")
+    if rows <= 1:
+        return cols or 1
+    if s0 < cols:
+        raise ValueError(f"{name}: rows must not overlap")
+    return s0
 
 
 def _vector(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype, n: int) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dim() == 1 and int(t.shape[0]) == n, f"{name} must be a vector of {n} values")
-    _need(t.device == dev, f"{name} must be on {dev}")
-    _need(t.dtype == dtype, f"{name} must have the type {dtype}")
-    _need(n <= 1 or t.stride(0) == 1, f"{name} must be contiguous")
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be a vector of {n} values")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must have the type {dtype}")
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must be contiguous")
 
 
 def _scalar(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
-    _need(isinstance(t, torch.Tensor) and t.numel() == 1 and t.device == dev and t.dtype == dtype,
-          f"{name} must be one {dtype} value on {dev}")
+    if not isinstance(t, torch.Tensor) or t.numel() != 1 or t.device != dev or t.dtype is not dtype:
+        raise ValueError(f"{name} must be one {dtype} value on {dev}")
 
 
-def _workspace(nbytes: int, dev: torch.device):
-    """(tensor, aligned address, bytes) of per-call scratch."""
+def _need(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
 
-    ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)
-    base = (ws.data_ptr() + 255) // 256 * 256
-    return ws, base, nbytes
+
+def _on(dev: torch.device):
+    """The device as the current one, where it is not."""
+
+    return _NOTHING if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_NOTHING = contextlib.nullcontext()
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
+    """Per-call scratch (torch's device allocations start at multiples of 512 bytes; the library checks for 256)."""
+
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
@@ -92,7 +118,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     n, d = int(x.shape[0]), int(x.shape[1])
     ld_w = _matrix("weight", weight, dev, (x.dtype,))
     c = int(weight.shape[0])
-    _need(int(weight.shape[1]) == d, f"weight must have {d} columns, as x")
+    if weight.shape[1] != d:
+        raise ValueError(f"weight must have {d} columns, as x")
     _need(c >= 1 and d >= 1, "weight must have at least one row and one column")
     _vector("targets", targets, dev, torch.int32, n)
     if bias is not None:
@@ -103,7 +130,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         _scalar("weight_sum", weight_sum, dev, torch.float32)
     if loss_sum is not None:
         _scalar("loss_sum", loss_sum, dev, torch.float64)
-    with torch.cuda.device(dev):
+    with _on(dev):
         out = {"loss": torch.empty((), dtype=torch.float32, device=dev),
                "row_loss": torch.empty(n, dtype=torch.float32, device=dev), "lse": torch.empty(n, dtype=torch.float32, device=dev)}
         h = LinearCeT()
@@ -111,9 +138,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
             out["dx"] = torch.empty((n, d), dtype=x.dtype, device=dev) if dx is None else dx
             out["dweight"] = torch.empty((c, d), dtype=x.dtype, device=dev) if dweight is None else dweight
             out["dbias"] = torch.empty(c, dtype=torch.float32, device=dev) if dbias is None else dbias
-            h.ld_dx = _matrix("dx", out["dx"], dev, (x.dtype,), (n, d))
-            h.ld_dweight = _matrix("dweight", out["dweight"], dev, (x.dtype,), (c, d))
-            _vector("dbias", out["dbias"], dev, torch.float32, c)
+            h.ld_dx = d if dx is None else _matrix("dx", dx, dev, (x.dtype,), (n, d))
+            h.ld_dweight = d if dweight is None else _matrix("dweight", dweight, dev, (x.dtype,), (c, d))
+            if dbias is not None:
+                _vector("dbias", dbias, dev, torch.float32, c)
             h.dx, h.dweight, h.dbias = (out[k].data_ptr() for k in ("dx", "dweight", "dbias"))
         else:
             _need(dx is None and dweight is None and dbias is None, "gradient buffers are given, but grad is False")
@@ -126,8 +154,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         lib = _lib.load()
         nbytes = C.c_size_t(0)
         _lib.check(lib.suave_linear_ce_workspace_bytes(C.byref(h), C.byref(nbytes)), "suave_linear_ce_workspace_bytes")
-        ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
-        _lib.check(lib.suave_linear_ce(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_ce")
+        ws = _workspace(nbytes.value, dev)
+        h.workspace, h.workspace_bytes = ws.data_ptr(), nbytes.value
+        _lib.check(lib.suave_linear_ce(C.byref(h), _stream(dev)), "suave_linear_ce")
     return out
 
 
@@ -145,7 +174,7 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, eps: floa
     _need(dt in _DTYPES, f"matrices must have one of the types {[str(d) for d in _DTYPES]}")
     lds = [_matrix(f"matrices[{i}]", t, dev, (dt,)) for i, t in enumerate(matrices)]
     _need(all(t.numel() > 0 for t in matrices), "a matrix needs at least one row and one column")
-    with torch.cuda.device(dev):
+    with _on(dev):
         if out is None:
             out = [torch.empty(t.shape, dtype=dt, device=dev) for t in matrices]
         out = list(out)
@@ -158,9 +187,9 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, eps: floa
         nbytes = C.c_size_t(0)
         _lib.check(lib.suave_orthogonalize_workspace_bytes(arr, len(matrices), _DTYPES[dt], C.byref(nbytes)),
                    "suave_orthogonalize_workspace_bytes")
-        ws, base, nb = _workspace(int(nbytes.value), dev)
-        _lib.check(lib.suave_orthogonalize(arr, len(matrices), _DTYPES[dt], int(steps), float(eps), base, nb,
-                                           torch.cuda.current_stream(dev).cuda_stream), "suave_orthogonalize")
+        ws = _workspace(nbytes.value, dev)
+        _lib.check(lib.suave_orthogonalize(arr, len(matrices), _DTYPES[dt], int(steps), float(eps), ws.data_ptr(), nbytes.value,
+                                           _stream(dev)), "suave_orthogonalize")
     return out
 
 
@@ -186,13 +215,13 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         a.ld_grad, a.ld_momentum = _matrix(f"grads[{i}]", g, dev, f32, p.shape), _matrix(f"momenta[{i}]", m, dev, f32, p.shape)
         a.param, a.grad, a.momentum = p.data_ptr(), g.data_ptr(), m.data_ptr()
         a.rows, a.cols, a.lr = int(p.shape[0]), int(p.shape[1]), lrs[i]
-    with torch.cuda.device(dev):
+    with _on(dev):
         lib = _lib.load()
         nbytes = C.c_size_t(0)
         _lib.check(lib.suave_muon_workspace_bytes(arr, n, C.byref(nbytes)), "suave_muon_workspace_bytes")
-        ws, base, nb = _workspace(int(nbytes.value), dev)
-        _lib.check(lib.suave_muon_step(arr, n, float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps), base, nb,
-                                       torch.cuda.current_stream(dev).cuda_stream), "suave_muon_step")
+        ws = _workspace(nbytes.value, dev)
+        _lib.check(lib.suave_muon_step(arr, n, float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps), ws.data_ptr(), nbytes.value,
+                                       _stream(dev)), "suave_muon_step")
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -204,11 +233,11 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     ld = _matrix("x", x, dev, tuple(_DTYPES))
     n, k = int(x.shape[0]), int(x.shape[1])
     _need(k >= 1, "x must have at least one column")
-    with torch.cuda.device(dev):
+    with _on(dev):
         q = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.int8, device=dev)
         scale = torch.empty(n, dtype=torch.float32, device=dev)
         _lib.check(_lib.load().suave_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], n, k, ld, q.data_ptr(), int(q.shape[1]),
-                                                   scale.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "suave_quantize_rows")
+                                                   scale.data_ptr(), _stream(dev)), "suave_quantize_rows")
     return q[:, :k], scale
 
 
@@ -224,27 +253,31 @@ def linear_quantized(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     n, k = int(x.shape[0]), int(x.shape[1])
     ldw = _matrix("weight", weight, dev, (torch.int8,))
     c = int(weight.shape[0])
-    _need(int(weight.shape[1]) == k, f"weight must have {k} columns, as x")
+    if weight.shape[1] != k:
+        raise ValueError(f"weight must have {k} columns, as x")
     _need(c >= 1 and k >= 1, "weight must have at least one row and one column")
     if c == 1:
         ldw = (k + 15) // 16 * 16
     _need(ldw % 16 == 0 and weight.data_ptr() % 16 == 0, "weight: rows must start at multiples of 16 bytes (quantize_rows)")
-    held = weight.untyped_storage().nbytes() - weight.storage_offset()
+    held = weight.untyped_storage().nbytes() - weight.storage_offset() if k % 16 else c * ldw
     _need(held >= (c - 1) * ldw + (k + 15) // 16 * 16, "weight: the last row must be held up to a multiple of 16 (quantize_rows)")
     _vector("weight_scale", weight_scale, dev, torch.float32, c)
     if bias is not None:
         _vector("bias", bias, dev, torch.float32, c)
-    with torch.cuda.device(dev):
+    with _on(dev):
+        h = LinearQuantizedT()
         if out is None:
             out = torch.empty((n, c), dtype=x.dtype, device=dev)
-        h = LinearQuantizedT()
-        h.ld_out = _matrix("out", out, dev, (x.dtype,), (n, c))
+            h.ld_out = c
+        else:
+            h.ld_out = _matrix("out", out, dev, (x.dtype,), (n, c))
         h.dtype, h.n_out, h.n_in, h.n_rows = _DTYPES[x.dtype], c, k, n
         h.x, h.ld_x, h.weight, h.ld_weight = x.data_ptr(), ld, weight.data_ptr(), ldw
         h.weight_scale, h.bias, h.out = weight_scale.data_ptr(), _ptr(bias), out.data_ptr()
         lib = _lib.load()
         nbytes = C.c_size_t(0)
         _lib.check(lib.suave_linear_quantized_workspace_bytes(C.byref(h), C.byref(nbytes)), "suave_linear_quantized_workspace_bytes")
-        ws, h.workspace, h.workspace_bytes = _workspace(int(nbytes.value), dev)
-        _lib.check(lib.suave_linear_quantized(C.byref(h), torch.cuda.current_stream(dev).cuda_stream), "suave_linear_quantized")
+        ws = _workspace(nbytes.value, dev)
+        h.workspace, h.workspace_bytes = ws.data_ptr(), nbytes.value
+        _lib.check(lib.suave_linear_quantized(C.byref(h), _stream(dev)), "suave_linear_quantized")
     return out
