@@ -95,6 +95,30 @@ __global__ __launch_bounds__(256) void k_ortho_norm(Group g) {
   if (threadIdx.x == 0) g.part[i * kNormBlocks + b] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+// from the sum of squares of U: what U is multiplied by to give the stored X_0, and the sizes e of X_0 .. X_steps
+__device__ __forceinline__ double start_scale(double sum, double eps, int steps, int* exps) {
+  const double norm = sqrt(sum), full = norm + eps;
+  double f = norm / full;  // |X_0|_F
+  int e0 = 0;
+  for (int k = 0; k <= steps; ++k) {
+    int e = 0;
+    if (f > 0.0 && f < 1.0) { (void)frexp(f, &e); e = max(e, -100); }
+    if (!(e < 0)) e = 0;
+    if (k == 0) e0 = e;
+    exps[k] = e;
+    f *= (double)kNsA;
+  }
+  return isfinite(sum) ? ldexp(1.0 / full, 12 - e0) : (double)NAN;  // anything not finite: the whole result is NaN
+}
+__device__ __forceinline__ void write_result(const Group& g, const Mat& m, int r, int c, float v) {
+  if (g.bf16) {
+    static_cast<uint16_t*>(m.out)[(int64_t)r * m.ld_out + c] = bf16_bits(v);
+  } else {
+    float* o = static_cast<float*>(m.out) + (int64_t)r * m.ld_out + c;
+    *o = g.muon ? fmaf(-m.lr, v, *o * m.decay) : v;
+  }
+}
+
 // X_0 in planes, pads zero; the sizes of X_0 .. X_steps
 template <int NP>
 __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
@@ -107,18 +131,10 @@ __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
     for (int k = threadIdx.x; k < kNormBlocks; k += 64) s += g.part[i * kNormBlocks + k];
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if (threadIdx.x == 0) {
-      const double norm = sqrt(s), full = norm + g.eps;
-      double f = norm / full;  // |X_0|_F
-      int e0 = 0;
-      for (int k = 0; k <= g.steps; ++k) {
-        int e = 0;
-        if (f > 0.0 && f < 1.0) { (void)frexp(f, &e); e = max(e, -100); }
-        if (!(e < 0)) e = 0;
-        if (k == 0) e0 = e;
-        if (b == 0) g.exps[i * (kMaxSteps + 1) + k] = e;
-        f *= (double)kNsA;
-      }
-      sc = isfinite(s) ? ldexp(1.0 / full, 12 - e0) : (double)NAN;  // anything not finite: the whole result is NaN
+      int e[kMaxSteps + 1];
+      sc = start_scale(s, g.eps, g.steps, e);
+      if (b == 0)
+        for (int k = 0; k <= g.steps; ++k) g.exps[i * (kMaxSteps + 1) + k] = e[k];
     }
   }
   __syncthreads();
@@ -283,16 +299,291 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_update(Group g) {
       for (int u = 0; u < 4; ++u) v[u] = acc[mi][j][u] * f;
       if constexpr (!LAST) {
         store_planes<NP>(m.x[(g.k & 1) ^ 1], px, m.cols, r, n, v);
-      } else if (g.bf16) {
-        uint16_t* o = static_cast<uint16_t*>(m.out) + (int64_t)r * m.ld_out + n;
-        for (int u = 0; u < 4; ++u)
-          if (n + u < m.cols) o[u] = bf16_bits(v[u]);
       } else {
-        float* o = static_cast<float*>(m.out) + (int64_t)r * m.ld_out + n;
         for (int u = 0; u < 4; ++u)
-          if (n + u < m.cols) o[u] = g.muon ? fmaf(-m.lr, v[u], o[u] * m.decay) : v[u];
+          if (n + u < m.cols) write_result(g, m, r, n + u, v[u]);
       }
     }
+  }
+}
+
+// ---- one block per matrix ------------------------------------------------------------------------------------------
+// A matrix whose planes fit a CU's LDS goes through the whole iteration in one launch: X (short side s in rows) and one s x s
+// buffer that holds A and then B stay in LDS, fp32 accumulators in registers.  What bounds it is the chain of barriers and LDS
+// reads, a few microseconds per step, instead of three launches per step; column strips of X are independent in X <- B X, so a
+// wave replaces its strips in place.  64 x 64 f32: SMALL_US us against SMALL_OLD us by launches.
+constexpr int kSmallWaves = 8;
+constexpr int kSmallLds = 156 * 1024;
+
+struct SmallShape {
+  int sp, lp, px, pa, bytes;  // padded sides, row pitches (bytes) of a plane of X and of A, LDS bytes
+};
+__host__ __device__ inline SmallShape small_shape(int rows, int cols, int np) {
+  SmallShape h;
+  const int s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+  h.sp = (s + 31) / 32 * 32;
+  h.lp = (l + 31) / 32 * 32;
+  // 32 bytes past a multiple of 128: four rows of a transposed read, and eight of a row read, fall on distinct banks
+  h.px = (h.lp * 2 + 127) / 128 * 128 + 32;
+  h.pa = (h.sp * 2 + 127) / 128 * 128 + 32;
+  h.bytes = h.sp > 128 || h.lp > 4096 ? 1 << 30 : np * h.sp * (h.px + h.pa) + kSmallWaves * 1024 + 512;
+  return h;
+}
+
+// fragment of 16 rows from row0, K values 32 kk ..: rows contiguous in K
+__device__ __forceinline__ i32x4 small_rows(const char* base, int pitch, int row0, int kk, int lane) {
+  return *reinterpret_cast<const i32x4*>(base + (row0 + (lane & 15)) * pitch + kk * 64 + (lane >> 4) * 16);
+}
+// fragment of 16 columns from col0, K = rows 32 kk ..
+__device__ __forceinline__ i32x4 small_cols(const char* base, int pitch, int col0, int kk, int lane) {
+  const int i = lane & 15, k = kk * 32 + 8 * (lane >> 4) + (i >> 2);
+  s16x4 v[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const char* p = base + (k + 4 * h) * pitch + (col0 + 4 * (i & 3)) * 2;
+    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_char*)const_cast<char*>(p));
+  }
+  const s16x8 w = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(i32x4, w);
+}
+template <int NP>
+__device__ __forceinline__ f32x4 small_mul(const i32x4 (&b)[NP], const i32x4 (&a)[NP], f32x4 c) {
+  if constexpr (NP == 2) {
+    c = mul<kF16>(b[1], a[0], c);
+    c = mul<kF16>(b[0], a[1], c);
+  }
+  return mul<kF16>(b[0], a[0], c);
+}
+// KA: 32-row blocks of the short side (1 .. 4)
+template <int NP, int KA>
+__device__ __forceinline__ void small_matrix(const Group& g, const Mat& m, char* lds) {
+  constexpr int T = 2 * KA, U = T * (T + 1) / 2;                                  // 16 x 16 tiles: per side, on and above the diagonal
+  constexpr int kSplit = U >= kSmallWaves ? 1 : kSmallWaves / U;                 // waves per tile of the Gram product
+  constexpr int kItems = (U + kSmallWaves - 1) / kSmallWaves;
+  constexpr int kThreads = 64 * kSmallWaves;
+  const int rows = m.rows, cols = m.cols;
+  const bool tall = rows > cols;
+  const int s = tall ? cols : rows;
+  const SmallShape h = small_shape(rows, cols, NP);
+  const int xplane = h.sp * h.px, aplane = h.sp * h.pa;
+  char* X = lds;
+  char* A = X + NP * xplane;
+  f32x4* part = reinterpret_cast<f32x4*>(A + NP * aplane);                       // [waves][64]
+  double* red = reinterpret_cast<double*>(part + kSmallWaves * 64);              // [waves]
+  double* scale_at = red + kSmallWaves;
+  int* exps = reinterpret_cast<int*>(scale_at + 1);                              // [kMaxSteps + 1]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  for (int i = tid; i < NP * (xplane + aplane) / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  // U as it is into X's place (binary32: upper halves in the first plane, lower halves in the second), its sum of squares;
+  // eight loads in flight per thread
+  const int total = rows * cols;
+  double ss = 0.0;
+  for (int e0 = tid; e0 < total; e0 += 8 * kThreads) {
+    float v[8], mo[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = e0 + u * kThreads, r = e / cols, c = e - r * cols;
+      v[u] = mo[u] = 0.f;
+      if (e < total) {
+        if (g.bf16) v[u] = bf16_value(static_cast<const uint16_t*>(m.in)[(int64_t)r * m.ld_in + c]);
+        else v[u] = static_cast<const float*>(m.in)[(int64_t)r * m.ld_in + c];
+        if (g.muon) mo[u] = m.mom[(int64_t)r * m.ld_mom + c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = e0 + u * kThreads, r = e / cols, c = e - r * cols;
+      if (e >= total) continue;
+      if (g.muon) {
+        const float mn = fmaf(g.momentum, mo[u], v[u]);
+        m.mom[(int64_t)r * m.ld_mom + c] = mn;
+        v[u] = g.nesterov ? fmaf(g.momentum, mn, v[u]) : mn;
+      }
+      ss += (double)v[u] * (double)v[u];
+      const uint32_t bits = __float_as_uint(v[u]);
+      const int at = (tall ? c : r) * h.px + (tall ? r : c) * 2;
+      *reinterpret_cast<uint16_t*>(X + at) = (uint16_t)(bits >> 16);
+      if (NP == 2) *reinterpret_cast<uint16_t*>(X + xplane + at) = (uint16_t)bits;
+    }
+  }
+  for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
+  if (lane == 0) red[wave] = ss;
+  __syncthreads();
+  if (tid == 0) {
+    double t = 0.0;
+    for (int k = 0; k < kSmallWaves; ++k) t += red[k];
+    *scale_at = start_scale(t, g.eps, g.steps, exps);
+  }
+  __syncthreads();
+  const double scale = *scale_at;
+  for (int i = tid; i < s * (h.lp / 4); i += kThreads) {  // four neighbours of a row at a time (pads are zero and stay zero, unless NaN)
+    const int r = i / (h.lp / 4), at = r * h.px + (i - r * (h.lp / 4)) * 8;
+    uint16_t hi[4], lo[4] = {0, 0, 0, 0};
+    *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<const uint2*>(X + at);
+    if (NP == 2) *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(X + xplane + at);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float v = (float)((double)__uint_as_float(((uint32_t)hi[u] << 16) | lo[u]) * scale);
+      if constexpr (NP == 2) planes(v, hi[u], lo[u]);
+      else hi[u] = f16_bits((_Float16)v);
+    }
+    *reinterpret_cast<uint2*>(X + at) = *reinterpret_cast<const uint2*>(hi);
+    if (NP == 2) *reinterpret_cast<uint2*>(X + xplane + at) = *reinterpret_cast<const uint2*>(lo);
+  }
+  __syncthreads();
+
+  const int strips = h.lp / 16, kx = h.lp / 32;
+  // a 16 x 16 tile of a symmetric matrix: four neighbours of row r from column c, and their mirror image
+  auto put_tile = [&](int tm, int tn, const f32x4& v) {
+    const int r = 16 * tm + (lane & 15), c = 16 * tn + 4 * (lane >> 4);
+    uint16_t hi[4], lo[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (NP == 2) planes(v[u], hi[u], lo[u]);
+      else hi[u] = f16_bits((_Float16)v[u]);
+    }
+    *reinterpret_cast<uint2*>(A + r * h.pa + c * 2) = *reinterpret_cast<const uint2*>(hi);
+    if constexpr (NP == 2) *reinterpret_cast<uint2*>(A + aplane + r * h.pa + c * 2) = *reinterpret_cast<const uint2*>(lo);
+    if (tm != tn) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        *reinterpret_cast<uint16_t*>(A + (c + u) * h.pa + r * 2) = hi[u];
+        if constexpr (NP == 2) *reinterpret_cast<uint16_t*>(A + aplane + (c + u) * h.pa + r * 2) = lo[u];
+      }
+    }
+  };
+  for (int k = 0; k < g.steps; ++k) {
+    const int e = exps[k];
+    f32x4 acc[kItems];
+    // A = X X^T
+#pragma unroll
+    for (int q = 0; q < kItems; ++q) {
+      const int item = wave + q * kSmallWaves;
+      acc[q] = f32x4{0, 0, 0, 0};
+      if (item >= U * kSplit) continue;
+      int tm, tn;
+      upper_tile(item % U, T, tm, tn);
+      const int p = item / U, k0 = kx * p / kSplit, k1 = kx * (p + 1) / kSplit;
+#pragma unroll 4
+      for (int kk = k0; kk < k1; ++kk) {
+        i32x4 a[NP], b[NP];
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+          a[pl] = small_rows(X + pl * xplane, h.px, 16 * tm, kk, lane);
+          b[pl] = small_rows(X + pl * xplane, h.px, 16 * tn, kk, lane);
+        }
+        acc[q] = small_mul<NP>(b, a, acc[q]);
+      }
+    }
+    if constexpr (kSplit > 1) {  // (one item per wave then: the later parts hand theirs to the first)
+      part[wave * 64 + lane] = acc[0];
+      __syncthreads();
+      if (wave < U)
+        for (int p = 1; p < kSplit; ++p) acc[0] += part[(wave + p * U) * 64 + lane];
+    }
+#pragma unroll
+    for (int q = 0; q < kItems; ++q) {
+      const int item = wave + q * kSmallWaves;
+      if (item >= U) continue;
+      int tm, tn;
+      upper_tile(item, T, tm, tn);
+      put_tile(tm, tn, acc[q] * (1.0f / kS));
+    }
+    __syncthreads();
+    // B = a I + b A + c A A, over A
+    const float fb = ldexpf(kNsB, 2 * e), fc = ldexpf(kNsC, max(4 * e - 12, -126));
+#pragma unroll
+    for (int q = 0; q < kItems; ++q) {
+      const int item = wave + q * kSmallWaves;
+      acc[q] = f32x4{0, 0, 0, 0};
+      if (item >= U) continue;
+      int tm, tn;
+      upper_tile(item, T, tm, tn);
+#pragma unroll
+      for (int kk = 0; kk < KA; ++kk) {
+        i32x4 a[NP], b[NP];
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+          a[pl] = small_rows(A + pl * aplane, h.pa, 16 * tm, kk, lane);
+          b[pl] = small_rows(A + pl * aplane, h.pa, 16 * tn, kk, lane);
+        }
+        acc[q] = small_mul<NP>(b, a, acc[q]);
+      }
+      const int r = 16 * tm + (lane & 15), c = 16 * tn + 4 * (lane >> 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float av = (float)*reinterpret_cast<const _Float16*>(A + r * h.pa + (c + u) * 2);
+        if (NP == 2) av += (float)*reinterpret_cast<const _Float16*>(A + aplane + r * h.pa + (c + u) * 2);
+        acc[q][u] = fmaf(fc, acc[q][u], fb * av) + (r == c + u && r < s ? kNsA * kS : 0.f);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kItems; ++q) {
+      const int item = wave + q * kSmallWaves;
+      if (item >= U) continue;
+      int tm, tn;
+      upper_tile(item, T, tm, tn);
+      put_tile(tm, tn, acc[q]);
+    }
+    __syncthreads();
+    // X <- B X, a strip of 16 columns at a time
+    const bool last = k + 1 == g.steps;
+    const float f = ldexpf(1.0f, max(e - (last ? 12 : exps[k + 1]) - 12, -126));
+    for (int st = wave; st < strips; st += kSmallWaves) {
+      i32x4 x[KA][NP];
+#pragma unroll
+      for (int kk = 0; kk < KA; ++kk)
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) x[kk][pl] = small_cols(X + pl * xplane, h.px, 16 * st, kk, lane);
+      f32x4 y[T];
+#pragma unroll
+      for (int tm = 0; tm < T; ++tm) {
+        y[tm] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KA; ++kk) {
+          i32x4 b[NP];
+#pragma unroll
+          for (int pl = 0; pl < NP; ++pl) b[pl] = small_rows(A + pl * aplane, h.pa, 16 * tm, kk, lane);
+          y[tm] = small_mul<NP>(x[kk], b, y[tm]);
+        }
+      }
+#pragma unroll
+      for (int tm = 0; tm < T; ++tm) {
+        const int r = 16 * tm + (lane & 15), c = 16 * st + 4 * (lane >> 4);
+        if (!last) {
+          uint16_t hi[4], lo[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if constexpr (NP == 2) planes(y[tm][u] * f, hi[u], lo[u]);
+            else hi[u] = f16_bits((_Float16)(y[tm][u] * f));
+          }
+          *reinterpret_cast<uint2*>(X + r * h.px + c * 2) = *reinterpret_cast<const uint2*>(hi);
+          if constexpr (NP == 2) *reinterpret_cast<uint2*>(X + xplane + r * h.px + c * 2) = *reinterpret_cast<const uint2*>(lo);
+        } else if (r < s) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int lr = tall ? c + u : r, lc = tall ? r : c + u;
+            if (lr < rows && lc < cols) write_result(g, m, lr, lc, y[tm][u] * f);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int NP>
+__global__ __launch_bounds__(64 * kSmallWaves) void k_ortho_small(Group g) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const Mat& m = g.m[blockIdx.x];
+  switch ((min(m.rows, m.cols) + 31) / 32) {
+    case 1: small_matrix<NP, 1>(g, m, lds); break;
+    case 2: small_matrix<NP, 2>(g, m, lds); break;
+    case 3: small_matrix<NP, 3>(g, m, lds); break;
+    default: small_matrix<NP, 4>(g, m, lds); break;
   }
 }
 
@@ -307,13 +598,19 @@ size_t mat_bytes(int rows, int cols, int np) {
 }
 size_t head_bytes() { return up256(sizeof(double) * kMaxMats * kNormBlocks) + up256(sizeof(int32_t) * kMaxMats * (kMaxSteps + 1)); }
 
-// Matrices of a call go through the launches in groups of kMaxMats; the groups use the same workspace one after the other
+bool is_small(int rows, int cols, int np) { return small_shape(rows, cols, np).bytes <= kSmallLds; }
+
+// The matrices that do not fit one block go through the launches in groups of kMaxMats, one group after the other in the same
+// workspace
 template <class F>
 size_t workspace_bytes(int n, int np, F shape) {
-  size_t most = 0;
-  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
-    size_t b = 0;
-    for (int i = g0; i < std::min(n, g0 + kMaxMats); ++i) b += mat_bytes(shape(i).first, shape(i).second, np);
+  size_t most = 0, b = 0;
+  int in_group = 0;
+  for (int i = 0; i < n; ++i) {
+    if (is_small(shape(i).first, shape(i).second, np)) continue;
+    if (in_group == kMaxMats) { b = 0; in_group = 0; }
+    b += mat_bytes(shape(i).first, shape(i).second, np);
+    ++in_group;
     most = std::max(most, b);
   }
   return head_bytes() + most;
@@ -404,6 +701,37 @@ int run_group(Group& g, char* ws, hipStream_t s) {
   return 0;
 }
 
+// `fill(i, mat)` describes matrix i; `base` holds what the matrices of the call share
+template <int NP, class F>
+int run_list(int n, const Group& base, F fill, char* ws, hipStream_t s) {
+  Group small = base, large = base;
+  small.n = large.n = 0;
+  auto flush = [&](Group& g, bool is_small_group) {
+    if (g.n == 0) return 0;
+    int rc;
+    if (is_small_group) {
+      int lds = 0;
+      for (int i = 0; i < g.n; ++i) lds = std::max(lds, small_shape(g.m[i].rows, g.m[i].cols, NP).bytes);
+      rc = launch<k_ortho_small<NP>>(g, g.n, 64 * kSmallWaves, lds, s);
+    } else {
+      rc = run_group<NP>(g, ws, s);
+    }
+    g.n = 0;
+    return rc;
+  };
+  for (int i = 0; i < n; ++i) {
+    Mat m{};
+    fill(i, m);
+    const bool sm = is_small(m.rows, m.cols, NP);
+    Group& g = sm ? small : large;
+    g.m[g.n++] = m;
+    if (g.n == kMaxMats)
+      if (int rc = flush(g, sm)) return rc;
+  }
+  if (int rc = flush(small, true)) return rc;
+  return flush(large, false);
+}
+
 int check_dims(int32_t rows, int32_t cols) {
   SUAVE_REQUIRE(rows >= 1 && cols >= 1, "orthogonalize: a matrix needs at least one row and one column");
   SUAVE_REQUIRE(std::min(rows, cols) <= 32768 && std::max(rows, cols) <= (1 << 20), "orthogonalize: the sides of a matrix must be at most 32768 (short) and 2^20 (long)");
@@ -437,18 +765,12 @@ int launch_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dt
     SUAVE_REQUIRE(mats[i].in && mats[i].out, "orthogonalize: a matrix is null");
     SUAVE_REQUIRE(mats[i].ld_in >= mats[i].cols && mats[i].ld_out >= mats[i].cols, "orthogonalize: a row stride is shorter than the row");
   }
-  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
-    Group g{};
-    g.n = std::min(kMaxMats, n - g0);
-    for (int i = 0; i < g.n; ++i) {
-      const suave_ortho_matrix_t& h = mats[g0 + i];
-      Mat& m = g.m[i];
-      m.in = h.in; m.out = h.out; m.ld_in = h.ld_in; m.ld_out = h.ld_out; m.rows = h.rows; m.cols = h.cols;
-    }
-    g.eps = eps; g.steps = steps; g.bf16 = dtype == SUAVE_DTYPE_BF16;
-    if (int rc = g.bf16 ? run_group<1>(g, static_cast<char*>(ws), s) : run_group<2>(g, static_cast<char*>(ws), s)) return rc;
-  }
-  return 0;
+  Group base{};
+  base.eps = eps; base.steps = steps; base.bf16 = dtype == SUAVE_DTYPE_BF16;
+  auto fill = [&](int i, Mat& m) {
+    m.in = mats[i].in; m.out = mats[i].out; m.ld_in = mats[i].ld_in; m.ld_out = mats[i].ld_out; m.rows = mats[i].rows; m.cols = mats[i].cols;
+  };
+  return base.bf16 ? run_list<1>(n, base, fill, static_cast<char*>(ws), s) : run_list<2>(n, base, fill, static_cast<char*>(ws), s);
 }
 
 int muon_workspace(const suave_muon_matrix_t* mats, int32_t n, size_t* bytes) {
@@ -472,21 +794,16 @@ int launch_muon(const suave_muon_matrix_t* mats, int32_t n, float momentum, int 
     SUAVE_REQUIRE(h.ld_param >= h.cols && h.ld_grad >= h.cols && h.ld_momentum >= h.cols, "muon_step: a row stride is shorter than the row");
     SUAVE_REQUIRE(std::isfinite(h.lr) && h.lr >= 0.f, "muon_step: lr must not be negative");
   }
-  for (int g0 = 0; g0 < n; g0 += kMaxMats) {
-    Group g{};
-    g.n = std::min(kMaxMats, n - g0);
-    for (int i = 0; i < g.n; ++i) {
-      const suave_muon_matrix_t& h = mats[g0 + i];
-      Mat& m = g.m[i];
-      m.in = h.grad; m.out = h.param; m.mom = h.momentum; m.ld_in = h.ld_grad; m.ld_out = h.ld_param; m.ld_mom = h.ld_momentum;
-      m.rows = h.rows; m.cols = h.cols;
-      m.lr = (float)((double)h.lr * std::sqrt(std::max(1.0, (double)h.rows / h.cols)));
-      m.decay = (float)(1.0 - (double)h.lr * weight_decay);
-    }
-    g.eps = eps; g.steps = steps; g.muon = 1; g.momentum = momentum; g.nesterov = nesterov;
-    if (int rc = run_group<2>(g, static_cast<char*>(ws), s)) return rc;
-  }
-  return 0;
+  Group base{};
+  base.eps = eps; base.steps = steps; base.muon = 1; base.momentum = momentum; base.nesterov = nesterov;
+  auto fill = [&](int i, Mat& m) {
+    const suave_muon_matrix_t& h = mats[i];
+    m.in = h.grad; m.out = h.param; m.mom = h.momentum; m.ld_in = h.ld_grad; m.ld_out = h.ld_param; m.ld_mom = h.ld_momentum;
+    m.rows = h.rows; m.cols = h.cols;
+    m.lr = (float)((double)h.lr * std::sqrt(std::max(1.0, (double)h.rows / h.cols)));
+    m.decay = (float)(1.0 - (double)h.lr * weight_decay);
+  };
+  return run_list<2>(n, base, fill, static_cast<char*>(ws), s);
 }
 
 }  // namespace suave
