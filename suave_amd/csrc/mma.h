@@ -271,6 +271,67 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  // For products of few tiles, whose time is the chain of K steps: the block has `groups` times the waves of a tile, group g takes the
+  // steps [g per, (g + 1) per) of K in LDS of its own (kLds bytes each, at lds), and the partial sums meet in LDS.  Every group walks
+  // `per` steps, those past K as zeros, so all waves pass the same barriers.  On return acc holds the whole sums of this
+  // group's share of the fragments: those with (MI j + i) % groups == g.
+  template <int GROUPS>
+  static __device__ __forceinline__ void run_split(char* lds, Operand A, Operand B, int K, acc_t (&acc)[MI][NI]) {
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all / (WM * WN), wave = all % (WM * WN);
+    const int wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+    const int steps = (K + kStepK - 1) / kStepK, per = (steps + GROUPS - 1) / GROUPS, first = group * per;
+    char* mine = lds + group * kLds;
+    const char* pa = uniform_ptr(A.base + SA::advance(A) * first);
+    const char* pb = uniform_ptr(B.base + SB::advance(B) * first);
+    uint32_t oa[SA::kPer], ob[SB::kPer];
+    auto load = [&](int s) {
+      offsets(A, B, wave, lane, K - (first + s) * kStepK, oa, ob);
+      planes_load(pa + SA::advance(A) * s, pb + SB::advance(B) * s, mine + (s & 1) * kStepBytes, wave, oa, ob);
+    };
+    load(0);
+    for (int s = 0; s < per; ++s) {
+      turn();
+      if constexpr (NP == 2) {
+        planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, acc);
+        if (s + 1 < per) load(s + 1);
+      } else {
+        Frags f[2];
+        read_all(mine + (s & 1) * kStepBytes, wm, wn, 0, lane, f[0]);
+        read_all(mine + (s & 1) * kStepBytes, wm, wn, 1, lane, f[1]);
+        if (s + 1 < per) load(s + 1);  // (behind the reads: the compiler lets a transposed read wait for earlier transfers)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(f[kk].b[j], f[kk].a[i], acc[i][j]);
+      }
+    }
+    turn();
+    acc_t* sums = reinterpret_cast<acc_t*>(lds);  // [group][wave][fragment][lane]
+    static_assert(WM * WN * MI * NI * 64 * 16 <= kLds, "the partial sums fit the groups' slots");
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sums[((group * WM * WN + wave) * MI * NI + MI * j + i) * 64 + lane] = acc[i][j];
+    turn();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if ((MI * j + i) % GROUPS != group) continue;
+        acc_t t = acc_t{0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) t += sums[((g * WM * WN + wave) * MI * NI + MI * j + i) * 64 + lane];
+        acc[i][j] = t;
+      }
+  }
+
   // K elements from the operands' bases.  Every thread of the block takes part; lds: kLds bytes, 16-byte aligned.
   static __device__ __forceinline__ void run(char* lds, Operand A, Operand B, int K, acc_t (&acc)[MI][NI]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -357,9 +418,12 @@ struct Tile {
 
 // Block -> tile: the blocks an XCD gets (every eighth) walk one contiguous range of tiles, `group` row tiles side by side
 // within it, so that the operand panels a die's L2 holds are shared by its blocks in flight.
-__device__ __forceinline__ void tile_of(int b, int n_blocks, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
+__device__ __forceinline__ int die_order(int b, int n_blocks) {
   const int q = n_blocks / 8, r = n_blocks % 8, x = b % 8, i = b / 8;
-  const int t = x * q + min(x, r) + i;
+  return x * q + min(x, r) + i;
+}
+__device__ __forceinline__ void tile_of(int b, int n_blocks, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
+  const int t = die_order(b, n_blocks);
   const int per = group * tiles_n, g = t / per, rem = t - g * per;
   const int gm = min(group, tiles_m - g * group);
   tm = g * group + rem % gm;

@@ -19,6 +19,7 @@
 
 #include "kernels.h"
 #include "mma.h"
+#include "tiles.h"
 
 namespace suave {
 
@@ -190,6 +191,12 @@ __device__ __forceinline__ void store_mirror(char* base, int pit, int cols, int 
   }
 }
 
+template <class T, int GROUPS>
+__device__ __forceinline__ void run_tile(char* lds, const Operand& A, const Operand& B, int K, typename T::acc_t (&acc)[T::MI][T::NI]) {
+  if constexpr (GROUPS > 1) T::template run_split<GROUPS>(lds, A, B, K, acc);
+  else T::run(lds, A, B, K, acc);
+}
+
 // tile t of the T (T + 1) / 2 on and above the diagonal
 __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
   tm = 0;
@@ -197,9 +204,12 @@ __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
   tn = tm + t;
 }
 
+// K splits inside a block: for lists with few tiles (Tile::run_split)
+constexpr int kGroups = 4;
+
 // POLY 0: A from X; 1: B from A
-template <int NP, int BM, int WM, int WN, int POLY>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
+template <int NP, int BM, int WM, int WN, int POLY, int GROUPS>
+__global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_sym(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> R;
   typedef Tile<kF16, NP, true, true, BM, BM, WM, WN> C;
@@ -208,22 +218,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
   const int s = min(m.rows, m.cols), T = (s + BM - 1) / BM;
   const int ps = pitch(s, NP);
   int tm, tn;
-  upper_tile(blockIdx.x - g.begin[i], T, tm, tn);
+  upper_tile(die_order(blockIdx.x - g.begin[i], T * (T + 1) / 2), T, tm, tn);
   const int m0 = tm * BM, n0 = tn * BM;
   f32x4 acc[R::MI][R::NI];
   if (POLY) {
     const uint32_t plane = (s + 7) / 8 * 16;
-    R::run(lds, Operand{m.a + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane}, Operand{m.a + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane}, s, acc);
+    run_tile<R, GROUPS>(lds, Operand{m.a + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane}, Operand{m.a + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane}, s, acc);
   } else {
     const int px = pitch(m.cols, NP);
     const uint32_t plane = (m.cols + 7) / 8 * 16;
     const char* x = m.x[g.k & 1];
     if (m.rows <= m.cols)
-      R::run(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, s - m0, plane}, Operand{x + (int64_t)n0 * px, (uint32_t)px, s - n0, plane}, m.cols, acc);
+      run_tile<R, GROUPS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, s - m0, plane}, Operand{x + (int64_t)n0 * px, (uint32_t)px, s - n0, plane}, m.cols, acc);
     else
-      C::run(lds, Operand{x + m0 * 2, (uint32_t)px, (s - m0 + 7) / 8 * 16, plane}, Operand{x + n0 * 2, (uint32_t)px, (s - n0 + 7) / 8 * 16, plane}, m.rows, acc);
+      run_tile<C, GROUPS>(lds, Operand{x + m0 * 2, (uint32_t)px, (s - m0 + 7) / 8 * 16, plane}, Operand{x + n0 * 2, (uint32_t)px, (s - n0 + 7) / 8 * 16, plane}, m.rows, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
   const int e = g.exps[i * (kMaxSteps + 1) + g.k];
   const float fb = ldexpf(kNsB, 2 * e), fc = ldexpf(kNsC, max(4 * e - 12, -126));
@@ -234,6 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
     if (r >= s) continue;
 #pragma unroll
     for (int j = 0; j < R::NI; ++j) {
+      if (GROUPS > 1 && (R::MI * j + mi) % GROUPS != group) continue;
       const int n = n0 + wn * (R::NI * 16) + 16 * j + 4 * (lane >> 4);
       if (n >= sp) continue;
       float v[4];
@@ -261,27 +272,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_sym(Group g) {
 }
 
 // X <- B X (wide) or X B (tall); the last step writes the result or takes the step on the parameter
-template <int NP, int BM, int WM, int WN, bool LAST>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_update(Group g) {
+template <int NP, int BM, int BN, int WM, int WN, bool LAST, int GROUPS>
+__global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_update(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  typedef Tile<kF16, NP, false, true, BM, BM, WM, WN> W;
-  typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> H;
+  typedef Tile<kF16, NP, false, true, BM, BN, WM, WN> W;
+  typedef Tile<kF16, NP, false, false, BM, BN, WM, WN> H;
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int s = min(m.rows, m.cols);
   const int ps = pitch(s, NP), px = pitch(m.cols, NP);
   const uint32_t plane_s = (s + 7) / 8 * 16, plane_x = (m.cols + 7) / 8 * 16;
-  const int tiles_m = (m.rows + BM - 1) / BM, tiles_n = (m.cols + BM - 1) / BM;
+  const int tiles_m = (m.rows + BM - 1) / BM, tiles_n = (m.cols + BN - 1) / BN;
   int tm, tn;
   tile_of(blockIdx.x - g.begin[i], tiles_m * tiles_n, tiles_m, tiles_n, 8, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BM;
+  const int m0 = tm * BM, n0 = tn * BN;
   const char* x = m.x[g.k & 1];
   f32x4 acc[W::MI][W::NI];
   if (m.rows <= m.cols)
-    W::run(lds, Operand{m.b + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane_s}, Operand{x + (int64_t)n0 * 2, (uint32_t)px, (m.cols - n0 + 7) / 8 * 16, plane_x}, s, acc);
+    run_tile<W, GROUPS>(lds, Operand{m.b + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane_s}, Operand{x + (int64_t)n0 * 2, (uint32_t)px, (m.cols - n0 + 7) / 8 * 16, plane_x}, s, acc);
   else
-    H::run(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    run_tile<H, GROUPS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
   const int e = g.exps[i * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[i * (kMaxSteps + 1) + g.k + 1];
   const float f = ldexpf(1.0f, max(e - e1 - 12, -126));
@@ -292,6 +303,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_ortho_update(Group g) {
     if (r >= m.rows) continue;
 #pragma unroll
     for (int j = 0; j < W::NI; ++j) {
+      if (GROUPS > 1 && (W::MI * j + mi) % GROUPS != group) continue;
       const int n = n0 + wn * (W::NI * 16) + 16 * j + 4 * (lane >> 4);
       if (n >= (LAST ? m.cols : cp)) continue;
       float v[4];
@@ -590,7 +602,6 @@ __global__ __launch_bounds__(64 * kSmallWaves) void k_ortho_small(Group g) {
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 size_t mat_bytes(int rows, int cols, int np) {
   const int s = std::min(rows, cols);
@@ -616,6 +627,7 @@ size_t workspace_bytes(int n, int np, F shape) {
   return head_bytes() + most;
 }
 
+// tiles on and above the diagonals, and all tiles, of a group's matrices
 int64_t sym_tiles(const Group& g, int bm) {
   int64_t t = 0;
   for (int i = 0; i < g.n; ++i) {
@@ -624,17 +636,39 @@ int64_t sym_tiles(const Group& g, int bm) {
   }
   return t;
 }
-int64_t all_tiles(const Group& g, int bm) {
+int64_t all_tiles(const Group& g, int bm, int bn) {
   int64_t t = 0;
-  for (int i = 0; i < g.n; ++i) t += ceil_div(g.m[i].rows, bm) * ceil_div(g.m[i].cols, bm);
+  for (int i = 0; i < g.n; ++i) t += ceil_div(g.m[i].rows, bm) * ceil_div(g.m[i].cols, bn);
   return t;
 }
-// the largest tile that still gives most CUs work
+// The tile with the smallest estimated time; `id` kSplit64: 64 x 64 with K cut into kGroups inside the block, whose step costs a
+// CU as much as kGroups steps of a 64 x 64 block and takes as long as one (plus about a step to join the sums)
+constexpr int kSplit64 = kTileIds;
 template <class F>
-int pick_tile(const Group& g, F tiles) {
-  if (tiles(g, 256) >= 200) return 256;
-  if (tiles(g, 128) >= 200) return 128;
-  return 64;
+int pick_tile(F tiles, int64_t steps, int planes, bool wide_too) {
+  int best = kT64;
+  double us = 1e30;
+  for (int t = 0; t <= kTileIds; ++t) {
+    if (t == kT64x128 && !wide_too) continue;
+    double e;
+    if (t == kSplit64) {
+      const double blocks = (double)tiles(64, 64);
+      const double per = (double)ceil_div(steps, kGroups);
+      e = std::ceil(blocks / kCUs) * (per * std::max(kAlone[planes - 1][kT64], kGroups * kShare[planes - 1][kT64]) + kAlone[planes - 1][kT64]);
+    } else {
+      const Work w{tiles(kTileM[t], kTileN[t]), steps, 0.0};
+      const int one = 1;
+      e = estimate_us((TileId)t, planes, &w, &one, 1);
+    }
+    if (e < us * 0.98) { us = e; best = t; }
+  }
+  return best;
+}
+// K steps of the longest chain of a group: over the long sides (gram) or the short ones
+int64_t most_steps(const Group& g, bool gram, int planes) {
+  int64_t k = 1;
+  for (int i = 0; i < g.n; ++i) k = std::max<int64_t>(k, gram ? std::max(g.m[i].rows, g.m[i].cols) : std::min(g.m[i].rows, g.m[i].cols));
+  return ceil_div(k, planes == 2 ? 32 : 64);
 }
 
 template <auto kernel>
@@ -657,21 +691,35 @@ int set_begin(Group& g, F blocks) {
   return (int)b;
 }
 
+template <int NP, int POLY, int BM, int WM, int WN, int GROUPS>
+int launch_sym_tile(Group& g, hipStream_t s) {
+  const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), BM); return T * (T + 1) / 2; });
+  return launch<k_ortho_sym<NP, BM, WM, WN, POLY, GROUPS>>(g, grid, 64 * WM * WN * GROUPS, GROUPS * Tile<kF16, NP, false, false, BM, BM, WM, WN>::kLds, s);
+}
 template <int NP, int POLY>
 int launch_sym(Group& g, hipStream_t s) {
-  const int bm = pick_tile(g, sym_tiles);
-  const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), bm); return T * (T + 1) / 2; });
-  if (bm == 256) return launch<k_ortho_sym<NP, 256, 2, 4, POLY>>(g, grid, 512, Tile<kF16, NP, false, false, 256, 256, 2, 4>::kLds, s);
-  if (bm == 128) return launch<k_ortho_sym<NP, 128, 2, 2, POLY>>(g, grid, 256, Tile<kF16, NP, false, false, 128, 128, 2, 2>::kLds, s);
-  return launch<k_ortho_sym<NP, 64, 2, 2, POLY>>(g, grid, 256, Tile<kF16, NP, false, false, 64, 64, 2, 2>::kLds, s);
+  switch (pick_tile([&](int bm, int) { return sym_tiles(g, bm); }, most_steps(g, POLY == 0, NP), NP, false)) {
+    case kSplit64: return launch_sym_tile<NP, POLY, 64, 2, 2, kGroups>(g, s);
+    case kT64: return launch_sym_tile<NP, POLY, 64, 2, 2, 1>(g, s);
+    case kT128: return launch_sym_tile<NP, POLY, 128, 2, 2, 1>(g, s);
+    default: return launch_sym_tile<NP, POLY, 256, 2, 4, 1>(g, s);
+  }
+}
+template <int NP, bool LAST, int BM, int BN, int WM, int WN, int GROUPS>
+int launch_update_tile(Group& g, hipStream_t s) {
+  const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, BM) * ceil_div(m.cols, BN); });
+  return launch<k_ortho_update<NP, BM, BN, WM, WN, LAST, GROUPS>>(g, grid, 64 * WM * WN * GROUPS,
+                                                                  GROUPS * Tile<kF16, NP, false, true, BM, BN, WM, WN>::kLds, s);
 }
 template <int NP, bool LAST>
 int launch_update(Group& g, hipStream_t s) {
-  const int bm = pick_tile(g, all_tiles);
-  const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, bm) * ceil_div(m.cols, bm); });
-  if (bm == 256) return launch<k_ortho_update<NP, 256, 2, 4, LAST>>(g, grid, 512, Tile<kF16, NP, false, true, 256, 256, 2, 4>::kLds, s);
-  if (bm == 128) return launch<k_ortho_update<NP, 128, 2, 2, LAST>>(g, grid, 256, Tile<kF16, NP, false, true, 128, 128, 2, 2>::kLds, s);
-  return launch<k_ortho_update<NP, 64, 2, 2, LAST>>(g, grid, 256, Tile<kF16, NP, false, true, 64, 64, 2, 2>::kLds, s);
+  switch (pick_tile([&](int bm, int bn) { return all_tiles(g, bm, bn); }, most_steps(g, false, NP), NP, true)) {
+    case kSplit64: return launch_update_tile<NP, LAST, 64, 64, 2, 2, kGroups>(g, s);
+    case kT64: return launch_update_tile<NP, LAST, 64, 64, 2, 2, 1>(g, s);
+    case kT64x128: return launch_update_tile<NP, LAST, 64, 128, 2, 2, 1>(g, s);
+    case kT128: return launch_update_tile<NP, LAST, 128, 128, 2, 2, 1>(g, s);
+    default: return launch_update_tile<NP, LAST, 256, 256, 2, 4, 1>(g, s);
+  }
 }
 
 template <int NP>
