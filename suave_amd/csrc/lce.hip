@@ -711,6 +711,7 @@ template <int TYPE, int NP>
 int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, hipStream_t s) {
   switch (tile) {
     case kT64: return launch_grads_tile<TYPE, NP, 64, 64, 2, 2>(dx, dw, s);
+    case kT96: return launch_grads_tile<TYPE, NP, 96, 96, 2, 2>(dx, dw, s);
     case kT64x128: return launch_grads_tile<TYPE, NP, 64, 128, 2, 2>(dx, dw, s);
     case kT128: return launch_grads_tile<TYPE, NP, 128, 128, 2, 2>(dx, dw, s);
     default: return launch_grads_tile<TYPE, NP, 256, 256, 2, 4>(dx, dw, s);

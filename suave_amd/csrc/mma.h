@@ -13,7 +13,7 @@
 // A K step is 128 bytes per row whatever the type: 64 bf16 / fp16, 32 values in two planes, 128 int8.  Tiles go from
 // global memory to LDS directly (buffer_load ... lds, 16 bytes per lane), into two slots.  The DMA writes lane i
 // at base + 16 i, so the bank swizzle is a permutation of the SOURCE chunks: row form slot s of row r holds chunk
-// s ^ (r & 7); column form slot s of k-row r holds chunk s ^ (2 (r & 3) [^ 8 ((r >> 3) & 1)]).  Chunks past the edge of an
+// s ^ (r & 7), column form by col_chunk.  Chunks past the edge of an
 // operand along K read as zero (an offset beyond the buffer resource's range), rows past the edge are clamped to the
 // last one (their products are never written).
 //
@@ -51,6 +51,20 @@ struct Operand {
   int rows;
   uint32_t plane;
 };
+
+// Column form, k-row r: the chunk in a slot, and the slot of a chunk.  Rows of 64 and of n 128 columns start on the same bank: the
+// four rows of a transposed read are set apart by exchanging pairs of chunks.  Rows of 96 columns (192 bytes) alternate
+// between two halves of the banks by themselves; every second pair of rows is turned by one pair of chunks.
+template <int EXT>
+__device__ __forceinline__ uint32_t col_chunk(uint32_t slot, int r) {
+  if constexpr (EXT == 96) return r & 2 ? (slot < 2 ? slot + 10 : slot - 2) : slot;
+  else return slot ^ (2 * (r & 3)) ^ (EXT >= 128 ? 8 * ((r >> 3) & 1) : 0);
+}
+template <int EXT>
+__device__ __forceinline__ uint32_t col_slot(uint32_t chunk, int r) {
+  if constexpr (EXT == 96) return r & 2 ? (chunk < 10 ? chunk + 2 : chunk - 10) : chunk;
+  else return chunk ^ (2 * (r & 3)) ^ (EXT >= 128 ? 8 * ((r >> 3) & 1) : 0);
+}
 
 constexpr uint32_t kOutside = 0x80000000u;  // any offset >= the resource's range reads zero
 
@@ -93,9 +107,7 @@ struct Stage {
   static constexpr int kPer = (kInstr + NW - 1) / NW;   // per wave
   static constexpr int kES = TYPE == kI8 ? 1 : 2;
   static constexpr int kStepK = 128 / NP / kES;         // K elements of a step
-  static_assert(!COL || (kES == 2 && EXT >= 64), "column form: 16-bit elements, 64 columns at least");
-
-  static __device__ __forceinline__ uint32_t col_swizzle(int r) { return (2 * (r & 3)) ^ (EXT >= 128 ? 8 * ((r >> 3) & 1) : 0); }
+  static_assert(!COL || (kES == 2 && (EXT == 64 || EXT == 96 || EXT % 128 == 0)), "column form: 16-bit elements, 64, 96 or n 128 columns");
 
   // source offset of lane's chunk of instruction i (of this wave) for a full step, and whether K-masked: kleft elements remain
   static __device__ __forceinline__ uint32_t offset(const Operand& o, int i, int wave, int lane, int kleft) {
@@ -110,7 +122,7 @@ struct Stage {
     } else {
       const int f = instr * 64 + lane;
       const int r = f / (EXT / 8);  // k-row, planes one behind the other
-      const uint32_t c = (uint32_t)(f % (EXT / 8)) ^ col_swizzle(r);
+      const uint32_t c = col_chunk<EXT>(f % (EXT / 8), r);
       const int pl = NP == 2 ? r / kStepK : 0;
       const int k = NP == 2 ? r - pl * kStepK : r;
       if (k >= kleft) return kOutside;
@@ -139,8 +151,7 @@ __device__ __forceinline__ i32x4 fragment(const char* lds, int row0, int kk, int
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = k0 + 4 * h;
-      const uint32_t sw = (2 * (r & 3)) ^ (EXT >= 128 ? 8 * ((r >> 3) & 1) : 0);
-      const char* p = lds + r * (EXT * 2) + ((c ^ sw) << 4) + 8 * (i & 1);
+      const char* p = lds + r * (EXT * 2) + (col_slot<EXT>(c, r) << 4) + 8 * (i & 1);
       v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_char*)const_cast<char*>(p));
     }
     s16x8 w = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -264,6 +275,28 @@ struct Tile {
       spread<I + 1, M, D, V>();
     }
   }
+  static __device__ __forceinline__ void planes_order() {
+    constexpr int da_reads = 2 * MI * (ACOL ? 2 : 1), db_reads = 2 * NI * (BCOL ? 2 : 1), first = db_reads + da_reads / MI * (MI > 1 ? 2 : 1);
+    __builtin_amdgcn_sched_group_barrier(0x100, first, 0);
+    spread<0, 3 * MI * NI, da_reads + db_reads - first, kEven ? kPerStep : 0>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // one plane, a whole step: its fragments, then `transfers` (behind the reads: the compiler lets a transposed read wait for
+  // earlier transfers), then its products
+  template <class F>
+  static __device__ __forceinline__ void both_halves(const char* lds, int wm, int wn, int lane, acc_t (&acc)[MI][NI], F transfers) {
+    Frags f[2];
+    read_all(lds, wm, wn, 0, lane, f[0]);
+    read_all(lds, wm, wn, 1, lane, f[1]);
+    transfers();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(f[kk].b[j], f[kk].a[i], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   static __device__ __forceinline__ void turn() {  // this wave's DMA has landed and its LDS reads are done; then everybody's
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -290,27 +323,39 @@ struct Tile {
     const char* pb = uniform_ptr(B.base + SB::advance(B) * first);
     uint32_t oa[SA::kPer], ob[SB::kPer];
     auto load = [&](int s) {
-      offsets(A, B, wave, lane, K - (first + s) * kStepK, oa, ob);
       planes_load(pa + SA::advance(A) * s, pb + SB::advance(B) * s, mine + (s & 1) * kStepBytes, wave, oa, ob);
     };
+    offsets(A, B, wave, lane, K - first * kStepK, oa, ob);
     load(0);
-    for (int s = 0; s < per; ++s) {
+    // steps that lie inside K for every group come first: their transfers need no masks and are spread between the products
+    const int whole = min(per, max(0, K / kStepK - (GROUPS - 1) * per));
+    int s = 0;
+    if (whole > 1) offsets(A, B, wave, lane, kStepK, oa, ob);
+    for (; s + 1 < whole; ++s) {
       turn();
       if constexpr (NP == 2) {
         planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, acc);
-        if (s + 1 < per) load(s + 1);
+        load(s + 1);
+        planes_order();
       } else {
-        Frags f[2];
-        read_all(mine + (s & 1) * kStepBytes, wm, wn, 0, lane, f[0]);
-        read_all(mine + (s & 1) * kStepBytes, wm, wn, 1, lane, f[1]);
-        if (s + 1 < per) load(s + 1);  // (behind the reads: the compiler lets a transposed read wait for earlier transfers)
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(f[kk].b[j], f[kk].a[i], acc[i][j]);
+        both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, acc, [&] { load(s + 1); });
       }
+    }
+    for (; s < per; ++s) {
+      turn();
+      auto next = [&] {
+        if (s + 1 < per) {
+          offsets(A, B, wave, lane, K - (first + s + 1) * kStepK, oa, ob);
+          load(s + 1);
+        }
+      };
+      if constexpr (NP == 2) {
+        planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, acc);
+        next();
+      } else {
+        both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, acc, next);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     turn();
     acc_t* sums = reinterpret_cast<acc_t*>(lds);  // [group][wave][fragment][lane]
@@ -389,15 +434,12 @@ struct Tile {
         for (int j = 0; j < NI; ++j) acc[i][j] = mul<TYPE>(f1.b[j], f1.a[i], acc[i][j]);
     } else {
       planes_load(pa, pb, lds, wave, oa, ob);
-      constexpr int da_reads = 2 * MI * (ACOL ? 2 : 1), db_reads = 2 * NI * (BCOL ? 2 : 1), first = db_reads + da_reads / MI * (MI > 1 ? 2 : 1);
       for (; s < steps - 2; ++s) {
         turn();
         pa += da; pb += db;
         planes_step(lds + (s & 1) * kStepBytes, wm, wn, lane, acc);
         planes_load(pa, pb, lds + (~s & 1) * kStepBytes, wave, oa, ob);
-        __builtin_amdgcn_sched_group_barrier(0x100, first, 0);
-        spread<0, 3 * MI * NI, da_reads + db_reads - first, kEven ? kPerStep : 0>();
-        __builtin_amdgcn_sched_barrier(0);
+        planes_order();
       }
       for (; s < steps; ++s) {  // the last step may be short: its chunks past K are masked
         turn();

@@ -30,7 +30,7 @@ using namespace mma;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr int kMaxMats = 24;      // matrices of one group of launches
 constexpr int kMaxSteps = 16;
-constexpr int kNormBlocks = 128;  // partial sums per matrix at most
+constexpr int kNormBlocks = 512;  // partial sums per matrix
 constexpr float kS = 4096.0f;
 
 struct Mat {
@@ -42,6 +42,7 @@ struct Mat {
   char* a;              // [short][pitch_s]
   char* b;
   int rows, cols;
+  int id;               // index of its partial sums and sizes
   float lr;             // muon: learning rate times shape factor
   float decay;          // muon: 1 - learning rate * weight decay
 };
@@ -72,28 +73,58 @@ __device__ __forceinline__ float in_value(const Group& g, const Mat& m, int64_t 
   return g.nesterov ? fmaf(g.momentum, mom, v) : mom;
 }
 
-// partial sums of squares (double: neither overflow nor loss over 2^24 values); muon: the momentum first
+// blocks of k_ortho_norm for a matrix: 2048 elements each, eight per thread
+__host__ __device__ inline int norm_blocks(int rows, int cols) {
+  const int64_t b = ((int64_t)rows * cols + 2047) / 2048;
+  return b < kNormBlocks ? (int)b : kNormBlocks;
+}
+
+// Partial sums of squares (double: neither overflow nor loss over 2^24 values); muon: the momentum first.  A block owns whole
+// rows where they are long, otherwise runs of the flat index (below 2^31 then); eight loads in flight per thread.
 __global__ __launch_bounds__(256) void k_ortho_norm(Group g) {
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
   double s = 0.0;
-  const int64_t total = (int64_t)m.rows * m.cols;
-  for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < total; e += (int64_t)nb * 256) {
-    const int64_t r = e / m.cols;
-    const int c = (int)(e - r * m.cols);
-    if (g.muon) {
-      float* mp = m.mom + r * m.ld_mom + c;
-      *mp = fmaf(g.momentum, *mp, static_cast<const float*>(m.in)[r * m.ld_in + c]);
+  auto eight = [&](int64_t e0, int64_t step, int64_t end, auto place) {
+    float v[8], mo[8];
+    int64_t r[8];
+    int c[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t e = e0 + u * step;
+      v[u] = mo[u] = 0.f;
+      if (e < end) {
+        place(e, r[u], c[u]);
+        v[u] = g.bf16 ? bf16_value(static_cast<const uint16_t*>(m.in)[r[u] * m.ld_in + c[u]]) : static_cast<const float*>(m.in)[r[u] * m.ld_in + c[u]];
+        if (g.muon) mo[u] = m.mom[r[u] * m.ld_mom + c[u]];
+      }
     }
-    const double v = in_value(g, m, r, c);
-    s += v * v;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (e0 + u * step >= end) continue;
+      if (g.muon) {
+        const float mn = fmaf(g.momentum, mo[u], v[u]);
+        m.mom[r[u] * m.ld_mom + c[u]] = mn;
+        v[u] = g.nesterov ? fmaf(g.momentum, mn, v[u]) : mn;
+      }
+      s += (double)v[u] * (double)v[u];
+    }
+  };
+  if (m.cols >= 2048) {
+    for (int64_t r = b; r < m.rows; r += nb)
+      for (int c0 = threadIdx.x; c0 < m.cols; c0 += 2048)
+        eight(c0, 256, m.cols, [&](int64_t e, int64_t& rr, int& cc) { rr = r; cc = (int)e; });
+  } else {
+    const int64_t total = (int64_t)m.rows * m.cols, step = (int64_t)nb * 256;
+    for (int64_t e0 = (int64_t)b * 256 + threadIdx.x; e0 < total; e0 += 8 * step)
+      eight(e0, step, total, [&](int64_t e, int64_t& rr, int& cc) { rr = (int)e / m.cols; cc = (int)e - (int)rr * m.cols; });
   }
   __shared__ double part[4];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) g.part[i * kNormBlocks + b] = (part[0] + part[1]) + (part[2] + part[3]);
+  if (threadIdx.x == 0) g.part[m.id * kNormBlocks + b] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // from the sum of squares of U: what U is multiplied by to give the stored X_0, and the sizes e of X_0 .. X_steps
@@ -129,13 +160,14 @@ __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
   __shared__ double sc;
   if (threadIdx.x < 64) {
     double s = 0.0;
-    for (int k = threadIdx.x; k < kNormBlocks; k += 64) s += g.part[i * kNormBlocks + k];
+    const int n = norm_blocks(m.rows, m.cols);
+    for (int k = threadIdx.x; k < n; k += 64) s += g.part[m.id * kNormBlocks + k];
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if (threadIdx.x == 0) {
       int e[kMaxSteps + 1];
       sc = start_scale(s, g.eps, g.steps, e);
       if (b == 0)
-        for (int k = 0; k <= g.steps; ++k) g.exps[i * (kMaxSteps + 1) + k] = e[k];
+        for (int k = 0; k <= g.steps; ++k) g.exps[m.id * (kMaxSteps + 1) + k] = e[k];
     }
   }
   __syncthreads();
@@ -143,13 +175,30 @@ __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
   const int cp = (m.cols + 7) / 8 * 8, q = cp / 8;
   const int64_t chunks = (int64_t)m.rows * q;
   const int pit = pitch(m.cols, NP);
+  // (rows that start at multiples of 16 bytes are read in such pieces)
+  const bool vec = !g.muon && (m.ld_in * (g.bf16 ? 2 : 4)) % 16 == 0 && (reinterpret_cast<uintptr_t>(m.in) & 15) == 0;
   for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
-    const int64_t r = e / q;
+    const int64_t r = chunks < (1 << 30) ? (int)e / q : e / q;
     const int c0 = (int)(e - r * q) * 8;
     uint16_t hi[8], lo[8];
+    float in[8];
+    if (vec && c0 + 8 <= m.cols) {
+      if (g.bf16) {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(m.in) + r * m.ld_in + c0);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) in[u] = bf16_value(reinterpret_cast<const uint16_t*>(&w)[u]);
+      } else {
+        const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(m.in) + r * m.ld_in + c0);
+        *reinterpret_cast<float4*>(in) = w[0];
+        *reinterpret_cast<float4*>(in + 4) = w[1];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) in[u] = c0 + u < m.cols ? in_value(g, m, r, c0 + u) : 0.f;
+    }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const float v = c0 + u < m.cols ? (float)((double)in_value(g, m, r, c0 + u) * scale) : 0.f;
+      const float v = c0 + u < m.cols ? (float)((double)in[u] * scale) : 0.f;
       if constexpr (NP == 2) planes(v, hi[u], lo[u]);
       else hi[u] = f16_bits((_Float16)v);
     }
@@ -204,9 +253,6 @@ __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
   tn = tm + t;
 }
 
-// K splits inside a block: for lists with few tiles (Tile::run_split)
-constexpr int kGroups = 4;
-
 // POLY 0: A from X; 1: B from A
 template <int NP, int BM, int WM, int WN, int POLY, int GROUPS>
 __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_sym(Group g) {
@@ -235,7 +281,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
   }
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
-  const int e = g.exps[i * (kMaxSteps + 1) + g.k];
+  const int e = g.exps[m.id * (kMaxSteps + 1) + g.k];
   const float fb = ldexpf(kNsB, 2 * e), fc = ldexpf(kNsC, max(4 * e - 12, -126));
   const int sp = (s + 7) / 8 * 8;
 #pragma unroll
@@ -294,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
     run_tile<H, GROUPS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
-  const int e = g.exps[i * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[i * (kMaxSteps + 1) + g.k + 1];
+  const int e = g.exps[m.id * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[m.id * (kMaxSteps + 1) + g.k + 1];
   const float f = ldexpf(1.0f, max(e - e1 - 12, -126));
   const int cp = (m.cols + 7) / 8 * 8;
 #pragma unroll
@@ -627,48 +673,49 @@ size_t workspace_bytes(int n, int np, F shape) {
   return head_bytes() + most;
 }
 
-// tiles on and above the diagonals, and all tiles, of a group's matrices
-int64_t sym_tiles(const Group& g, int bm) {
-  int64_t t = 0;
-  for (int i = 0; i < g.n; ++i) {
-    const int64_t T = ceil_div(std::min(g.m[i].rows, g.m[i].cols), bm);
-    t += T * (T + 1) / 2;
-  }
-  return t;
+// What a matrix asks of a launch: its products with A = X X^T, with B from A, and X <- B X
+enum Phase : int { kGram, kPoly, kUpdate };
+int64_t tiles_of(const Mat& m, Phase p, int bm, int bn) {
+  if (p == kUpdate) return ceil_div(m.rows, bm) * ceil_div(m.cols, bn);
+  const int64_t T = ceil_div(std::min(m.rows, m.cols), bm);
+  return T * (T + 1) / 2;
 }
-int64_t all_tiles(const Group& g, int bm, int bn) {
-  int64_t t = 0;
-  for (int i = 0; i < g.n; ++i) t += ceil_div(g.m[i].rows, bm) * ceil_div(g.m[i].cols, bn);
-  return t;
+int64_t steps_of(const Mat& m, Phase p, int planes) {
+  return ceil_div(p == kGram ? std::max(m.rows, m.cols) : std::min(m.rows, m.cols), planes == 2 ? 32 : 64);
 }
-// The tile with the smallest estimated time; `id` kSplit64: 64 x 64 with K cut into kGroups inside the block, whose step costs a
-// CU as much as kGroups steps of a 64 x 64 block and takes as long as one (plus about a step to join the sums)
-constexpr int kSplit64 = kTileIds;
-template <class F>
-int pick_tile(F tiles, int64_t steps, int planes, bool wide_too) {
+double launch_us(double blocks_per_cu, int64_t steps, int planes, int tile, int groups) {
+  const double alone = kAlone[planes - 1][tile], share = kShare[planes - 1][tile], per = (double)ceil_div(steps, groups);
+  const double on_cu = blocks_per_cu < 6 ? std::ceil(blocks_per_cu) : blocks_per_cu;  // whole blocks per CU while there are few
+  return std::max(per * alone, on_cu * per * groups * share) + (groups > 1 ? 2 * alone : 0.0);
+}
+// Into how many groups of waves the blocks of a matrix's product cut K (Tile::run_split: a step of the block costs a CU as much as
+// that many steps of the tile and takes as long as one; about two steps more join the sums): 4 on 64 x 64 tiles, 2 on 96 x 96, 1 on
+// any.  Decided by the matrix alone, so that its result does not depend on what else is in the list: the order of the sums does
+// not depend on the tile, only on the groups.
+int groups_of(const Mat& m, Phase p, int planes) {
+  const int64_t steps = steps_of(m, p, planes);
+  double us = 1e30;
+  for (int t = 0; t < kTileIds; ++t) us = std::min(us, launch_us((double)tiles_of(m, p, kTileM[t], kTileN[t]) / kCUs, steps, planes, t, 1));
+  const double two = launch_us((double)tiles_of(m, p, 96, 96) / kCUs, steps, planes, kT96, 2);
+  const double four = launch_us((double)tiles_of(m, p, 64, 64) / kCUs, steps, planes, kT64, 4);
+  // (a microsecond for staying with the other small matrices of a list: a launch of its own costs more)
+  return four < us + 1.0 && four <= two + 1.0 ? 4 : two < us * 0.98 ? 2 : 1;
+}
+// The tile of the ungrouped launches: the smallest estimated time for the whole list
+int pick_tile(const Group& g, Phase p, int planes) {
   int best = kT64;
   double us = 1e30;
-  for (int t = 0; t <= kTileIds; ++t) {
-    if (t == kT64x128 && !wide_too) continue;
-    double e;
-    if (t == kSplit64) {
-      const double blocks = (double)tiles(64, 64);
-      const double per = (double)ceil_div(steps, kGroups);
-      e = std::ceil(blocks / kCUs) * (per * std::max(kAlone[planes - 1][kT64], kGroups * kShare[planes - 1][kT64]) + kAlone[planes - 1][kT64]);
-    } else {
-      const Work w{tiles(kTileM[t], kTileN[t]), steps, 0.0};
-      const int one = 1;
-      e = estimate_us((TileId)t, planes, &w, &one, 1);
+  for (int t = 0; t < kTileIds; ++t) {
+    if (t == kT64x128 && p != kUpdate) continue;
+    int64_t tiles = 0, steps = 1;
+    for (int i = 0; i < g.n; ++i) {
+      tiles += tiles_of(g.m[i], p, kTileM[t], kTileN[t]);
+      steps = std::max(steps, steps_of(g.m[i], p, planes));
     }
+    const double e = launch_us((double)tiles / kCUs, steps, planes, t, 1);
     if (e < us * 0.98) { us = e; best = t; }
   }
   return best;
-}
-// K steps of the longest chain of a group: over the long sides (gram) or the short ones
-int64_t most_steps(const Group& g, bool gram, int planes) {
-  int64_t k = 1;
-  for (int i = 0; i < g.n; ++i) k = std::max<int64_t>(k, gram ? std::max(g.m[i].rows, g.m[i].cols) : std::min(g.m[i].rows, g.m[i].cols));
-  return ceil_div(k, planes == 2 ? 32 : 64);
 }
 
 template <auto kernel>
@@ -693,29 +740,33 @@ int set_begin(Group& g, F blocks) {
 
 template <int NP, int POLY, int BM, int WM, int WN, int GROUPS>
 int launch_sym_tile(Group& g, hipStream_t s) {
-  const int grid = set_begin(g, [&](const Mat& m) { const int64_t T = ceil_div(std::min(m.rows, m.cols), BM); return T * (T + 1) / 2; });
+  const int grid = set_begin(g, [](const Mat& m) { return tiles_of(m, kGram, BM, BM); });
   return launch<k_ortho_sym<NP, BM, WM, WN, POLY, GROUPS>>(g, grid, 64 * WM * WN * GROUPS, GROUPS * Tile<kF16, NP, false, false, BM, BM, WM, WN>::kLds, s);
 }
+template <int NP, bool LAST, int BM, int BN, int WM, int WN, int GROUPS>
+int launch_update_tile(Group& g, hipStream_t s) {
+  const int grid = set_begin(g, [](const Mat& m) { return tiles_of(m, kUpdate, BM, BN); });
+  return launch<k_ortho_update<NP, BM, BN, WM, WN, LAST, GROUPS>>(g, grid, 64 * WM * WN * GROUPS,
+                                                                  GROUPS * Tile<kF16, NP, false, true, BM, BN, WM, WN>::kLds, s);
+}
 template <int NP, int POLY>
-int launch_sym(Group& g, hipStream_t s) {
-  switch (pick_tile([&](int bm, int) { return sym_tiles(g, bm); }, most_steps(g, POLY == 0, NP), NP, false)) {
-    case kSplit64: return launch_sym_tile<NP, POLY, 64, 2, 2, kGroups>(g, s);
+int launch_sym(Group& g, int groups, hipStream_t s) {
+  if (groups == 4) return launch_sym_tile<NP, POLY, 64, 2, 2, 4>(g, s);
+  if (groups == 2) return launch_sym_tile<NP, POLY, 96, 2, 2, 2>(g, s);
+  switch (pick_tile(g, POLY ? kPoly : kGram, NP)) {
     case kT64: return launch_sym_tile<NP, POLY, 64, 2, 2, 1>(g, s);
+    case kT96: return launch_sym_tile<NP, POLY, 96, 2, 2, 1>(g, s);
     case kT128: return launch_sym_tile<NP, POLY, 128, 2, 2, 1>(g, s);
     default: return launch_sym_tile<NP, POLY, 256, 2, 4, 1>(g, s);
   }
 }
-template <int NP, bool LAST, int BM, int BN, int WM, int WN, int GROUPS>
-int launch_update_tile(Group& g, hipStream_t s) {
-  const int grid = set_begin(g, [&](const Mat& m) { return ceil_div(m.rows, BM) * ceil_div(m.cols, BN); });
-  return launch<k_ortho_update<NP, BM, BN, WM, WN, LAST, GROUPS>>(g, grid, 64 * WM * WN * GROUPS,
-                                                                  GROUPS * Tile<kF16, NP, false, true, BM, BN, WM, WN>::kLds, s);
-}
 template <int NP, bool LAST>
-int launch_update(Group& g, hipStream_t s) {
-  switch (pick_tile([&](int bm, int bn) { return all_tiles(g, bm, bn); }, most_steps(g, false, NP), NP, true)) {
-    case kSplit64: return launch_update_tile<NP, LAST, 64, 64, 2, 2, kGroups>(g, s);
+int launch_update(Group& g, int groups, hipStream_t s) {
+  if (groups == 4) return launch_update_tile<NP, LAST, 64, 64, 2, 2, 4>(g, s);
+  if (groups == 2) return launch_update_tile<NP, LAST, 96, 96, 2, 2, 2>(g, s);
+  switch (pick_tile(g, kUpdate, NP)) {
     case kT64: return launch_update_tile<NP, LAST, 64, 64, 2, 2, 1>(g, s);
+    case kT96: return launch_update_tile<NP, LAST, 96, 96, 2, 2, 1>(g, s);
     case kT64x128: return launch_update_tile<NP, LAST, 64, 128, 2, 2, 1>(g, s);
     case kT128: return launch_update_tile<NP, LAST, 128, 128, 2, 2, 1>(g, s);
     default: return launch_update_tile<NP, LAST, 256, 256, 2, 4, 1>(g, s);
@@ -729,23 +780,40 @@ int run_group(Group& g, char* ws, hipStream_t s) {
   char* at = ws + head_bytes();
   for (int i = 0; i < g.n; ++i) {
     Mat& m = g.m[i];
+    m.id = i;
     const int sh = std::min(m.rows, m.cols);
     for (int k = 0; k < 2; ++k) { m.x[k] = at; at += up256((size_t)m.rows * pitch(m.cols, NP)); }
     m.a = at; at += up256((size_t)sh * pitch(sh, NP));
     m.b = at; at += up256((size_t)sh * pitch(sh, NP));
   }
-  // every partial of a matrix is written: kNormBlocks blocks whatever its size
-  int grid = set_begin(g, [](const Mat&) { return (int64_t)kNormBlocks; });
+  int grid = set_begin(g, [](const Mat& m) { return norm_blocks(m.rows, m.cols); });
   hipLaunchKernelGGL(k_ortho_norm, dim3(grid), dim3(256), 0, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
   grid = set_begin(g, [](const Mat& m) { return std::min<int64_t>(1024, std::max<int64_t>(1, ceil_div((int64_t)m.rows * ((m.cols + 7) / 8), 256))); });
   hipLaunchKernelGGL(k_ortho_pack<NP>, dim3(grid), dim3(256), 0, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
-  for (g.k = 0; g.k < g.steps; ++g.k) {
-    if (int rc = launch_sym<NP, 0>(g, s)) return rc;
-    if (int rc = launch_sym<NP, 1>(g, s)) return rc;
-    if (int rc = g.k + 1 < g.steps ? launch_update<NP, false>(g, s) : launch_update<NP, true>(g, s)) return rc;
-  }
+  Group part[3];  // the matrices of a phase by groups 1, 2, 4
+  for (int k = 0; k < g.steps; ++k)
+    for (Phase p : {kGram, kPoly, kUpdate}) {
+      for (int c = 0; c < 3; ++c) {
+        part[c] = g;
+        part[c].n = 0;
+        part[c].k = k;
+      }
+      for (int i = 0; i < g.n; ++i) {
+        Group& to = part[groups_of(g.m[i], p, NP) >> 1];
+        to.m[to.n++] = g.m[i];
+      }
+      for (int c = 0; c < 3; ++c) {
+        if (part[c].n == 0) continue;
+        const int groups = 1 << c;
+        int rc;
+        if (p == kGram) rc = launch_sym<NP, 0>(part[c], groups, s);
+        else if (p == kPoly) rc = launch_sym<NP, 1>(part[c], groups, s);
+        else rc = k + 1 < g.steps ? launch_update<NP, false>(part[c], groups, s) : launch_update<NP, true>(part[c], groups, s);
+        if (rc) return rc;
+      }
+    }
   return 0;
 }
 
