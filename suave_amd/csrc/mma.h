@@ -485,6 +485,37 @@ __device__ __forceinline__ void planes(float x, uint16_t& hi, uint16_t& lo) {
   lo = __builtin_isinf((float)h) ? 0 : f16_bits((_Float16)r);
 }
 
+// Rows of a wave's tile leave through LDS: a lane holds four neighbours of one row (8 bytes of 16-bit values), stored as they are a
+// wave instruction touches 16 rows by 32 bytes.  Staged 16 rows at a time (wave-private, no barrier) they leave as whole rows of
+// COLS elements, 16 bytes per lane.  The pitch keeps the 16 rows of a write on distinct banks.
+template <class E, int COLS>
+struct RowStage {
+  static constexpr int kRowBytes = COLS * (int)sizeof(E), kPitch = kRowBytes + 16, kBytes = 16 * kPitch;
+  static constexpr int kLanes = kRowBytes / 16;  // lanes per row
+  static_assert(kRowBytes % 16 == 0, "whole 16-byte pieces");
+  // four neighbours of row r (0 .. 15) from column c (a multiple of 4)
+  static __device__ __forceinline__ void put(char* lds, int r, int c, const E (&v)[4]) {
+    if constexpr (sizeof(E) == 2) *reinterpret_cast<uint2*>(lds + r * kPitch + c * 2) = *reinterpret_cast<const uint2*>(v);
+    else *reinterpret_cast<float4*>(lds + r * kPitch + c * 4) = *reinterpret_cast<const float4*>(v);
+  }
+  // rows 0 .. rows - 1, columns 0 .. cols - 1 to out (16-byte aligned rows of ld bytes)
+  static __device__ __forceinline__ void flush(const char* lds, char* out, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll
+    for (int p = 0; p < (16 * kLanes + 63) / 64; ++p) {
+      const int at = p * 64 + lane, r = at / kLanes, c = (at % kLanes) * (16 / (int)sizeof(E));
+      if (r >= rows || c >= cols) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(lds + r * kPitch + c * sizeof(E));
+      char* o = out + r * ld + c * sizeof(E);
+      if (c + 16 / (int)sizeof(E) <= cols) {
+        *reinterpret_cast<uint4*>(o) = v;
+      } else {
+        const E* e = reinterpret_cast<const E*>(&v);
+        for (int u = 0; c + u < cols; ++u) reinterpret_cast<E*>(o)[u] = e[u];
+      }
+    }
+  }
+};
+
 // Dynamic LDS beyond 64 KB has to be allowed once per kernel and device; `done` is the caller's record for one kernel.
 inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
   if (bytes <= 64 * 1024) return hipSuccess;

@@ -9,15 +9,17 @@
 // that holds an infinity or a NaN gets that as its scale and q = 0: its outputs are NaN.
 //
 // The sums are exact int32 (127^2 * 2^17 < 2^31).  Two kernels, by the number of rows:
-//  * up to 64 rows the call is bound by reading Q once: k_linear_rows.  A block owns 64 channels, its four waves a quarter of
-//    K each; a wave loads the 16 x 64 byte fragments of Q straight into registers (no LDS: nothing is reused) and those of q
-//    through L2; the four partial sums meet in LDS.
-//  * above, the tile product of mma.h (K step 128, 256 x 256 or 128 x 128 tiles), bound by the matrix pipe.
+//  * up to 64 rows and few channels the call is a chain of latencies: k_linear_rows.  A block owns 64 channels, its four waves
+//    a quarter of K each; a wave loads the 16 x 64 byte fragments of Q straight into registers (no LDS: nothing is reused)
+//    and those of q through L2; the four partial sums meet in LDS.
+//  * otherwise the tile product of mma.h: with few rows and many channels 16 x 256 or 64 x 256 tiles, bound by reading Q once;
+//    above, square tiles, bound by the matrix pipe or, for short K, by writing the result.
 #include <algorithm>
 #include <cmath>
 
 #include "kernels.h"
 #include "mma.h"
+#include "tiles.h"
 
 namespace suave {
 
@@ -36,7 +38,13 @@ struct QuantArgs {
   int vec;  // rows may be read 16 bytes at a time
 };
 
-__device__ __forceinline__ int quantize_one(float x, float s, float inv) {
+// The quotient by the reciprocal is off by at most 127 * 3 * 2^-24 < 3e-5: away from a half-integer it decides
+__device__ __forceinline__ bool quantize_near(float x, float inv, int& k) {
+  const float t = x * inv, r = rintf(t);
+  k = (int)r;
+  return fabsf(t - r) > 0.4999f;
+}
+__device__ __forceinline__ int quantize_exact(float x, float s, float inv) {
   const float k = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
   const float up = fmaf(-(k + 0.5f), s, x), down = fmaf(-(k - 0.5f), s, x);  // signs are exact: one rounding each
   const int ki = (int)k;
@@ -57,11 +65,11 @@ template <> __device__ __forceinline__ float as_float<float>(float v) { return v
 template <> __device__ __forceinline__ float as_float<uint16_t>(uint16_t v) { return bf16_value(v); }
 
 template <class T>
-__device__ __forceinline__ void load16(const T* row, int k0, int cols, int vec, float (&v)[16]) {  // zeros past the row
-  if (vec && k0 + 16 <= cols) {
+__device__ __forceinline__ void load8(const T* row, int k0, int cols, int vec, float (&v)[8]) {  // zeros past the row
+  if (vec && k0 + 8 <= cols) {
     constexpr int per = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16 / per; ++i) {
+    for (int i = 0; i < 8 / per; ++i) {
       const uint4 u = *reinterpret_cast<const uint4*>(row + k0 + i * per);
       const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
@@ -69,30 +77,35 @@ __device__ __forceinline__ void load16(const T* row, int k0, int cols, int vec, 
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k0 + i < cols ? as_float<T>(row[k0 + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = k0 + i < cols ? as_float<T>(row[k0 + i]) : 0.f;
   }
 }
 
-// W waves share a row: 16 values per lane and pass; the first pass's values stay in registers, rows beyond are read twice
-template <class T, int W>
+// W waves share a row; a lane keeps P runs of 8 values, all loaded at once, and quantises them from its registers.  What a
+// row holds beyond W P 512 values is read twice.
+template <class T, int W, int P>
 __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
   __shared__ uint32_t part[4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * (4 / W) + wave / W;
   const int t = (wave % W) * 64 + lane;
+  constexpr int kRun = W * 64 * 8;
   const bool in = r < a.rows;
   const T* row = static_cast<const T*>(a.x) + (in ? r : 0) * a.ld;
-  float v[16];
-  load16<T>(row, t * 16, a.cols, a.vec, v);
+  float v[P][8];
+#pragma unroll
+  for (int p = 0; p < P; ++p) load8<T>(row, p * kRun + t * 8, a.cols, a.vec, v[p]);
   // |x| as an integer: monotonic, infinity above every number and NaN above infinity, so neither is lost in the maximum
   uint32_t mx = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
-  for (int k0 = (t + W * 64) * 16; k0 < a.cols; k0 += W * 64 * 16) {
-    float u[16];
-    load16<T>(row, k0, a.cols, a.vec, u);
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(u[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[p][i]) & 0x7fffffffu);
+  for (int k0 = P * kRun + t * 8; k0 < a.cols; k0 += kRun) {
+    float u[8];
+    load8<T>(row, k0, a.cols, a.vec, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(u[i]) & 0x7fffffffu);
   }
   for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
   if constexpr (W > 1) {
@@ -108,12 +121,27 @@ __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
   const bool finite = mx < 0x7f800000u, tiny = s < 1e-30f;
   const float inv = 1.0f / s;
   const int end = (a.cols + 15) / 16 * 16;
-  for (int k0 = t * 16; k0 < end; k0 += W * 64 * 16) {
-    if (k0 != t * 16) load16<T>(row, k0, a.cols, a.vec, v);
-    int8_t o[16];
+  auto write = [&](int k0, const float (&u)[8]) {
+    int k[8];
+    bool near = !finite || tiny;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = (int8_t)(!finite ? 0 : tiny ? quantize_tiny(v[i], s) : quantize_one(v[i], s, inv));
-    *reinterpret_cast<uint4*>(a.q + r * a.ldq + k0) = *reinterpret_cast<const uint4*>(o);
+    for (int i = 0; i < 8; ++i) near = quantize_near(u[i], inv, k[i]) || near;
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = !finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv);
+    }
+    uint2 o;
+    o.x = (k[0] & 255) | (k[1] & 255) << 8 | (k[2] & 255) << 16 | (uint32_t)k[3] << 24;
+    o.y = (k[4] & 255) | (k[5] & 255) << 8 | (k[6] & 255) << 16 | (uint32_t)k[7] << 24;
+    *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = o;
+  };
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (p * kRun + t * 8 < end) write(p * kRun + t * 8, v[p]);
+  for (int k0 = P * kRun + t * 8; k0 < end; k0 += kRun) {
+    float u[8];
+    load8<T>(row, k0, a.cols, a.vec, u);
+    write(k0, u);
   }
 }
 
@@ -126,7 +154,7 @@ struct ProductArgs {
   int64_t M;
   int N, K;
   void* out; int64_t ld_out;
-  int bf16, vec;
+  int bf16, vec;   // vec: rows of out may be stored four elements at a time (1), 16 bytes at a time (2)
   int group;
 };
 
@@ -172,19 +200,34 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_linear_tile(ProductArgs a) {
       sw[j][u] = n < a.N ? a.ws[n] : 0.f;
       b[j][u] = n < a.N && a.bias ? a.bias[n] : 0.f;
     }
+  const int n_wave = n_base + wn * (T::NI * 16);
+  typedef RowStage<uint16_t, T::NI * 16> Half;
+  typedef RowStage<float, T::NI * 16> Full;
+  char* stage = lds + wave * Full::kBytes;
+  static_assert(T::WM * T::WN * Full::kBytes <= T::kLds, "the stages fit the tile's LDS");
 #pragma unroll
   for (int i = 0; i < T::MI; ++i) {
-    const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
-    if (m >= a.M) continue;
-    const float sx = a.xs[m];
+    const int64_t m0 = m_base + wm * (T::MI * 16) + 16 * i, m = m0 + (lane & 15);
+    const float sx = m < a.M ? a.xs[m] : 0.f;
 #pragma unroll
     for (int j = 0; j < T::NI; ++j) {
-      const int n = n_base + wn * (T::NI * 16) + 16 * j + 4 * (lane >> 4);
-      if (n >= a.N) continue;
+      const int n = n_wave + 16 * j + 4 * (lane >> 4);
       float v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = fmaf((float)acc[i][j][u], sx * sw[j][u], b[j][u]);
-      store_out(a, m, n, v);
+      if (a.vec < 2) {
+        if (m < a.M && n < a.N) store_out(a, m, n, v);
+      } else if (a.bf16) {
+        const uint16_t h[4] = {bf16_bits(v[0]), bf16_bits(v[1]), bf16_bits(v[2]), bf16_bits(v[3])};
+        Half::put(stage, lane & 15, n - n_wave, h);
+      } else {
+        Full::put(stage, lane & 15, n - n_wave, v);
+      }
+    }
+    if (a.vec == 2 && m0 < a.M && n_wave < a.N) {
+      const int rows = (int)min<int64_t>(16, a.M - m0), cols = a.N - n_wave;
+      if (a.bf16) Half::flush(stage, reinterpret_cast<char*>(static_cast<uint16_t*>(a.out) + m0 * a.ld_out + n_wave), a.ld_out * 2, rows, cols, lane);
+      else Full::flush(stage, reinterpret_cast<char*>(static_cast<float*>(a.out) + m0 * a.ld_out + n_wave), a.ld_out * 4, rows, cols, lane);
     }
   }
 }
@@ -222,7 +265,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a) {
       const bool in = s + u < s1 && c < chunks;           // past the row: q is taken as zero, so whatever Q gives does not count
       const int64_t off = (int64_t)(in ? c : 0) * 16;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[u][j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp[j] + off));
+      for (int j = 0; j < 4; ++j) w[u][j] = *reinterpret_cast<const i32x4*>(wp[j] + off);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         x[u][i] = *reinterpret_cast<const i32x4*>(xp[i] + off);
@@ -279,11 +322,20 @@ int launch_tile(ProductArgs a, hipStream_t s) {
   return 0;
 }
 
+// A wave per row; four where the rows are few (the chain of one row is then what takes the time) or long
+template <class T, int W>
+void launch_quantize_w(const QuantArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.rows + 4 / W - 1) / (4 / W)));
+  const int runs = (a.cols + W * 512 - 1) / (W * 512);
+  if (runs <= 1) hipLaunchKernelGGL((k_quantize_rows<T, W, 1>), grid, dim3(256), 0, s, a);
+  else if (runs <= 2) hipLaunchKernelGGL((k_quantize_rows<T, W, 2>), grid, dim3(256), 0, s, a);
+  else if (runs <= 4) hipLaunchKernelGGL((k_quantize_rows<T, W, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_quantize_rows<T, W, 8>), grid, dim3(256), 0, s, a);
+}
 template <class T>
 void launch_quantize(const QuantArgs& a, hipStream_t s) {
-  // a wave per row up to 2048 columns (two passes of 1024), then four
-  if (a.cols <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_quantize_rows<T, 4>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+  if (a.rows <= 512 || a.cols > 4096) launch_quantize_w<T, 4>(a, s);
+  else launch_quantize_w<T, 1>(a, s);
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -344,13 +396,37 @@ int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
   ProductArgs a{};
   a.x = q; a.ldx = ldq; a.xs = xs; a.w = h->weight; a.ldw = h->ld_weight; a.ws = h->weight_scale; a.bias = h->bias;
   a.M = h->n_rows; a.N = h->n_out; a.K = h->n_in; a.out = h->out; a.ld_out = h->ld_out; a.bf16 = h->dtype == SUAVE_DTYPE_BF16;
-  a.vec = h->ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(h->out) & (a.bf16 ? 7 : 15)) == 0;
+  const int per = a.bf16 ? 8 : 4;  // elements of 16 bytes
+  a.vec = h->ld_out % per == 0 && (reinterpret_cast<uintptr_t>(h->out) & 15) == 0 ? 2
+          : h->ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(h->out) & (a.bf16 ? 7 : 15)) == 0 ? 1 : 0;
   const unsigned blocks = (unsigned)((h->n_out + kRowChannels - 1) / kRowChannels);
+  // Few rows: with 256 channels for half the CUs at least, tiles as low as the batch stream the weights best (16 x 100000 x 2048: 47
+  // us against 74 by k_linear_rows, 64 x 100000 x 1000: 38 against 54); with fewer, blocks of 64 channels and K over the waves
+  // (1 x 5000 x 4096: 21 us against 29).
+  const bool many = (a.N + 255) / 256 >= 128;
+  if (a.M <= 16 && many) return launch_tile<Tile<kI8, 1, false, false, 16, 256, 1, 4>>(a, s);
+  if (a.M <= 64 && many) return launch_tile<Tile<kI8, 1, false, false, 64, 256, 1, 4>>(a, s);
   if (a.M <= 16) hipLaunchKernelGGL(k_linear_rows<1>, dim3(blocks), dim3(256), 0, s, a);
   else if (a.M <= 32) hipLaunchKernelGGL(k_linear_rows<2>, dim3(blocks), dim3(256), 0, s, a);
   else if (a.M <= 64) hipLaunchKernelGGL(k_linear_rows<4>, dim3(blocks), dim3(256), 0, s, a);
-  else if ((a.M + 255) / 256 * ((a.N + 255) / 256) >= 256) return launch_tile<Tile<kI8, 1, false, false, 256, 256, 2, 4>>(a, s);
-  else return launch_tile<Tile<kI8, 1, false, false, 128, 128, 2, 2>>(a, s);
+  else {
+    // the tile with the smallest estimated time
+    int best = kT64;
+    double us = 1e30;
+    for (int t = 0; t < kTileIds; ++t) {
+      if (t == kT64x128) continue;
+      const Work w{(a.M + kTileM[t] - 1) / kTileM[t] * ((a.N + kTileN[t] - 1) / kTileN[t]), (a.K + 127) / 128, 0.0};
+      const int one = 1;
+      const double e = estimate_us((TileId)t, 1, &w, &one, 1);
+      if (e < us * 0.98) { us = e; best = t; }
+    }
+    switch (best) {
+      case kT64: return launch_tile<Tile<kI8, 1, false, false, 64, 64, 2, 2>>(a, s);
+      case kT96: return launch_tile<Tile<kI8, 1, false, false, 96, 96, 2, 2>>(a, s);
+      case kT128: return launch_tile<Tile<kI8, 1, false, false, 128, 128, 2, 2>>(a, s);
+      default: return launch_tile<Tile<kI8, 1, false, false, 256, 256, 2, 4>>(a, s);
+    }
+  }
   SUAVE_CHECK_HIP(hipGetLastError());
   return 0;
 }
