@@ -38,11 +38,17 @@ struct QuantArgs {
   int vec;  // rows may be read 16 bytes at a time
 };
 
-// The quotient by the reciprocal is off by at most 127 * 3 * 2^-24 < 3e-5: away from a half-integer it decides
-__device__ __forceinline__ bool quantize_near(float x, float inv, int& k) {
-  const float t = x * inv, r = rintf(t);
-  k = (int)r;
-  return fabsf(t - r) > 0.4999f;
+// Adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits.  The quotient by the reciprocal is off
+// by at most 127 * 3 * 2^-24 < 3e-5: away from a half-integer it decides.
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ uint32_t quantize_near(float x, float inv, float& off) {
+  const float t = fmaf(x, inv, kRound);
+  off = fmaxf(off, fabsf(fmaf(x, inv, kRound - t)));
+  return __float_as_uint(t);
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+  return __builtin_amdgcn_perm(cd, ab, 0x05040100u);
 }
 __device__ __forceinline__ int quantize_exact(float x, float s, float inv) {
   const float k = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
@@ -122,17 +128,15 @@ __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
   const float inv = 1.0f / s;
   const int end = (a.cols + 15) / 16 * 16;
   auto write = [&](int k0, const float (&u)[8]) {
-    int k[8];
-    bool near = !finite || tiny;
+    uint32_t k[8];
+    float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) near = quantize_near(u[i], inv, k[i]) || near;
-    if (near) {
+    for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], inv, off);
+    if (!finite || tiny || off > 0.4999f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = !finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv);
+      for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(!finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv));
     }
-    uint2 o;
-    o.x = (k[0] & 255) | (k[1] & 255) << 8 | (k[2] & 255) << 16 | (uint32_t)k[3] << 24;
-    o.y = (k[4] & 255) | (k[5] & 255) << 8 | (k[6] & 255) << 16 | (uint32_t)k[7] << 24;
+    const uint2 o = make_uint2(low_bytes(k[0], k[1], k[2], k[3]), low_bytes(k[4], k[5], k[6], k[7]));
     *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = o;
   };
 #pragma unroll
@@ -333,9 +337,17 @@ void launch_quantize_w(const QuantArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((k_quantize_rows<T, W, 8>), grid, dim3(256), 0, s, a);
 }
 template <class T>
-void launch_quantize(const QuantArgs& a, hipStream_t s) {
-  if (a.rows <= 512 || a.cols > 4096) launch_quantize_w<T, 4>(a, s);
-  else launch_quantize_w<T, 1>(a, s);
+void launch_quantize(QuantArgs a, hipStream_t s) {
+  const int64_t rows = a.rows, step = 1 << 23;  // a launch is limited to 2^32 threads
+  for (int64_t r = 0; r < rows; r += step) {
+    QuantArgs p = a;
+    p.x = static_cast<const T*>(a.x) + r * a.ld;
+    p.rows = std::min(step, rows - r);
+    p.q += r * a.ldq;
+    p.scale += r;
+    if (rows <= 512 || a.cols > 4096) launch_quantize_w<T, 4>(p, s);
+    else launch_quantize_w<T, 1>(p, s);
+  }
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
