@@ -38,7 +38,6 @@ struct Scalars {
   float x_scale, w_scale;    // powers of two the planes were multiplied by (1 for bf16)
   float g_unit;              // loss_scale * max_w / total / g_scale: what one unit of the stored G is worth
   float max_w;               // largest |class weight| (1 for bf16 and without class weights): G is stored relative to it
-  uint32_t ticket;           // blocks of k_lce_rows that have written their partial sums
 };
 
 // G is stored relative to the largest row weight (entries in [-1, 1]) times 2^14: fp16's hi plane is normal down to 2^-28
@@ -62,50 +61,56 @@ struct PackArgs {
   int C, C_pad;
 };
 
-__device__ __forceinline__ float load_as_float(const float* p) { return *p; }
-__device__ __forceinline__ float load_as_float(const uint16_t* p) { return bf16_value(*p); }
+// Eight neighbours in 16-byte loads, wherever the row begins (the memory system takes them at element alignment)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const f32x4_any a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+__device__ __forceinline__ void load8(const uint16_t* p, uint16_t (&v)[8]) {
+  const u16x8_any a = *reinterpret_cast<const u16x8_any*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = a[i];
+}
+__device__ __forceinline__ int64_t row_of(int64_t chunk, int64_t chunks, int q) {  // 32-bit division where it reaches
+  return chunks <= 0xffffffffll ? (int64_t)((uint32_t)chunk / (uint32_t)q) : chunk / q;
+}
 
 __device__ __forceinline__ float finite_abs(float v) {
   v = fabsf(v);
   return v < INFINITY ? v : 0.f;  // (a NaN compares false)
 }
 
-// largest finite |value| of rows first, first + step, ...: of x (rows that count) or W, this thread's share
+// largest finite |value| of x (rows that count) or W: the share of thread `first` of `step`, in chunks of eight
 __device__ __forceinline__ float scan_rows(const PackArgs& a, int t, int64_t first, int64_t step) {
   const float* src = static_cast<const float*>(a.src[t]);
-  const int64_t rows = a.rows[t], ld = a.ld[t];
+  const int64_t ld = a.ld[t];
+  const int q = (a.D + 7) / 8;
+  const int64_t chunks = a.rows[t] * q;
   float m = 0.f;
-  if (t == 1 && ld == a.D && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {  // one flat array: `first` / `step` are threads
-    const int64_t total = rows * ld, quads = total / 4;
-    const float4* p = reinterpret_cast<const float4*>(src);
-    int64_t e = first;
-    for (; e + 3 * step < quads; e += 4 * step) {
-      float4 v[4];
+  constexpr int U = 4;  // chunks in flight
+  for (int64_t e0 = first; e0 < chunks; e0 += U * step) {
+    float v[U][8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = p[e + u * step];
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)), fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
-    }
-    for (; e < quads; e += step) {
-      const float4 v = p[e];
-      m = fmaxf(m, fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
-    }
-    if (first < total - 4 * quads) m = fmaxf(m, finite_abs(src[4 * quads + first]));
-    return m;
-  }
-  if (a.D >= 64) {  // a wave per row
-    const int lane = (int)(first & 63);
-    for (int64_t r = first >> 6; r < rows; r += step >> 6) {
+      for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+      const int64_t e = e0 + u * step;
+      if (e >= chunks) continue;
+      const int64_t r = row_of(e, chunks, q);
+      const int d0 = (int)(e - r * q) * 8;
       if (t == 0 && a.targets[r] < 0) continue;
       const float* p = src + r * ld;
-      for (int d = lane; d < a.D; d += 64) m = fmaxf(m, finite_abs(p[d]));
+      if (a.D >= 8) load8(p + min(d0, a.D - 8), v[u]);  // (the last chunk may repeat some of the one before)
+      else
+        for (int i = 0; i < a.D; ++i) v[u][i] = p[i];
     }
-  } else {  // narrow rows: a thread per row
-    for (int64_t r = first; r < rows; r += step) {
-      if (t == 0 && a.targets[r] < 0) continue;
-      const float* p = src + r * ld;
-      for (int d = 0; d < a.D; ++d) m = fmaxf(m, finite_abs(p[d]));
-    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[u][i]));
   }
   return m;
 }
@@ -166,7 +171,6 @@ __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
     if (t == 0) {
       a.scal->x_scale = scale;
       a.scal->max_w = max_w;
-      a.scal->ticket = 0;
     } else {
       a.scal->w_scale = scale;
     }
@@ -180,24 +184,65 @@ __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
   const int q = a.Dp / 8;  // 16-byte chunks of a row
   const int64_t chunks = a.rows[t] * q, ld = a.ld[t];
   for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
-    const int64_t r = e / q;
+    const int64_t r = row_of(e, chunks, q);
     const int d0 = (int)(e - r * q) * 8;
     const bool gone = t == 0 && a.targets[r] < 0;
     const T* p = src + r * ld + d0;
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)0;
+    if (!gone) {
+      if (d0 + 8 <= a.D) load8(p, v);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (d0 + i < a.D) v[i] = p[i];
+    }
     uint16_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = !gone && d0 + i < a.D;
-      if constexpr (PLANES) {
-        planes(in ? load_as_float(p + i) * scale : 0.f, hi[i], lo[i]);
-      } else {
-        hi[i] = in ? p[i] : (T)0;
-      }
+      if constexpr (PLANES) planes(v[i] * scale, hi[i], lo[i]);
+      else hi[i] = v[i];
     }
     char* o = a.dst[t] + r * a.dst_ld[t] + d0 * 2;
     *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
     if constexpr (PLANES) *reinterpret_cast<uint4*>(o + (size_t)a.Dp * 2) = *reinterpret_cast<const uint4*>(lo);
   }
+}
+
+struct TotalArgs {   // loss and the unit of G, from the partial sums of k_lce_rows
+  const double* part; int blocks;  // [blocks][2]: sum of ce, sum of w
+  const float* weight_sum; float loss_scale, loss_rows; float gs;
+  float* loss; double* loss_sum; Scalars* scal;
+};
+// Every thread of a block of 256 or more takes part; the first 256 add, in a fixed order.
+__device__ __forceinline__ void total_loss(const TotalArgs& a, double (&sce)[4], double (&sw)[4]) {
+  if (threadIdx.x < 256) {
+    double ce = 0.0, w = 0.0;
+    for (int i = threadIdx.x; i < a.blocks; i += 256) {
+      ce += a.part[2 * i];
+      w += a.part[2 * i + 1];
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+      ce += __shfl_xor(ce, off, 64);
+      w += __shfl_xor(w, off, 64);
+    }
+    if ((threadIdx.x & 63) == 0) { sce[threadIdx.x >> 6] = ce; sw[threadIdx.x >> 6] = w; }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double ce = ((sce[0] + sce[1]) + sce[2]) + sce[3], w = ((sw[0] + sw[1]) + sw[2]) + sw[3];
+    const double total = a.weight_sum ? (double)*a.weight_sum : w;
+    const bool none = total == 0.0;  // (NaN stays NaN)
+    const double loss = none ? 0.0 : ce / total;
+    if (a.loss) *a.loss = (float)loss;
+    if (a.loss_sum) *a.loss_sum += loss * (double)a.loss_rows;
+    a.scal->g_unit = none ? 0.f : (float)((double)a.loss_scale * (double)a.scal->max_w / total / (double)a.gs);
+  }
+}
+__global__ __launch_bounds__(256) void k_lce_total(TotalArgs a) {
+  __shared__ double sce[4], sw[4];
+  total_loss(a, sce, sw);
 }
 
 struct LogitArgs {
@@ -219,35 +264,68 @@ struct LogitArgs {
   char* g; int64_t ldg; uint32_t g_plane;  // [n][c1 - c0 rounded up], bytes
   float* db;                       // [row tiles of a wave][C_pad]
   int64_t db_ld;
+  int totals;                      // 1: the first block of the launch finishes the loss instead
+  TotalArgs total;
 };
 
-// One tile of logits; SWEEP 0: strip statistics, 1: G
+// One tile of logits; SWEEP 0: strip statistics, 1: G.  What the epilogue needs of bias, targets and rows is asked for before the
+// product, one value per thread, and spread through LDS behind it: the matrix pipe covers the latency.
 template <class T, int SWEEP>
 __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  int block = blockIdx.x, blocks = gridDim.x;
+  if constexpr (SWEEP == 1) {
+    if (a.totals) {
+      if (block == 0) {
+        double* d = reinterpret_cast<double*>(lds);
+        total_loss(a.total, *reinterpret_cast<double(*)[4]>(d), *reinterpret_cast<double(*)[4]>(d + 4));
+        return;
+      }
+      --block; --blocks;
+    }
+  }
   const int tiles_m = (int)((a.n + T::BM - 1) / T::BM), tiles_n = (a.c1 - a.c0 + T::BN - 1) / T::BN;
   int tm, tn;
-  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, a.group, tm, tn);
+  tile_of(block, blocks, tiles_m, tiles_n, a.group, tm, tn);
   const int64_t m_base = (int64_t)tm * T::BM;
   const int c_base = a.c0 + tn * T::BN;
+  const int t = threadIdx.x;
+  static_assert(T::BM <= T::kThreads && T::BN <= T::kThreads, "one value per thread");
+  const bool has_row = t < T::BM && m_base + t < a.n;
+  const float my_bias = t < T::BN ? a.bias[c_base + t] : 0.f;
+  const int my_target = has_row ? a.targets[m_base + t] : -1;
+  float2 my_row = make_float2(0.f, 0.f);
+  if (SWEEP == 1 && has_row) my_row = a.row[m_base + t];
+  const float unit = 1.0f / (a.scal->x_scale * a.scal->w_scale);  // a power of two
   const Operand A{a.x + m_base * a.ldx, (uint32_t)a.ldx, (int)min<int64_t>(T::BM, a.n - m_base), a.plane};
   const Operand B{a.w + (int64_t)c_base * a.ldw, (uint32_t)a.ldw, a.C - c_base, a.plane};
   typename T::acc_t acc[T::MI][T::NI];
   T::run(lds, A, B, a.D, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = t & 63, wave = t >> 6;
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int g = lane >> 4;
-  const float unit = 1.0f / (a.scal->x_scale * a.scal->w_scale);  // a power of two
-  const int cw = c_base + wn * (T::NI * 16);
+  static_assert(T::NI * 16 == kStrip, "a wave owns one strip");
+  typedef RowStage<uint16_t, kStrip> Rows;
+  float2* row_tab = reinterpret_cast<float2*>(lds);
+  float* bias_tab = reinterpret_cast<float*>(row_tab + T::BM);
+  int* target_tab = reinterpret_cast<int*>(bias_tab + T::BN);
+  constexpr int kTabs = T::BM * 12 + T::BN * 4;
+  static_assert(kTabs % 16 == 0 && kTabs + T::WM * T::WN * T::NP * Rows::kBytes <= T::kLds, "tables and stages fit the tile's LDS");
+  if (t < T::BN) bias_tab[t] = my_bias;
+  if (t < T::BM) {
+    target_tab[t] = my_target;
+    if (SWEEP == 1) row_tab[t] = my_row;
+  }
+  __syncthreads();
+  const int cw = c_base + wn * kStrip;
   float4 bias[T::NI];
 #pragma unroll
-  for (int j = 0; j < T::NI; ++j) bias[j] = *reinterpret_cast<const float4*>(a.bias + cw + 16 * j + 4 * g);
-  static_assert(T::NI * 16 == kStrip, "a wave owns one strip");
+  for (int j = 0; j < T::NI; ++j) bias[j] = *reinterpret_cast<const float4*>(bias_tab + wn * kStrip + 16 * j + 4 * g);
   if constexpr (SWEEP == 0) {
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
-      const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
-      const int y = m < a.n ? a.targets[m] : -1;
+      const int ml = wm * (T::MI * 16) + 16 * i + (lane & 15);
+      const int64_t m = m_base + ml;
       float v[T::NI][4], mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
@@ -256,8 +334,15 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
         for (int u = 0; u < 4; ++u) {
           v[j][u] = fmaf(acc[i][j][u], unit, bj[u]);
           mx = fmaxf(mx, v[j][u]);
-          if (cw + 16 * j + 4 * g + u == y) a.target_logit[m] = v[j][u];
         }
+      }
+      const int at = target_tab[ml] - cw;  // the target's place in the strip
+      if (__any(at >= 0 && at < kStrip)) {
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (16 * j + 4 * g + u == at) a.target_logit[m] = v[j][u];
       }
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -273,6 +358,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
     }
   } else {
     constexpr bool P = T::NP == 2;
+    char* stage = lds + kTabs + wave * (T::NP * Rows::kBytes);
     float cs[T::NI][4];
 #pragma unroll
     for (int j = 0; j < T::NI; ++j)
@@ -280,30 +366,41 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
       for (int u = 0; u < 4; ++u) cs[j][u] = 0.f;
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
-      const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
-      const bool in = m < a.n;
-      const int y = in ? a.targets[m] : -1;
-      const float2 rw = in ? a.row[m] : make_float2(0.f, 0.f);
-      char* grow = a.g + m * a.ldg + (int64_t)(cw - a.c0 + 4 * g) * 2;
+      const int m0 = wm * (T::MI * 16) + 16 * i, ml = m0 + (lane & 15);
+      const float2 rw = row_tab[ml];
+      const int at = target_tab[ml] - cw;
+      float p[T::NI][4];
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
         const float* bj = reinterpret_cast<const float*>(&bias[j]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[j][u] = __expf(fmaf(acc[i][j][u], unit, bj[u]) - rw.x);
+      }
+      if (__any(at >= 0 && at < kStrip)) {
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (16 * j + 4 * g + u == at) p[j][u] -= 1.0f;
+      }
+      const bool counts = rw.y != 0.f;  // a row without weight contributes nothing, whatever it holds
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
         uint16_t hi[4], lo[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const float l = fmaf(acc[i][j][u], unit, bj[u]);
-          float p = __expf(l - rw.x);
-          if (cw + 16 * j + 4 * g + u == y) p -= 1.0f;
-          const float gv = rw.y == 0.f ? 0.f : p * rw.y;  // a row without weight contributes nothing, whatever it holds
+          const float gv = counts ? p[j][u] * rw.y : 0.f;
           cs[j][u] += gv;
           if constexpr (P) planes(gv * g_scale(true), hi[u], lo[u]);
           else hi[u] = bf16_bits(gv);
         }
-        if (in) {
-          *reinterpret_cast<uint2*>(grow + 32 * j) = *reinterpret_cast<const uint2*>(hi);
-          if constexpr (P) *reinterpret_cast<uint2*>(grow + 32 * j + a.g_plane) = *reinterpret_cast<const uint2*>(lo);
-        }
+        Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
+        if constexpr (P) Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
       }
+      const int rows = (int)max<int64_t>(0, min<int64_t>(16, a.n - m_base - m0));
+      char* out = a.g + (m_base + m0) * a.ldg + (int64_t)(cw - a.c0) * 2;
+      Rows::flush(stage, out, a.ldg, rows, kStrip, lane);
+      if constexpr (P) Rows::flush(stage + Rows::kBytes, out + a.g_plane, a.ldg, rows, kStrip, lane);
     }
     if (a.db != nullptr) {  // column sums over the wave's rows: lanes of equal g hold the same columns
 #pragma unroll
@@ -312,10 +409,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
         float* sp = reinterpret_cast<float*>(&s);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          float t = cs[j][u];
+          float v = cs[j][u];
 #pragma unroll
-          for (int off = 8; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
-          sp[u] = t;
+          for (int off = 8; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+          sp[u] = v;
         }
         if ((lane & 15) == 0) *reinterpret_cast<float4*>(a.db + (int64_t)(tm * T::WM + wm) * a.db_ld + cw + 16 * j + 4 * g) = s;
       }
@@ -333,16 +430,14 @@ struct RowArgs {
   float* lse_out;    // or null
   float2* row;       // (lse, w / max_w)
   double* part;      // [blocks][2]: sum of ce, sum of w over the block's rows
-  const float* weight_sum; float loss_scale, loss_rows; float gs;
-  float* loss; double* loss_sum; Scalars* scal;
+  const Scalars* scal;
 };
 
-// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights; the block that is done
-// last adds up the partial sums of all blocks, in their order
+// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights.  The sums over all blocks are
+// left to the next launch: a ticket that lets the last block do it costs every block a release and an acquire at device scope
+// (4096 rows: 18 us, this 8).
 __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
   __shared__ float2 ms[64][17];
-  __shared__ double sce[16], sw[16];
-  __shared__ int last;
   const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int64_t m = (int64_t)blockIdx.x * 16 + r;
   float mx = -INFINITY, s = 0.f;
@@ -399,33 +494,7 @@ __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
     if (threadIdx.x == 0) {
       a.part[2 * blockIdx.x] = ce;
       a.part[2 * blockIdx.x + 1] = wsum;
-      // the partial sums are visible to the whole device before the ticket is, and to the last block behind it
-      last = __hip_atomic_fetch_add(&a.scal->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
     }
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  double ce = 0.0, w = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) {
-    ce += __hip_atomic_load(&a.part[2 * i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    w += __hip_atomic_load(&a.part[2 * i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  for (int off = 32; off > 0; off >>= 1) {
-    ce += __shfl_xor(ce, off, 64);
-    w += __shfl_xor(w, off, 64);
-  }
-  if ((threadIdx.x & 63) == 0) { sce[threadIdx.x >> 6] = ce; sw[threadIdx.x >> 6] = w; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    ce = w = 0.0;
-    for (int k = 0; k < 16; ++k) { ce += sce[k]; w += sw[k]; }
-    const double total = a.weight_sum ? (double)*a.weight_sum : w;
-    const bool none = total == 0.0;  // (NaN stays NaN)
-    const double loss = none ? 0.0 : ce / total;
-    if (a.loss) *a.loss = (float)loss;
-    if (a.loss_sum) *a.loss_sum += loss * (double)a.loss_rows;
-    a.scal->g_unit = none ? 0.f : (float)((double)a.loss_scale * (double)a.scal->max_w / total / (double)a.gs);
   }
 }
 
@@ -679,7 +748,7 @@ int launch_tile(const void* fn, int grid, int threads, int lds, void** args, std
 
 template <class T, int SWEEP>
 int launch_logits_tile(LogitArgs a, hipStream_t s) {
-  const int64_t grid = ceil_div(a.n, T::BM) * ceil_div(a.c1 - a.c0, T::BN);
+  const int64_t grid = ceil_div(a.n, T::BM) * ceil_div(a.c1 - a.c0, T::BN) + a.totals;
   a.group = 8;
   void* args[] = {&a};
   static std::atomic<uint64_t> done{0};
@@ -758,11 +827,15 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
   r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
   r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part);
-  r.weight_sum = h.weight_sum; r.loss_scale = h.loss_scale;
-  r.loss_rows = h.loss_rows; r.gs = g_scale(F); r.loss = h.loss; r.loss_sum = h.loss_sum; r.scal = scal;
+  r.scal = scal;
   hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
   SUAVE_CHECK_HIP(hipGetLastError());
-  if (!grad) return 0;
+  a.total = TotalArgs{r.part, L.row_blocks, h.weight_sum, h.loss_scale, h.loss_rows, g_scale(F), h.loss, h.loss_sum, scal};
+  if (!grad) {
+    hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(256), 0, s, a.total);
+    SUAVE_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
 
   const bool bf = !F;
   auto vec_ok = [&](const void* ptr, int64_t ld) {
@@ -774,6 +847,7 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     a.c0 = piece * L.piece;
     a.c1 = std::min(a.c0 + L.piece, (int)h.n_classes);
     a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
+    a.totals = piece == 0;
     if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
     const int cp = a.c1 - a.c0;
     GradArgs gx{}, gw{};

@@ -500,6 +500,8 @@ struct RowStage {
   }
   // rows 0 .. rows - 1, columns 0 .. cols - 1 to out (16-byte aligned rows of ld bytes)
   static __device__ __forceinline__ void flush(const char* lds, char* out, int64_t ld, int rows, int cols, int lane) {
+    asm volatile("" ::: "memory");  // the reads below are of other lanes' writes: a wave's LDS operations run in order, so order is all they need
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int p = 0; p < (16 * kLanes + 63) / 64; ++p) {
       const int at = p * 64 + lane, r = at / kLanes, c = (at % kLanes) * (16 / (int)sizeof(E));
@@ -513,6 +515,8 @@ struct RowStage {
         for (int u = 0; c + u < cols; ++u) reinterpret_cast<E*>(o)[u] = e[u];
       }
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
   }
 };
 
