@@ -245,6 +245,35 @@ __global__ __launch_bounds__(256) void k_lce_total(TotalArgs a) {
   total_loss(a, sce, sw);
 }
 
+struct RowArgs {
+  const float2* strips; int n_strips;
+  int64_t n;
+  const int32_t* targets; int C;
+  const float* class_weight;
+  const float* target_logit;
+  float* row_loss;   // or null
+  float* lse_out;    // or null
+  float2* row;       // (lse, w / max_w)
+  double* part;      // [blocks][2]: sum of ce, sum of w over the block's rows
+  const Scalars* scal;
+};
+// What a row's lse and its target's logit give: the row's outputs, and its terms of the two sums
+__device__ __forceinline__ void finish_row(const RowArgs& a, int64_t m, float lse, float target_logit, float& ce, float2& row, float& weight) {
+  const int y = a.targets[m];
+  float w = 0.f, l = 0.f;
+  if (y >= a.C) {
+    w = l = NAN;
+  } else if (y >= 0) {
+    w = a.class_weight ? a.class_weight[y] : 1.0f;
+    l = w == 0.f ? 0.f : w * (lse - target_logit);
+  }
+  if (a.row_loss) a.row_loss[m] = l;
+  if (a.lse_out) a.lse_out[m] = lse;
+  row = make_float2(lse, w / a.scal->max_w);
+  ce = l;
+  weight = w;
+}
+
 struct LogitArgs {
   const char* x; int64_t ldx;      // packed [n][..], bytes
   const char* w; int64_t ldw;
@@ -266,9 +295,80 @@ struct LogitArgs {
   int64_t db_ld;
   int totals;                      // 1: the first block of the launch finishes the loss instead
   TotalArgs total;
+  RowArgs rows;                    // whole rows in one tile
 };
 
-// One tile of logits; SWEEP 0: strip statistics, 1: G.  What the epilogue needs of bias, targets and rows is asked for before the
+// G of a tile from its logits and its rows' (lse, weight), and the column sums that db is made of
+template <class T>
+__device__ __forceinline__ void write_gradients(const LogitArgs& a, const typename T::acc_t (&acc)[T::MI][T::NI], const float4 (&bias)[T::NI], float unit,
+                                                int tm, int cw, const float2* row_tab, const int* target_tab, char* stages) {
+  constexpr bool P = T::NP == 2;
+  typedef RowStage<uint16_t, kStrip> Rows;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, g = lane >> 4;
+  const int64_t m_base = (int64_t)tm * T::BM;
+  char* stage = stages + wave * (T::NP * Rows::kBytes);
+  float cs[T::NI][4];
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) cs[j][u] = 0.f;
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i) {
+    const int m0 = wm * (T::MI * 16) + 16 * i, ml = m0 + (lane & 15);
+    const float2 rw = row_tab[ml];
+    const int at = target_tab[ml] - cw;
+    float p[T::NI][4];
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const float* bj = reinterpret_cast<const float*>(&bias[j]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[j][u] = __expf(fmaf(acc[i][j][u], unit, bj[u]) - rw.x);
+    }
+    if (__any(at >= 0 && at < kStrip)) {
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (16 * j + 4 * g + u == at) p[j][u] -= 1.0f;
+    }
+    const bool counts = rw.y != 0.f;  // a row without weight contributes nothing, whatever it holds
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      uint16_t hi[4], lo[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float gv = counts ? p[j][u] * rw.y : 0.f;
+        cs[j][u] += gv;
+        if constexpr (P) planes(gv * g_scale(true), hi[u], lo[u]);
+        else hi[u] = bf16_bits(gv);
+      }
+      Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
+      if constexpr (P) Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
+    }
+    const int rows = (int)max<int64_t>(0, min<int64_t>(16, a.n - m_base - m0));
+    char* out = a.g + (m_base + m0) * a.ldg + (int64_t)(cw - a.c0) * 2;
+    Rows::flush(stage, out, a.ldg, rows, kStrip, lane);
+    if constexpr (P) Rows::flush(stage + Rows::kBytes, out + a.g_plane, a.ldg, rows, kStrip, lane);
+  }
+  if (a.db != nullptr) {  // column sums over the wave's rows: lanes of equal g hold the same columns
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      float4 s;
+      float* sp = reinterpret_cast<float*>(&s);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float v = cs[j][u];
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        sp[u] = v;
+      }
+      if ((lane & 15) == 0) *reinterpret_cast<float4*>(a.db + (int64_t)(tm * T::WM + wm) * a.db_ld + cw + 16 * j + 4 * g) = s;
+    }
+  }
+}
+
+// One tile of logits; SWEEP 0: strip statistics, 1: G, 2: both, for tiles that hold whole rows (few classes: no second product and two
+// launches less; 1000 x 250 x 256 f32: 38 us against 53 in two sweeps).  What the epilogue needs of bias, targets and rows is asked for before the
 // product, one value per thread, and spread through LDS behind it: the matrix pipe covers the latency.
 template <class T, int SWEEP>
 __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
@@ -305,12 +405,13 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int g = lane >> 4;
   static_assert(T::NI * 16 == kStrip, "a wave owns one strip");
-  typedef RowStage<uint16_t, kStrip> Rows;
   float2* row_tab = reinterpret_cast<float2*>(lds);
   float* bias_tab = reinterpret_cast<float*>(row_tab + T::BM);
   int* target_tab = reinterpret_cast<int*>(bias_tab + T::BN);
-  constexpr int kTabs = T::BM * 12 + T::BN * 4;
-  static_assert(kTabs % 16 == 0 && kTabs + T::WM * T::WN * T::NP * Rows::kBytes <= T::kLds, "tables and stages fit the tile's LDS");
+  float2* strip_tab = reinterpret_cast<float2*>(target_tab + T::BM);  // whole rows only
+  float* logit_tab = reinterpret_cast<float*>(strip_tab + T::WN * T::BM);
+  constexpr int kTabs = T::BM * 12 + T::BN * 4 + (SWEEP == 2 ? T::BM * (8 * T::WN + 4) : 0);
+  static_assert(kTabs % 16 == 0 && kTabs + T::WM * T::WN * T::NP * RowStage<uint16_t, kStrip>::kBytes <= T::kLds, "tables and stages fit the tile's LDS");
   if (t < T::BN) bias_tab[t] = my_bias;
   if (t < T::BM) {
     target_tab[t] = my_target;
@@ -321,7 +422,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
   float4 bias[T::NI];
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) bias[j] = *reinterpret_cast<const float4*>(bias_tab + wn * kStrip + 16 * j + 4 * g);
-  if constexpr (SWEEP == 0) {
+  if constexpr (SWEEP != 1) {
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
       const int ml = wm * (T::MI * 16) + 16 * i + (lane & 15);
@@ -342,7 +443,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
         for (int j = 0; j < T::NI; ++j)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (16 * j + 4 * g + u == at) a.target_logit[m] = v[j][u];
+            if (16 * j + 4 * g + u == at) (SWEEP == 2 ? logit_tab[ml] : a.target_logit[m]) = v[j][u];
       }
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -354,84 +455,49 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
         for (int u = 0; u < 4; ++u) s += __expf(v[j][u] - base);
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
-      if (g == 0 && m < a.n && cw < a.c1) a.strips[(int64_t)(cw / kStrip) * a.n + m] = make_float2(base, s);
-    }
-  } else {
-    constexpr bool P = T::NP == 2;
-    char* stage = lds + kTabs + wave * (T::NP * Rows::kBytes);
-    float cs[T::NI][4];
-#pragma unroll
-    for (int j = 0; j < T::NI; ++j)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) cs[j][u] = 0.f;
-#pragma unroll
-    for (int i = 0; i < T::MI; ++i) {
-      const int m0 = wm * (T::MI * 16) + 16 * i, ml = m0 + (lane & 15);
-      const float2 rw = row_tab[ml];
-      const int at = target_tab[ml] - cw;
-      float p[T::NI][4];
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) {
-        const float* bj = reinterpret_cast<const float*>(&bias[j]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) p[j][u] = __expf(fmaf(acc[i][j][u], unit, bj[u]) - rw.x);
-      }
-      if (__any(at >= 0 && at < kStrip)) {
-#pragma unroll
-        for (int j = 0; j < T::NI; ++j)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (16 * j + 4 * g + u == at) p[j][u] -= 1.0f;
-      }
-      const bool counts = rw.y != 0.f;  // a row without weight contributes nothing, whatever it holds
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) {
-        uint16_t hi[4], lo[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float gv = counts ? p[j][u] * rw.y : 0.f;
-          cs[j][u] += gv;
-          if constexpr (P) planes(gv * g_scale(true), hi[u], lo[u]);
-          else hi[u] = bf16_bits(gv);
-        }
-        Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
-        if constexpr (P) Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
-      }
-      const int rows = (int)max<int64_t>(0, min<int64_t>(16, a.n - m_base - m0));
-      char* out = a.g + (m_base + m0) * a.ldg + (int64_t)(cw - a.c0) * 2;
-      Rows::flush(stage, out, a.ldg, rows, kStrip, lane);
-      if constexpr (P) Rows::flush(stage + Rows::kBytes, out + a.g_plane, a.ldg, rows, kStrip, lane);
-    }
-    if (a.db != nullptr) {  // column sums over the wave's rows: lanes of equal g hold the same columns
-#pragma unroll
-      for (int j = 0; j < T::NI; ++j) {
-        float4 s;
-        float* sp = reinterpret_cast<float*>(&s);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float v = cs[j][u];
-#pragma unroll
-          for (int off = 8; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-          sp[u] = v;
-        }
-        if ((lane & 15) == 0) *reinterpret_cast<float4*>(a.db + (int64_t)(tm * T::WM + wm) * a.db_ld + cw + 16 * j + 4 * g) = s;
+      if (SWEEP == 2) {
+        if (g == 0) strip_tab[wn * T::BM + ml] = make_float2(base, s);
+      } else {
+        if (g == 0 && m < a.n && cw < a.c1) a.strips[(int64_t)(cw / kStrip) * a.n + m] = make_float2(base, s);
       }
     }
   }
+  if constexpr (SWEEP == 2) {
+    static_assert(T::BM <= 64, "one wave finishes the rows");
+    __syncthreads();
+    if (t < 64) {
+      double ce = 0.0, w = 0.0;
+      if (has_row) {
+        float mx = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int k = 0; k < T::WN; ++k)
+          if (strip_tab[k * T::BM + t].y != 0.f) mx = fmaxf(mx, strip_tab[k * T::BM + t].x);
+#pragma unroll
+        for (int k = 0; k < T::WN; ++k)
+          if (strip_tab[k * T::BM + t].y != 0.f) s += strip_tab[k * T::BM + t].y * __expf(strip_tab[k * T::BM + t].x - mx);
+        float l, rw;
+        finish_row(a.rows, m_base + t, s == 0.f ? -INFINITY : mx + logf(s), logit_tab[t], l, row_tab[t], rw);
+        ce = l;
+        w = rw;
+      } else if (t < T::BM) {
+        row_tab[t] = make_float2(0.f, 0.f);
+      }
+      for (int off = 32; off > 0; off >>= 1) {
+        ce += __shfl_xor(ce, off, 64);
+        w += __shfl_xor(w, off, 64);
+      }
+      if (t == 0) {
+        a.rows.part[2 * tm] = ce;
+        a.rows.part[2 * tm + 1] = w;
+      }
+    }
+    if (a.g == nullptr) return;
+    __syncthreads();
+  }
+  if constexpr (SWEEP != 0) {
+    write_gradients<T>(a, acc, bias, unit, tm, cw, row_tab, target_tab, lds + kTabs);
+  }
 }
-
-struct RowArgs {
-  const float2* strips; int n_strips;
-  int64_t n;
-  const int32_t* targets; int C;
-  const float* class_weight;
-  const float* target_logit;
-  float* row_loss;   // or null
-  float* lse_out;    // or null
-  float2* row;       // (lse, w / max_w)
-  double* part;      // [blocks][2]: sum of ce, sum of w over the block's rows
-  const Scalars* scal;
-};
 
 // lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights.  The sums over all blocks are
 // left to the next launch: a ticket that lets the last block do it costs every block a release and an acquire at device scope
@@ -473,17 +539,8 @@ __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
     double ce = 0.0, wsum = 0.0;
     if (part == 0 && m < a.n) {
       const float lse = S == 0.f ? -INFINITY : M + logf(S);
-      const int y = a.targets[m];
-      float w = 0.f, l = 0.f;
-      if (y >= a.C) {
-        w = l = NAN;
-      } else if (y >= 0) {
-        w = a.class_weight ? a.class_weight[y] : 1.0f;
-        l = w == 0.f ? 0.f : w * (lse - a.target_logit[m]);
-      }
-      if (a.row_loss) a.row_loss[m] = l;
-      if (a.lse_out) a.lse_out[m] = lse;
-      a.row[m] = make_float2(lse, w / a.scal->max_w);
+      float l, w;
+      finish_row(a, m, lse, a.target_logit[m], l, a.row[m], w);
       ce = l;
       wsum = w;
     }
@@ -552,7 +609,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
   T::run(lds, A, B, k1 - k0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const float f = grad_factor(a.scal, a.which);
+  const float f = a.slab ? 1.0f : grad_factor(a.scal, a.which);
 #pragma unroll
   for (int i = 0; i < T::MI; ++i) {
     const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
@@ -579,10 +636,17 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
 
 // dx and dW of one piece of the classes in one launch: they only share G
 template <class TX, class TW>
-__global__ __launch_bounds__(TX::kThreads, 2) void k_lce_grads(GradArgs dx, GradArgs dw, int dx_blocks) {
+__global__ __launch_bounds__(TX::kThreads, 2) void k_lce_grads(GradArgs dx, GradArgs dw, int dx_blocks, int totals, TotalArgs total) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  if ((int)blockIdx.x < dx_blocks) grad_tile<TX>(dx, blockIdx.x, lds);
-  else grad_tile<TW>(dw, blockIdx.x - dx_blocks, lds);
+  const int block = (int)blockIdx.x - totals;
+  if (block < 0) {  // finishes the loss instead: nothing else in this launch needs it
+    double* d = reinterpret_cast<double*>(lds);
+    total_loss(total, *reinterpret_cast<double(*)[4]>(d), *reinterpret_cast<double(*)[4]>(d + 4));
+  } else if (block < dx_blocks) {
+    grad_tile<TX>(dx, block, lds);
+  } else {
+    grad_tile<TW>(dw, block - dx_blocks, lds);
+  }
 }
 
 struct FinishArgs {  // out = factor * sum over the slabs, for dx and dW; db = unit * sum over the row tiles
@@ -637,6 +701,7 @@ struct Layout {  // offsets into the workspace, bytes
   bool pack_w, dw_direct;
   TileId grad_tile;
   int row_blocks, db_rows;
+  bool whole;            // one sweep: a tile holds whole rows
   int tile_s, tile_g;    // LogitTile of the two sweeps (one per call: the db partials of all pieces have the same rows)
 };
 
@@ -644,13 +709,18 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Tile height and width of the logit products.  Up to 16 and 64 rows the tile is as low as the batch and 256 classes wide
 // (the weights stream past once; a taller tile would multiply rows that are not there); otherwise 256 x 256 with eight
-// waves once that gives every CU a tile, else 128 x 128 (two blocks per CU).
-enum LogitTile : int { kLow16, kLow64, kMid128, kBig256 };
+// waves once that gives every CU a tile, else 128 x 128 (two blocks per CU), or 64 x 128 while there are not enough tiles for
+// every CU either (512 x 4000 x 256 f32: 61 us against 65).  Up to 256 classes a tile of 256 holds whole rows.
+enum LogitTile : int { kLow16, kLow64, kMid64, kMid128, kBig256 };
+constexpr int kLogitM[] = {16, 64, 64, 128, 256}, kLogitWM[] = {1, 1, 2, 2, 2};  // rows, waves side by side in them
 LogitTile logit_tile(int64_t n, int64_t classes) {
   if (n <= 16) return kLow16;
   if (n <= 64) return kLow64;
-  return ceil_div(n, 256) * ceil_div(classes, 256) >= kCUs ? kBig256 : kMid128;
+  if (ceil_div(n, 256) * ceil_div(classes, 256) >= kCUs) return kBig256;
+  return ceil_div(n, 128) * ceil_div(classes, 128) >= kCUs ? kMid128 : kMid64;
 }
+// (1000 x 250 x 256: 38 us by 16 rows against 43; 4096 x 256 x 128: 54 against 48)
+LogitTile whole_tile(int64_t n) { return n <= 1024 ? kLow16 : kLow64; }
 
 // Tile and K splits of the two gradient products of a piece.  A split takes whole multiples of 64 values of K, so a product of
 // K values has at most K / 64 of them; dW is not split when the classes come in several pieces (its rows are then plenty).
@@ -699,11 +769,12 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.grad_tile = kT64;
   L.dx_splits = L.dw_splits = 1;
   if (h.dx || h.dweight) pick_grad(n, cp, h.dim, np, h.dx != nullptr, h.dweight != nullptr, L.pieces == 1, L);
-  L.dw_direct = L.dw_splits == 1;
-  L.tile_s = logit_tile(n, h.n_classes);
-  L.tile_g = logit_tile(n, cp);
-  L.db_rows = L.tile_g == kBig256 ? (int)ceil_div(n, 256) * 2 : L.tile_g == kMid128 ? (int)ceil_div(n, 128) * 2 : 1;
-  L.row_blocks = (int)ceil_div(n, 16);
+  L.whole = h.n_classes <= 256;
+  L.dw_direct = L.dw_splits == 1 && !L.whole;  // (in one sweep the unit of G is not known before the gradients' launch ends)
+  L.tile_s = L.whole ? whole_tile(n) : logit_tile(n, h.n_classes);
+  L.tile_g = L.whole ? L.tile_s : logit_tile(n, cp);
+  L.db_rows = (int)ceil_div(n, kLogitM[L.tile_g]) * kLogitWM[L.tile_g];
+  L.row_blocks = (int)ceil_div(n, L.whole ? kLogitM[L.tile_s] : 16);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
   L.scal = take(sizeof(Scalars));
@@ -760,30 +831,37 @@ int launch_logits(const LogitArgs& a, int tile, hipStream_t s) {
   switch (tile) {
     case kLow16: return launch_logits_tile<Tile<TYPE, NP, false, false, 16, 256, 1, 4>, SWEEP>(a, s);
     case kLow64: return launch_logits_tile<Tile<TYPE, NP, false, false, 64, 256, 1, 4>, SWEEP>(a, s);
+    case kMid64: return launch_logits_tile<Tile<TYPE, NP, false, false, 64, 128, 2, 2>, SWEEP>(a, s);
     case kMid128: return launch_logits_tile<Tile<TYPE, NP, false, false, 128, 128, 2, 2>, SWEEP>(a, s);
     default: return launch_logits_tile<Tile<TYPE, NP, false, false, 256, 256, 2, 4>, SWEEP>(a, s);
   }
 }
 
+template <int TYPE, int NP>
+int launch_whole(const LogitArgs& a, int tile, hipStream_t s) {
+  return tile == kLow16 ? launch_logits_tile<Tile<TYPE, NP, false, false, 16, 256, 1, 4>, 2>(a, s)
+                        : launch_logits_tile<Tile<TYPE, NP, false, false, 64, 256, 1, 4>, 2>(a, s);
+}
+
 template <int TYPE, int NP, int BM, int BN, int WM, int WN>
-int launch_grads_tile(GradArgs dx, GradArgs dw, hipStream_t s) {
+int launch_grads_tile(GradArgs dx, GradArgs dw, int totals, TotalArgs total, hipStream_t s) {
   typedef Tile<TYPE, NP, false, true, BM, BN, WM, WN> X;
   typedef Tile<TYPE, NP, true, true, BM, BN, WM, WN> W;
   dx.group = dw.group = 8;
   int dx_blocks = (int)(ceil_div(dx.M, BM) * ceil_div(dx.N, BN) * dx.splits);  // (M = 0: not wanted)
-  const int blocks = dx_blocks + (int)(ceil_div(dw.M, BM) * ceil_div(dw.N, BN) * dw.splits);
-  void* args[] = {&dx, &dw, &dx_blocks};
+  const int blocks = dx_blocks + (int)(ceil_div(dw.M, BM) * ceil_div(dw.N, BN) * dw.splits) + totals;
+  void* args[] = {&dx, &dw, &dx_blocks, &totals, &total};
   static std::atomic<uint64_t> done{0};
   return launch_tile(reinterpret_cast<const void*>(k_lce_grads<X, W>), blocks, X::kThreads, X::kLds, args, done, s);
 }
 template <int TYPE, int NP>
-int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, hipStream_t s) {
+int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, int totals, const TotalArgs& total, hipStream_t s) {
   switch (tile) {
-    case kT64: return launch_grads_tile<TYPE, NP, 64, 64, 2, 2>(dx, dw, s);
-    case kT96: return launch_grads_tile<TYPE, NP, 96, 96, 2, 2>(dx, dw, s);
-    case kT64x128: return launch_grads_tile<TYPE, NP, 64, 128, 2, 2>(dx, dw, s);
-    case kT128: return launch_grads_tile<TYPE, NP, 128, 128, 2, 2>(dx, dw, s);
-    default: return launch_grads_tile<TYPE, NP, 256, 256, 2, 4>(dx, dw, s);
+    case kT64: return launch_grads_tile<TYPE, NP, 64, 64, 2, 2>(dx, dw, totals, total, s);
+    case kT96: return launch_grads_tile<TYPE, NP, 96, 96, 2, 2>(dx, dw, totals, total, s);
+    case kT64x128: return launch_grads_tile<TYPE, NP, 64, 128, 2, 2>(dx, dw, totals, total, s);
+    case kT128: return launch_grads_tile<TYPE, NP, 128, 128, 2, 2>(dx, dw, totals, total, s);
+    default: return launch_grads_tile<TYPE, NP, 256, 256, 2, 4>(dx, dw, totals, total, s);
   }
 }
 
@@ -821,34 +899,42 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   a.strips = reinterpret_cast<float2*>(ws + L.strips);
   a.target_logit = reinterpret_cast<float*>(ws + L.target);
   a.row = reinterpret_cast<const float2*>(ws + L.row);
-  if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
 
-  RowArgs r{};
+  RowArgs& r = a.rows;
   r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
   r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
-  r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part);
-  r.scal = scal;
-  hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
-  SUAVE_CHECK_HIP(hipGetLastError());
+  r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part); r.scal = scal;
   a.total = TotalArgs{r.part, L.row_blocks, h.weight_sum, h.loss_scale, h.loss_rows, g_scale(F), h.loss, h.loss_sum, scal};
-  if (!grad) {
+  a.db_ld = L.C_pad;
+  a.ldg = L.ldg; a.g_plane = L.g_plane;
+  if (grad) {
+    a.g = ws + L.g;
+    a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
+  }
+  const bool products = h.dx || h.dweight;
+  if (L.whole) {
+    if (int rc = launch_whole<TYPE, NP>(a, L.tile_s, s)) return rc;
+  } else {
+    if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
+    SUAVE_CHECK_HIP(hipGetLastError());
+  }
+  if (!grad || (L.whole && !products)) {
     hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(256), 0, s, a.total);
     SUAVE_CHECK_HIP(hipGetLastError());
-    return 0;
+    if (!grad) return 0;
   }
 
   const bool bf = !F;
   auto vec_ok = [&](const void* ptr, int64_t ld) {
     return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) & (bf ? 7 : 15)) == 0;
   };
-  a.g = ws + L.g; a.ldg = L.ldg; a.g_plane = L.g_plane;
-  a.db_ld = L.C_pad;
   for (int piece = 0; piece < L.pieces; ++piece) {
     a.c0 = piece * L.piece;
     a.c1 = std::min(a.c0 + L.piece, (int)h.n_classes);
-    a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
     a.totals = piece == 0;
-    if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
+    if (!L.whole)
+      if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
     const int cp = a.c1 - a.c0;
     GradArgs gx{}, gw{};
     if (h.dx) {
@@ -871,8 +957,8 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
       g.out_bf16 = bf; g.out_vec = vec_ok(h.dweight, h.ld_dweight);
       g.scal = scal; g.which = 1;
     }
-    if (h.dx || h.dweight)
-      if (int rc = launch_grads<TYPE, NP>(gx, gw, L.grad_tile, s)) return rc;
+    if (products)
+      if (int rc = launch_grads<TYPE, NP>(gx, gw, L.grad_tile, L.whole, a.total, s)) return rc;
   }
   FinishArgs f{};
   f.scal = scal; f.out_bf16 = bf; f.ld_slab = L.Dp; f.N = h.dim; f.gs = g_scale(F);
