@@ -367,7 +367,8 @@ __device__ __forceinline__ void write_gradients(const LogitArgs& a, const typena
   }
 }
 
-// One tile of logits; SWEEP 0: strip statistics, 1: G, 2: both, for tiles that hold whole rows (few classes: no second product and two
+// One tile of logits; SWEEP 0: strip statistics, 1: G, 3: statistics and the exponentials they are made of, for k_lce_scale; 2: statistics
+// and G, for tiles that hold whole rows (few classes: no second product and two
 // launches less; 1000 x 250 x 256 f32: 38 us against 53 in two sweeps).  What the epilogue needs of bias, targets and rows is asked for before the
 // product, one value per thread, and spread through LDS behind it: the matrix pipe covers the latency.
 template <class T, int SWEEP>
@@ -452,9 +453,29 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
 #pragma unroll
       for (int j = 0; j < T::NI; ++j)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s += __expf(v[j][u] - base);
+        for (int u = 0; u < 4; ++u) {
+          v[j][u] = __expf(v[j][u] - base);
+          s += v[j][u];
+        }
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
+      if constexpr (SWEEP == 3) {
+        typedef RowStage<uint16_t, kStrip> Rows;
+        char* stage = lds + kTabs + wave * (2 * Rows::kBytes);
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j) {
+          uint16_t hi[4], lo[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) planes(v[j][u] * g_scale(true), hi[u], lo[u]);
+          Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
+          Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
+        }
+        const int64_t m0 = m_base + wm * (T::MI * 16) + 16 * i;
+        const int rows = (int)max<int64_t>(0, min<int64_t>(16, a.n - m0));
+        char* out = a.g + m0 * a.ldg + (int64_t)cw * 2;
+        Rows::flush(stage, out, a.ldg, rows, kStrip, lane);
+        Rows::flush(stage + Rows::kBytes, out + a.g_plane, a.ldg, rows, kStrip, lane);
+      }
       if (SWEEP == 2) {
         if (g == 0) strip_tab[wn * T::BM + ml] = make_float2(base, s);
       } else {
@@ -494,9 +515,94 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
     if (a.g == nullptr) return;
     __syncthreads();
   }
-  if constexpr (SWEEP != 0) {
+  if constexpr (SWEEP == 1 || SWEEP == 2) {
     write_gradients<T>(a, acc, bias, unit, tm, cw, row_tab, target_tab, lds + kTabs);
   }
+}
+
+struct ScaleArgs {
+  char* g; int64_t ldg; uint32_t g_plane;
+  int64_t n;
+  int n_strips, groups;            // groups: of 256 classes
+  const float2* strips;
+  const float2* row;
+  const float* target_logit;
+  const int32_t* targets;
+  float* db; int64_t db_ld;        // [ceil(n / kScaleRows)][db_ld], or null
+  TotalArgs total;
+};
+constexpr int kScaleRows = 32;
+
+// G from the exponentials of a sweep that kept them, in place: exp(l - strip's max) exp(strip's max - lse) instead of a second product.
+// A block takes 32 rows x 256 classes, a thread eight neighbouring classes of every eighth row.  Only for planes, whose rounding
+// (2^-22) may be made twice, and where all the classes are one piece.  Bound by the memory-side cache: 1777 x 20011 50 us for 285 MB,
+// against 177 us for the second sweep at 501 columns (and 34 more in the first one for the writing).  The first block finishes the loss.
+__global__ __launch_bounds__(256) void k_lce_scale(ScaleArgs a) {
+  __shared__ double tot[8];
+  __shared__ float sums[8][256];
+  if (blockIdx.x == 0) {
+    total_loss(a.total, *reinterpret_cast<double(*)[4]>(tot), *reinterpret_cast<double(*)[4]>(tot + 4));
+    return;
+  }
+  const int b = blockIdx.x - 1;
+  const int64_t rb = b / a.groups;
+  const int cl = threadIdx.x & 31, rr = threadIdx.x >> 5;
+  const int c = (b - (int)rb * a.groups) * 256 + cl * 8, strip = c / kStrip;
+  float cs[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) cs[u] = 0.f;
+  constexpr int U = 4;
+#pragma unroll
+  for (int h = 0; h < kScaleRows / 8 / U; ++h) {
+    uint4 hi[U], lo[U];
+    float2 st[U], rw[U];
+    int y[U];
+    float tl[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t m = rb * kScaleRows + (h * U + u) * 8 + rr;
+      const bool in = m < a.n;
+      const char* p = a.g + (in ? m : 0) * a.ldg + (int64_t)c * 2;
+      hi[u] = *reinterpret_cast<const uint4*>(p);
+      lo[u] = *reinterpret_cast<const uint4*>(p + a.g_plane);
+      st[u] = in && strip < a.n_strips ? a.strips[(int64_t)strip * a.n + m] : make_float2(0.f, 0.f);
+      rw[u] = in ? a.row[m] : make_float2(0.f, 0.f);
+      y[u] = in ? a.targets[m] : -1;
+      tl[u] = in ? a.target_logit[m] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t m = rb * kScaleRows + (h * U + u) * 8 + rr;
+      if (m >= a.n) continue;
+      // (a strip without any class, or with all its logits -inf, holds zeros; without any logit in the row the result is NaN)
+      const bool none = strip >= a.n_strips || (st[u].y == 0.f && rw[u].x > -INFINITY);
+      const float f = none || rw[u].y == 0.f ? 0.f : __expf(st[u].x - rw[u].x) * rw[u].y;
+      const bool zero = none || rw[u].y == 0.f;  // a row without weight contributes nothing, whatever it holds
+      const int at = y[u] - c;
+      const uint16_t* ph = reinterpret_cast<const uint16_t*>(&hi[u]);
+      const uint16_t* pl = reinterpret_cast<const uint16_t*>(&lo[u]);
+      uint16_t oh[8], ol[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v = ((float)__builtin_bit_cast(_Float16, ph[i]) + (float)__builtin_bit_cast(_Float16, pl[i])) * f;
+        if (i == at) v = (__expf(tl[u] - rw[u].x) - 1.0f) * (rw[u].y * g_scale(true));
+        if (zero) v = i == at && rw[u].y != 0.f ? v : 0.f;
+        cs[i] += v;
+        planes(v, oh[i], ol[i]);
+      }
+      char* p = a.g + m * a.ldg + (int64_t)c * 2;
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(oh);
+      *reinterpret_cast<uint4*>(p + a.g_plane) = *reinterpret_cast<const uint4*>(ol);
+    }
+  }
+  if (a.db == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[rr][cl * 8 + i] = cs[i];
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
+  a.db[rb * a.db_ld + (c - cl * 8) + threadIdx.x] = s * (1.0f / g_scale(true));
 }
 
 // lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights.  The sums over all blocks are
@@ -702,6 +808,7 @@ struct Layout {  // offsets into the workspace, bytes
   TileId grad_tile;
   int row_blocks, db_rows;
   bool whole;            // one sweep: a tile holds whole rows
+  bool keep;             // one sweep: the exponentials stay in G's scratch until lse is known
   int tile_s, tile_g;    // LogitTile of the two sweeps (one per call: the db partials of all pieces have the same rows)
 };
 
@@ -773,7 +880,10 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.dw_direct = L.dw_splits == 1 && !L.whole;  // (in one sweep the unit of G is not known before the gradients' launch ends)
   L.tile_s = L.whole ? whole_tile(n) : logit_tile(n, h.n_classes);
   L.tile_g = L.whole ? L.tile_s : logit_tile(n, cp);
-  L.db_rows = (int)ceil_div(n, kLogitM[L.tile_g]) * kLogitWM[L.tile_g];
+  // (pays where the second product costs more than the pass over G: 1777 x 20011 x 501: 493 us against 576, 4096 x 1000 x 256: 82 against
+  // 81, 4096 x 1000 x 16: 64 against 57)
+  L.keep = f32 && grad && L.pieces == 1 && !L.whole && h.dim >= 256;
+  L.db_rows = L.keep ? (int)ceil_div(n, kScaleRows) : (int)ceil_div(n, kLogitM[L.tile_g]) * kLogitWM[L.tile_g];
   L.row_blocks = (int)ceil_div(n, L.whole ? kLogitM[L.tile_s] : 16);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
@@ -915,7 +1025,11 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   if (L.whole) {
     if (int rc = launch_whole<TYPE, NP>(a, L.tile_s, s)) return rc;
   } else {
-    if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    if constexpr (F) {
+      if (int rc = L.keep ? launch_logits<TYPE, NP, 3>(a, L.tile_s, s) : launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    } else {
+      if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    }
     hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
     SUAVE_CHECK_HIP(hipGetLastError());
   }
@@ -923,6 +1037,12 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(256), 0, s, a.total);
     SUAVE_CHECK_HIP(hipGetLastError());
     if (!grad) return 0;
+  }
+
+  if (L.keep) {
+    const ScaleArgs k{a.g, L.ldg, L.g_plane, n, L.n_strips, L.C_pad / 256, a.strips, a.row, a.target_logit, h.targets, a.db, a.db_ld, a.total};
+    hipLaunchKernelGGL(k_lce_scale, dim3((unsigned)(1 + ceil_div(n, kScaleRows) * k.groups)), dim3(256), 0, s, k);
+    SUAVE_CHECK_HIP(hipGetLastError());
   }
 
   const bool bf = !F;
@@ -933,7 +1053,7 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     a.c0 = piece * L.piece;
     a.c1 = std::min(a.c0 + L.piece, (int)h.n_classes);
     a.totals = piece == 0;
-    if (!L.whole)
+    if (!L.whole && !L.keep)
       if (int rc = launch_logits<TYPE, NP, 1>(a, L.tile_g, s)) return rc;
     const int cp = a.c1 - a.c0;
     GradArgs gx{}, gw{};
