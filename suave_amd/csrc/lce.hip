@@ -61,19 +61,6 @@ struct PackArgs {
   int C, C_pad;
 };
 
-// Eight neighbours in 16-byte loads, wherever the row begins (the memory system takes them at element alignment)
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const f32x4_any a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-}
-__device__ __forceinline__ void load8(const uint16_t* p, uint16_t (&v)[8]) {
-  const u16x8_any a = *reinterpret_cast<const u16x8_any*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = a[i];
-}
 __device__ __forceinline__ int64_t row_of(int64_t chunk, int64_t chunks, int q) {  // 32-bit division where it reaches
   return chunks <= 0xffffffffll ? (int64_t)((uint32_t)chunk / (uint32_t)q) : chunk / q;
 }

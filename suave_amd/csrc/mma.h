@@ -304,76 +304,85 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // For products of few tiles, whose time is the chain of K steps: the block has `groups` times the waves of a tile, group g takes the
-  // steps [g per, (g + 1) per) of K in LDS of its own (kLds bytes each, at lds), and the partial sums meet in LDS.  Every group walks
-  // `per` steps, those past K as zeros, so all waves pass the same barriers.  On return acc holds the whole sums of this
-  // group's share of the fragments: those with (MI j + i) % groups == g.
-  template <int GROUPS>
+  // For products of few tiles, whose time is the chain of K steps: K is cut into GROUPS x PARTS ranges of `per` steps, the block has
+  // GROUPS times the waves of a tile, and group g takes PARTS neighbouring ranges, one after the other, in LDS of its own (kLds bytes
+  // each, at lds); the partial sums meet in LDS.  Every group walks `per` steps of a range, those past K as zeros, so all waves
+  // pass the same barriers.  On return acc holds the whole sums of this group's share of the fragments: those with
+  // (MI j + i) % GROUPS == g.  The ranges are added in their order, so the result depends on GROUPS x PARTS only.
+  template <int GROUPS, int PARTS>
   static __device__ __forceinline__ void run_split(char* lds, Operand A, Operand B, int K, acc_t (&acc)[MI][NI]) {
     const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = all / (WM * WN), wave = all % (WM * WN);
     const int wm = wave / WN, wn = wave % WN;
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
-    const int steps = (K + kStepK - 1) / kStepK, per = (steps + GROUPS - 1) / GROUPS, first = group * per;
+    const int steps = (K + kStepK - 1) / kStepK, per = (steps + GROUPS * PARTS - 1) / (GROUPS * PARTS);
     char* mine = lds + group * kLds;
-    const char* pa = uniform_ptr(A.base + SA::advance(A) * first);
-    const char* pb = uniform_ptr(B.base + SB::advance(B) * first);
-    uint32_t oa[SA::kPer], ob[SB::kPer];
-    auto load = [&](int s) {
-      planes_load(pa + SA::advance(A) * s, pb + SB::advance(B) * s, mine + (s & 1) * kStepBytes, wave, oa, ob);
-    };
-    offsets(A, B, wave, lane, K - first * kStepK, oa, ob);
-    load(0);
-    // steps that lie inside K for every group come first: their transfers need no masks and are spread between the products
-    const int whole = min(per, max(0, K / kStepK - (GROUPS - 1) * per));
-    int s = 0;
-    if (whole > 1) offsets(A, B, wave, lane, kStepK, oa, ob);
-    for (; s + 1 < whole; ++s) {
-      turn();
-      if constexpr (NP == 2) {
-        planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, acc);
-        load(s + 1);
-        planes_order();
-      } else {
-        both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, acc, [&] { load(s + 1); });
-      }
-    }
-    for (; s < per; ++s) {
-      turn();
-      auto next = [&] {
-        if (s + 1 < per) {
-          offsets(A, B, wave, lane, K - (first + s + 1) * kStepK, oa, ob);
-          load(s + 1);
-        }
+    acc_t sum[PARTS][MI][NI];
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) sum[part][i][j] = acc_t{0, 0, 0, 0};
+      const int first = (group * PARTS + part) * per;
+      const char* pa = uniform_ptr(A.base + SA::advance(A) * first);
+      const char* pb = uniform_ptr(B.base + SB::advance(B) * first);
+      uint32_t oa[SA::kPer], ob[SB::kPer];
+      auto load = [&](int s) {
+        planes_load(pa + SA::advance(A) * s, pb + SB::advance(B) * s, mine + (s & 1) * kStepBytes, wave, oa, ob);
       };
-      if constexpr (NP == 2) {
-        planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, acc);
-        next();
-      } else {
-        both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, acc, next);
+      if (part > 0) turn();  // the last step of the range before is read
+      offsets(A, B, wave, lane, K - first * kStepK, oa, ob);
+      load(0);
+      // steps that lie inside K for every group come first: their transfers need no masks and are spread between the products
+      const int whole = min(per, max(0, K / kStepK - ((GROUPS - 1) * PARTS + part) * per));
+      int s = 0;
+      if (whole > 1) offsets(A, B, wave, lane, kStepK, oa, ob);
+      for (; s + 1 < whole; ++s) {
+        turn();
+        if constexpr (NP == 2) {
+          planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, sum[part]);
+          load(s + 1);
+          planes_order();
+        } else {
+          both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, sum[part], [&] { load(s + 1); });
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      for (; s < per; ++s) {
+        turn();
+        auto next = [&] {
+          if (s + 1 < per) {
+            offsets(A, B, wave, lane, K - (first + s + 1) * kStepK, oa, ob);
+            load(s + 1);
+          }
+        };
+        if constexpr (NP == 2) {
+          planes_step(mine + (s & 1) * kStepBytes, wm, wn, lane, sum[part]);
+          next();
+        } else {
+          both_halves(mine + (s & 1) * kStepBytes, wm, wn, lane, sum[part], next);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     turn();
-    acc_t* sums = reinterpret_cast<acc_t*>(lds);  // [group][wave][fragment][lane]
-    static_assert(WM * WN * MI * NI * 64 * 16 <= kLds, "the partial sums fit the groups' slots");
+    acc_t* sums = reinterpret_cast<acc_t*>(lds);  // [range][wave][fragment][lane]
+    static_assert(WM * WN * MI * NI * 64 * 16 * PARTS <= kLds, "the partial sums fit the groups' slots");
+    auto at = [&](int range, int i, int j) { return ((range * WM * WN + wave) * MI * NI + MI * j + i) * 64 + lane; };
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sums[((group * WM * WN + wave) * MI * NI + MI * j + i) * 64 + lane] = acc[i][j];
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) sums[at(group * PARTS + part, i, j)] = sum[part][i][j];
     turn();
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
+        acc[i][j] = acc_t{0, 0, 0, 0};
         if ((MI * j + i) % GROUPS != group) continue;
-        acc_t t = acc_t{0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) t += sums[((g * WM * WN + wave) * MI * NI + MI * j + i) * 64 + lane];
-        acc[i][j] = t;
+        for (int r = 0; r < GROUPS * PARTS; ++r) acc[i][j] += sums[at(r, i, j)];
       }
   }
 
@@ -470,6 +479,20 @@ __device__ __forceinline__ void tile_of(int b, int n_blocks, int tiles_m, int ti
   const int gm = min(group, tiles_m - g * group);
   tm = g * group + rem % gm;
   tn = rem / gm;
+}
+
+// Eight neighbours in 16-byte loads, wherever the row begins (the memory system takes them at element alignment)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const f32x4_any a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+__device__ __forceinline__ void load8(const uint16_t* p, uint16_t (&v)[8]) {
+  const u16x8_any a = *reinterpret_cast<const u16x8_any*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = a[i];
 }
 
 __device__ __forceinline__ uint16_t bf16_bits(float x) {

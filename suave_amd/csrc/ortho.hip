@@ -79,46 +79,90 @@ __host__ __device__ inline int norm_blocks(int rows, int cols) {
   return b < kNormBlocks ? (int)b : kNormBlocks;
 }
 
-// Partial sums of squares (double: neither overflow nor loss over 2^24 values); muon: the momentum first.  A block owns whole
-// rows where they are long, otherwise runs of the flat index (below 2^31 then); eight loads in flight per thread.
+// Eight neighbours of U's row r from column c0 (zeros past the row); muon: from the gradient and this step's momentum
+__device__ __forceinline__ void in_values(const Group& g, const Mat& m, int64_t r, int c0, float (&v)[8]) {
+  if (c0 + 8 <= m.cols) {
+    if (g.bf16) {
+      uint16_t w[8];
+      load8(static_cast<const uint16_t*>(m.in) + r * m.ld_in + c0, w);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = bf16_value(w[u]);
+      return;
+    }
+    load8(static_cast<const float*>(m.in) + r * m.ld_in + c0, v);
+    if (g.muon) {
+      float mom[8];
+      load8(m.mom + r * m.ld_mom + c0, mom);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = g.nesterov ? fmaf(g.momentum, mom[u], v[u]) : mom[u];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = c0 + u < m.cols ? in_value(g, m, r, c0 + u) : 0.f;
+  }
+}
+
+// Partial sums of squares (double: neither overflow nor loss over 2^24 values); muon: the momentum first.  Chunks of eight
+// neighbours, two in flight per thread.
 __global__ __launch_bounds__(256) void k_ortho_norm(Group g) {
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
+  const int q = (m.cols + 7) / 8;
+  const int64_t chunks = (int64_t)m.rows * q, step = (int64_t)nb * 256;
   double s = 0.0;
-  auto eight = [&](int64_t e0, int64_t step, int64_t end, auto place) {
-    float v[8], mo[8];
-    int64_t r[8];
-    int c[8];
+  for (int64_t e0 = (int64_t)b * 256 + threadIdx.x; e0 < chunks; e0 += 2 * step) {
+    float v[2][8], mom[2][8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int64_t e = e0 + u * step;
-      v[u] = mo[u] = 0.f;
-      if (e < end) {
-        place(e, r[u], c[u]);
-        v[u] = g.bf16 ? bf16_value(static_cast<const uint16_t*>(m.in)[r[u] * m.ld_in + c[u]]) : static_cast<const float*>(m.in)[r[u] * m.ld_in + c[u]];
-        if (g.muon) mo[u] = m.mom[r[u] * m.ld_mom + c[u]];
+    for (int h = 0; h < 2; ++h) {
+      const int64_t e = e0 + h * step;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[h][u] = mom[h][u] = 0.f;
+      if (e >= chunks) continue;
+      const int64_t r = chunks < (1ll << 31) ? (int64_t)((uint32_t)e / (uint32_t)q) : e / q;
+      const int c0 = (int)(e - r * q) * 8;
+      if (!g.muon) {
+        in_values(g, m, r, c0, v[h]);
+      } else {
+        const float* gr = static_cast<const float*>(m.in) + r * m.ld_in + c0;
+        const float* mo = m.mom + r * m.ld_mom + c0;
+        if (c0 + 8 <= m.cols) {
+          load8(gr, v[h]);
+          load8(mo, mom[h]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c0 + u < m.cols) { v[h][u] = gr[u]; mom[h][u] = mo[u]; }
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (e0 + u * step >= end) continue;
+    for (int h = 0; h < 2; ++h) {
+      const int64_t e = e0 + h * step;
+      if (e >= chunks) continue;
       if (g.muon) {
-        const float mn = fmaf(g.momentum, mo[u], v[u]);
-        m.mom[r[u] * m.ld_mom + c[u]] = mn;
-        v[u] = g.nesterov ? fmaf(g.momentum, mn, v[u]) : mn;
+        const int64_t r = chunks < (1ll << 31) ? (int64_t)((uint32_t)e / (uint32_t)q) : e / q;
+        const int c0 = (int)(e - r * q) * 8;
+        float* mo = m.mom + r * m.ld_mom + c0;
+        f32x4_any w[2];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float mn = fmaf(g.momentum, mom[h][u], v[h][u]);
+          w[u / 4][u % 4] = mn;
+          v[h][u] = g.nesterov ? fmaf(g.momentum, mn, v[h][u]) : mn;
+        }
+        if (c0 + 8 <= m.cols) {
+          *reinterpret_cast<f32x4_any*>(mo) = w[0];
+          *reinterpret_cast<f32x4_any*>(mo + 4) = w[1];
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c0 + u < m.cols) mo[u] = w[u / 4][u % 4];
+        }
       }
-      s += (double)v[u] * (double)v[u];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += (double)v[h][u] * (double)v[h][u];
     }
-  };
-  if (m.cols >= 2048) {
-    for (int64_t r = b; r < m.rows; r += nb)
-      for (int c0 = threadIdx.x; c0 < m.cols; c0 += 2048)
-        eight(c0, 256, m.cols, [&](int64_t e, int64_t& rr, int& cc) { rr = r; cc = (int)e; });
-  } else {
-    const int64_t total = (int64_t)m.rows * m.cols, step = (int64_t)nb * 256;
-    for (int64_t e0 = (int64_t)b * 256 + threadIdx.x; e0 < total; e0 += 8 * step)
-      eight(e0, step, total, [&](int64_t e, int64_t& rr, int& cc) { rr = (int)e / m.cols; cc = (int)e - (int)rr * m.cols; });
   }
   __shared__ double part[4];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -151,21 +195,42 @@ __device__ __forceinline__ void write_result(const Group& g, const Mat& m, int r
   }
 }
 
+// four neighbours, as one access each way
+__device__ __forceinline__ void write_results(const Group& g, const Mat& m, int r, int c, const float (&v)[4]) {
+  if (c + 4 > m.cols) {
+    for (int u = 0; c + u < m.cols; ++u) write_result(g, m, r, c + u, v[u]);
+  } else if (g.bf16) {
+    typedef uint16_t u16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+    *reinterpret_cast<u16x4_any*>(static_cast<uint16_t*>(m.out) + (int64_t)r * m.ld_out + c) = u16x4_any{bf16_bits(v[0]), bf16_bits(v[1]), bf16_bits(v[2]), bf16_bits(v[3])};
+  } else {
+    f32x4_any* o = reinterpret_cast<f32x4_any*>(static_cast<float*>(m.out) + (int64_t)r * m.ld_out + c);
+    f32x4_any w = f32x4_any{v[0], v[1], v[2], v[3]};
+    if (g.muon) {
+      const f32x4_any p = *o;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[u] = fmaf(-m.lr, v[u], p[u] * m.decay);
+    }
+    *o = w;
+  }
+}
+
 // X_0 in planes, pads zero; the sizes of X_0 .. X_steps
 template <int NP>
 __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
-  __shared__ double sc;
-  if (threadIdx.x < 64) {
+  __shared__ double sc, part[4];
+  {
     double s = 0.0;
     const int n = norm_blocks(m.rows, m.cols);
-    for (int k = threadIdx.x; k < n; k += 64) s += g.part[m.id * kNormBlocks + k];
+    for (int k = threadIdx.x; k < n; k += 256) s += g.part[m.id * kNormBlocks + k];
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
     if (threadIdx.x == 0) {
       int e[kMaxSteps + 1];
-      sc = start_scale(s, g.eps, g.steps, e);
+      sc = start_scale((part[0] + part[1]) + (part[2] + part[3]), g.eps, b == 0 ? g.steps : 0, e);
       if (b == 0)
         for (int k = 0; k <= g.steps; ++k) g.exps[m.id * (kMaxSteps + 1) + k] = e[k];
     }
@@ -175,27 +240,12 @@ __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
   const int cp = (m.cols + 7) / 8 * 8, q = cp / 8;
   const int64_t chunks = (int64_t)m.rows * q;
   const int pit = pitch(m.cols, NP);
-  // (rows that start at multiples of 16 bytes are read in such pieces)
-  const bool vec = !g.muon && (m.ld_in * (g.bf16 ? 2 : 4)) % 16 == 0 && (reinterpret_cast<uintptr_t>(m.in) & 15) == 0;
   for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
-    const int64_t r = chunks < (1 << 30) ? (int)e / q : e / q;
+    const int64_t r = chunks < (1ll << 31) ? (int64_t)((uint32_t)e / (uint32_t)q) : e / q;
     const int c0 = (int)(e - r * q) * 8;
     uint16_t hi[8], lo[8];
     float in[8];
-    if (vec && c0 + 8 <= m.cols) {
-      if (g.bf16) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(m.in) + r * m.ld_in + c0);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) in[u] = bf16_value(reinterpret_cast<const uint16_t*>(&w)[u]);
-      } else {
-        const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(m.in) + r * m.ld_in + c0);
-        *reinterpret_cast<float4*>(in) = w[0];
-        *reinterpret_cast<float4*>(in + 4) = w[1];
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) in[u] = c0 + u < m.cols ? in_value(g, m, r, c0 + u) : 0.f;
-    }
+    in_values(g, m, r, c0, in);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const float v = c0 + u < m.cols ? (float)((double)in[u] * scale) : 0.f;
@@ -240,9 +290,9 @@ __device__ __forceinline__ void store_mirror(char* base, int pit, int cols, int 
   }
 }
 
-template <class T, int GROUPS>
+template <class T, int GROUPS, int PARTS>
 __device__ __forceinline__ void run_tile(char* lds, const Operand& A, const Operand& B, int K, typename T::acc_t (&acc)[T::MI][T::NI]) {
-  if constexpr (GROUPS > 1) T::template run_split<GROUPS>(lds, A, B, K, acc);
+  if constexpr (GROUPS > 1) T::template run_split<GROUPS, PARTS>(lds, A, B, K, acc);
   else T::run(lds, A, B, K, acc);
 }
 
@@ -254,7 +304,7 @@ __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
 }
 
 // POLY 0: A from X; 1: B from A
-template <int NP, int BM, int WM, int WN, int POLY, int GROUPS>
+template <int NP, int BM, int WM, int WN, int POLY, int GROUPS, int PARTS>
 __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_sym(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> R;
@@ -269,15 +319,15 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
   f32x4 acc[R::MI][R::NI];
   if (POLY) {
     const uint32_t plane = (s + 7) / 8 * 16;
-    run_tile<R, GROUPS>(lds, Operand{m.a + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane}, Operand{m.a + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane}, s, acc);
+    run_tile<R, GROUPS, PARTS>(lds, Operand{m.a + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane}, Operand{m.a + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane}, s, acc);
   } else {
     const int px = pitch(m.cols, NP);
     const uint32_t plane = (m.cols + 7) / 8 * 16;
     const char* x = m.x[g.k & 1];
     if (m.rows <= m.cols)
-      run_tile<R, GROUPS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, s - m0, plane}, Operand{x + (int64_t)n0 * px, (uint32_t)px, s - n0, plane}, m.cols, acc);
+      run_tile<R, GROUPS, PARTS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, s - m0, plane}, Operand{x + (int64_t)n0 * px, (uint32_t)px, s - n0, plane}, m.cols, acc);
     else
-      run_tile<C, GROUPS>(lds, Operand{x + m0 * 2, (uint32_t)px, (s - m0 + 7) / 8 * 16, plane}, Operand{x + n0 * 2, (uint32_t)px, (s - n0 + 7) / 8 * 16, plane}, m.rows, acc);
+      run_tile<C, GROUPS, PARTS>(lds, Operand{x + m0 * 2, (uint32_t)px, (s - m0 + 7) / 8 * 16, plane}, Operand{x + n0 * 2, (uint32_t)px, (s - n0 + 7) / 8 * 16, plane}, m.rows, acc);
   }
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
@@ -335,9 +385,9 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
   const char* x = m.x[g.k & 1];
   f32x4 acc[W::MI][W::NI];
   if (m.rows <= m.cols)
-    run_tile<W, GROUPS>(lds, Operand{m.b + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane_s}, Operand{x + (int64_t)n0 * 2, (uint32_t)px, (m.cols - n0 + 7) / 8 * 16, plane_x}, s, acc);
+    run_tile<W, GROUPS, 1>(lds, Operand{m.b + (int64_t)m0 * ps, (uint32_t)ps, s - m0, plane_s}, Operand{x + (int64_t)n0 * 2, (uint32_t)px, (m.cols - n0 + 7) / 8 * 16, plane_x}, s, acc);
   else
-    run_tile<H, GROUPS>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
+    run_tile<H, GROUPS, 1>(lds, Operand{x + (int64_t)m0 * px, (uint32_t)px, m.rows - m0, plane_x}, Operand{m.b + (int64_t)n0 * ps, (uint32_t)ps, s - n0, plane_s}, s, acc);
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % (WM * WN), group = (threadIdx.x >> 6) / (WM * WN);
   const int wm = wave / WN, wn = wave % WN;
   const int e = g.exps[m.id * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[m.id * (kMaxSteps + 1) + g.k + 1];
@@ -358,8 +408,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
       if constexpr (!LAST) {
         store_planes<NP>(m.x[(g.k & 1) ^ 1], px, m.cols, r, n, v);
       } else {
-        for (int u = 0; u < 4; ++u)
-          if (n + u < m.cols) write_result(g, m, r, n + u, v[u]);
+        write_results(g, m, r, n, v);
       }
     }
   }
@@ -369,7 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
 // A matrix whose planes fit a CU's LDS goes through the whole iteration in one launch: X (short side s in rows) and one s x s
 // buffer that holds A and then B stay in LDS, fp32 accumulators in registers.  What bounds it is the chain of barriers and LDS
 // reads, a few microseconds per step, instead of three launches per step; column strips of X are independent in X <- B X, so a
-// wave replaces its strips in place.  64 x 64 f32: SMALL_US us against SMALL_OLD us by launches.
+// wave replaces its strips in place.  64 x 64 f32: 23 us against 73 us by launches.
 constexpr int kSmallWaves = 8;
 constexpr int kSmallLds = 156 * 1024;
 
@@ -738,10 +787,10 @@ int set_begin(Group& g, F blocks) {
   return (int)b;
 }
 
-template <int NP, int POLY, int BM, int WM, int WN, int GROUPS>
+template <int NP, int POLY, int BM, int WM, int WN, int GROUPS, int PARTS = 1>
 int launch_sym_tile(Group& g, hipStream_t s) {
   const int grid = set_begin(g, [](const Mat& m) { return tiles_of(m, kGram, BM, BM); });
-  return launch<k_ortho_sym<NP, BM, WM, WN, POLY, GROUPS>>(g, grid, 64 * WM * WN * GROUPS, GROUPS * Tile<kF16, NP, false, false, BM, BM, WM, WN>::kLds, s);
+  return launch<k_ortho_sym<NP, BM, WM, WN, POLY, GROUPS, PARTS>>(g, grid, 64 * WM * WN * GROUPS, GROUPS * Tile<kF16, NP, false, false, BM, BM, WM, WN>::kLds, s);
 }
 template <int NP, bool LAST, int BM, int BN, int WM, int WN, int GROUPS>
 int launch_update_tile(Group& g, hipStream_t s) {
@@ -751,7 +800,13 @@ int launch_update_tile(Group& g, hipStream_t s) {
 }
 template <int NP, int POLY>
 int launch_sym(Group& g, int groups, hipStream_t s) {
-  if (groups == 4) return launch_sym_tile<NP, POLY, 64, 2, 2, 4>(g, s);
+  if (groups == 4) {
+    // one block per CU; a list with more of them takes two quarters of K in turn, two blocks per CU (2 x (1024 x 4096) bf16: 272 blocks in
+    // 32 us, against 38 with a second round for the last 16)
+    int64_t blocks = 0;
+    for (int i = 0; i < g.n; ++i) blocks += tiles_of(g.m[i], kGram, 64, 64);
+    return blocks > kCUs ? launch_sym_tile<NP, POLY, 64, 2, 2, 2, 2>(g, s) : launch_sym_tile<NP, POLY, 64, 2, 2, 4>(g, s);
+  }
   if (groups == 2) return launch_sym_tile<NP, POLY, 96, 2, 2, 2>(g, s);
   switch (pick_tile(g, POLY ? kPoly : kGram, NP)) {
     case kT64: return launch_sym_tile<NP, POLY, 64, 2, 2, 1>(g, s);
