@@ -1126,6 +1126,11 @@ int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s) {
     return 0;
   }
   SUAVE_REQUIRE(h->x && h->weight && h->targets, "linear_ce: x / weight / targets is null");
+  const uintptr_t align = h->dtype == SUAVE_DTYPE_BF16 ? 1 : 3;
+  for (const void* ptr : {h->x, h->weight, static_cast<const void*>(h->dx), static_cast<const void*>(h->dweight)})
+    SUAVE_REQUIRE((reinterpret_cast<uintptr_t>(ptr) & align) == 0, "linear_ce: x / weight / dx / dweight is not aligned to its elements");
+  SUAVE_REQUIRE(h->dx != h->x && h->dx != h->weight && h->dweight != h->x && h->dweight != h->weight && (!h->dx || h->dx != h->dweight),
+                "linear_ce: an output is an input or another output");
   Layout L;
   make_layout(*h, L);
   SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_ce: workspace is null or not 256-byte aligned");

@@ -935,6 +935,8 @@ int launch_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dt
   for (int i = 0; i < n; ++i) {
     SUAVE_REQUIRE(mats[i].in && mats[i].out, "orthogonalize: a matrix is null");
     SUAVE_REQUIRE(mats[i].ld_in >= mats[i].cols && mats[i].ld_out >= mats[i].cols, "orthogonalize: a row stride is shorter than the row");
+    for (int j = 0; j < i; ++j)
+      SUAVE_REQUIRE(mats[i].out != mats[j].out && mats[i].out != mats[j].in && mats[i].in != mats[j].out, "orthogonalize: an output is another matrix of the list");
   }
   Group base{};
   base.eps = eps; base.steps = steps; base.bf16 = dtype == SUAVE_DTYPE_BF16;
@@ -964,6 +966,10 @@ int launch_muon(const suave_muon_matrix_t* mats, int32_t n, float momentum, int 
     SUAVE_REQUIRE(h.param && h.grad && h.momentum, "muon_step: param / grad / momentum is null");
     SUAVE_REQUIRE(h.ld_param >= h.cols && h.ld_grad >= h.cols && h.ld_momentum >= h.cols, "muon_step: a row stride is shorter than the row");
     SUAVE_REQUIRE(std::isfinite(h.lr) && h.lr >= 0.f, "muon_step: lr must not be negative");
+    SUAVE_REQUIRE(h.param != h.grad && h.param != h.momentum && h.grad != h.momentum, "muon_step: param, grad and momentum must be three matrices");
+    for (int j = 0; j < i; ++j)
+      SUAVE_REQUIRE(h.param != mats[j].param && h.momentum != mats[j].momentum && h.param != mats[j].momentum && h.momentum != mats[j].param,
+                    "muon_step: a matrix is in the list twice");
   }
   Group base{};
   base.eps = eps; base.steps = steps; base.muon = 1; base.momentum = momentum; base.nesterov = nesterov;

@@ -8,7 +8,7 @@ torch operator runs on the compute path.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Mapping, Optional, Sequence
+from typing import Dict, Mapping, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -263,6 +263,61 @@ class Engine:
                                       self.exp_avg_sq.data_ptr(), gb, lra, 3, self.adam_t, float(betas[0]),
                                       float(betas[1]), float(eps), self._stream())
         _lib.check(rc, "suave_adam_step")
+
+    def hidden_matrices(self) -> Dict[str, Tuple[int, int, int, int]]:
+        """The hidden layers' weight matrices in the flat buffers: name -> (offset, rows, columns, row stride).  Without the
+        first encoder layer of wide schemas, whose columns are spread over embedding blocks."""
+
+        return {name: (s.offset, int(s.shape[0]), int(s.shape[1]), int(s.ld)) for name, s in self.layout.slots.items()
+                if ".backbone." in name and name.endswith(".weight") and s.col_index is None}
+
+    def muon_step(self, lr: float | Mapping[str, float], *, adam_lr: float | Mapping[str, float], momentum: float = 0.95,
+                  nesterov: bool = True, weight_decay: float = 0.0, betas=(0.9, 0.999), eps: float = 1e-8) -> None:
+        """``adam_step`` with the hidden layers' weight matrices updated by Muon (suave_muon_step) instead: orthogonalised
+        momentum at ``lr``; biases, heads and the prior by Adam at ``adam_lr``.  Either may map group name
+        (encoder/decoder/prior) -> lr (0 = frozen: nothing of the group moves, nor its momenta).  A matrix's momentum lives
+        in its part of ``exp_avg``; ``reset_optimizer`` before changing over from ``adam_step`` or back."""
+
+        from . import operators as ops
+
+        names = ["encoder", "decoder", "prior"]
+        by_group = [{n: float(v[n]) if isinstance(v, Mapping) else float(v) for n in names} for v in (lr, adam_lr)]
+        mats = [(name.split(".", 1)[0], m) for name, m in self.hidden_matrices().items()]
+        moving = [(g, m) for g, m in mats if by_group[0][g] != 0.0]
+        if moving:
+            view = lambda t, m: t.as_strided((m[1], m[2]), (m[3], 1), m[0])  # noqa: E731
+            ops.muon_step([view(self.params, m) for _, m in moving], [view(self.grads, m) for _, m in moving],
+                          [view(self.exp_avg, m) for _, m in moving], lr=[by_group[0][g] for g, _ in moving],
+                          momentum=momentum, nesterov=nesterov, weight_decay=weight_decay)
+        self.adam_t += 1
+        begins, lrs = [], []  # ranges of the flat buffer and their learning rates: a matrix's own range stays as it is
+
+        def add(begin: int, v: float) -> None:
+            if lrs and lrs[-1] == v:
+                return
+            begins.append(begin)
+            lrs.append(v)
+
+        for n in names:
+            g0, g1 = self.layout.group_ranges[n]
+            at = g0
+            for off, rows, _, ld in sorted(m for g, m in mats if g == n):
+                if off > at:
+                    add(at, by_group[1][n])
+                add(off, 0.0)
+                at = off + rows * ld
+            if g1 > at:
+                add(at, by_group[1][n])
+        end = self.layout.group_ranges["prior"][1]
+        for i in range(0, len(lrs), 8):  # a call takes eight ranges
+            part, b0 = lrs[i:i + 8], begins[i]
+            b1 = begins[i + 8] if i + 8 < len(begins) else end
+            gb = (C.c_int32 * (len(part) + 1))(*[b - b0 for b in begins[i:i + 8]], b1 - b0)
+            lra = (C.c_float * len(part))(*part)
+            rc = self.lib.suave_adam_step(*(t.data_ptr() + 4 * b0 for t in (self.params, self.grads, self.exp_avg, self.exp_avg_sq)),
+                                          gb, lra, len(part), self.adam_t, float(betas[0]), float(betas[1]), float(eps),
+                                          self._stream())
+            _lib.check(rc, "suave_adam_step")
 
     def head_step(self, head, latent: torch.Tensor, rows: torch.Tensor, *, logits: Optional[torch.Tensor] = None) -> None:
         """suave_head_step: one batch of the classifier-head phase on cached latents -- ``rows`` (int32) are row ids into

@@ -145,6 +145,7 @@ class SUAVE:
         self._warmup_val_history: list = []
         self._train_history: list = []
         self._classifier: Optional[sup.ClassificationHead] = None
+        self._quantized_head: Optional[sup.QuantizedHead] = None
         self._temperature_scaler = sup.TemperatureScaler()
         self._is_calibrated = False
         self._joint_val_metrics: Optional[Dict[str, float]] = None
@@ -453,6 +454,7 @@ class SUAVE:
         self._gen.manual_seed(self.random_state)
         self._step = 0
         self._classifier = None
+        self._quantized_head = None
         self._warmup_phase(train, val, n_epochs, bs, kl_epochs)
         supervised = self.behaviour == "supervised" and y_train_t is not None
         if supervised:
@@ -1128,8 +1130,20 @@ class SUAVE:
         if table.n_rows == 0:
             return np.empty((0, len(self._classes)), np.float32)
         self._classifier.eval()
+        served = self._quantized_head
+        if served is not None and served.clf is self._classifier:
+            return served(self._posterior_mean(table)).cpu().numpy()
         with torch.no_grad():
             return self._classifier(self._posterior_mean(table)).cpu().numpy()
+
+    def quantize_classifier(self, enable: bool = True) -> "SUAVE":
+        """Serve the classifier's logits (``predict``, ``predict_proba``, ``calibrate``) from 8-bit weights
+        (``supervised.QuantizedHead``) until the next ``fit`` or ``quantize_classifier(False)``.  Not saved with the model;
+        off by default."""
+
+        self._ensure_classifier("quantize_classifier")
+        self._quantized_head = sup.QuantizedHead(self._classifier) if enable else None
+        return self
 
     def _resolve_attribute(self, attr):
         names = list(self.schema.feature_names)

@@ -215,6 +215,102 @@ class DeviceHead:
         return self.class_weight[self.targets[rows].long()].sum().reshape(1)
 
 
+class ManyClassHead:
+    """Library-side training state of a ``ClassificationHead`` without hidden layers and with ANY number of classes
+    (``DeviceHead`` serves 2..64): the loss and its gradients come from ``suave_linear_ce``, which never holds the
+    ``[rows, classes]`` logits, the update from ``suave_adam_step``; ``quantized`` gives the serving form.  The module's
+    ``linear`` parameters are re-homed as views of one flat buffer (weight [C, D] then bias [C]), as ``DeviceHead`` does.
+    """
+
+    def __init__(self, clf: ClassificationHead) -> None:
+        if not self.supports(clf):
+            raise ValueError("ManyClassHead serves heads without hidden layers on a GPU device")
+        w, b = clf.linear.weight, clf.linear.bias
+        self.C, self.D = int(w.shape[0]), int(w.shape[1])
+        n = self.C * self.D
+        self.flat = torch.cat([w.detach().reshape(-1), b.detach().reshape(-1)]).to(torch.float32).contiguous()
+        w.data, b.data = self.flat[:n].view(self.C, self.D), self.flat[n:]
+        self.clf = clf
+        self.grads = torch.zeros_like(self.flat)
+        self._dw, self._db = self.grads[:n].view(self.C, self.D), self.grads[n:]
+        self.m, self.v = torch.zeros_like(self.flat), torch.zeros_like(self.flat)
+        self.t = 0
+        self.class_weight = clf.class_weight.to(torch.float32).contiguous() if clf._use_weight else None
+
+    @staticmethod
+    def supports(clf: ClassificationHead) -> bool:
+        return clf.hidden_layers is None and clf.linear.weight.is_cuda
+
+    def reset_optimizer(self) -> None:
+        self.m.zero_()
+        self.v.zero_()
+        self.t = 0
+
+    def loss(self, latent: torch.Tensor, targets: torch.Tensor, *, training: bool = True, loss_scale: float = 1.0,
+             weight_sum: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None, key: int = 0) -> Dict[str, torch.Tensor]:
+        """``loss`` and ``row_loss`` of ``latent`` [n, D] against ``targets`` [n] (negative: the row is left out).
+        ``training``: through the head's dropout (``rows`` / ``key`` as in ``ClassificationHead.forward``), with ``grads``
+        overwritten and ``dlatent`` [n, D] returned, both multiplied by ``loss_scale``."""
+
+        from . import operators as ops
+
+        w, b = self.clf.linear.weight.detach(), self.clf.linear.bias.detach()
+        latent, t32 = latent.detach(), targets.to(torch.int32).contiguous()
+        keep = None
+        drop = self.clf._final_dropout
+        if training and drop is not None and drop.p > 0.0:
+            was, drop.training, drop.ctx = drop.training, True, None if rows is None else (rows, key)
+            try:
+                keep = drop(torch.ones_like(latent))
+            finally:
+                drop.training, drop.ctx = was, None
+            latent = latent * keep
+        grads = {"dweight": self._dw, "dbias": self._db} if training else {}
+        out = ops.linear_cross_entropy(latent, w, t32, bias=b, class_weight=self.class_weight, weight_sum=weight_sum,
+                                       loss_scale=loss_scale, grad=training, **grads)
+        res = {"loss": out["loss"], "row_loss": out["row_loss"]}
+        if training:
+            res["dlatent"] = out["dx"] if keep is None else out["dx"] * keep
+        return res
+
+    def step(self, engine, latent: torch.Tensor, targets: torch.Tensor, lr: float, **kw) -> Dict[str, torch.Tensor]:
+        """``loss`` in training mode, then one Adam step of the head's parameters."""
+
+        res = self.loss(latent, targets, training=True, **kw)
+        self.t += 1
+        engine.adam_flat(self.flat, self.grads, self.m, self.v, self.t, lr)
+        return res
+
+    def quantized(self) -> "QuantizedHead":
+        return QuantizedHead(self.clf)
+
+
+class QuantizedHead:
+    """Serving form of a ``ClassificationHead``: the eval-mode logits with the last layer as 8-bit integers, one scale per
+    class and per row (``suave_quantize_rows`` once here, ``suave_linear_quantized`` per call).  A snapshot: later changes
+    of the head's parameters do not reach it.  Each logit is off by at most ``sum |x| s_w / 2 + sum |w| s_x / 2 + D s_w s_x / 4``
+    (half a step of either scale)."""
+
+    def __init__(self, clf: ClassificationHead) -> None:
+        from . import operators as ops
+
+        self.clf = clf
+        self.weight, self.scale = ops.quantize_rows(clf.linear.weight.detach())
+        self.bias = clf.linear.bias.detach().to(torch.float32).clone()
+
+    def __call__(self, latents: torch.Tensor) -> torch.Tensor:
+        from . import operators as ops
+
+        x = latents.detach()
+        if self.clf.hidden_layers is not None:
+            was = self.clf.hidden_layers.training
+            self.clf.hidden_layers.eval()
+            with torch.no_grad():
+                x = self.clf.hidden_layers(x)
+            self.clf.hidden_layers.train(was)
+        return ops.linear_quantized(x.contiguous(), self.weight, self.scale, bias=self.bias)
+
+
 class TemperatureScaler:
     """calibrate.py:16-112: one log-temperature fitted by Adam on the cross-entropy of ``logits / T``."""
 
