@@ -899,7 +899,7 @@ int check_args(const suave_linear_ce_t* h) {
   SUAVE_REQUIRE(h->n_classes >= 1 && h->n_classes <= (1 << 24), "linear_ce: n_classes must be in 1..2^24");
   SUAVE_REQUIRE(h->dim >= 1 && h->dim <= 32768, "linear_ce: dim must be in 1..32768");
   SUAVE_REQUIRE(h->n_rows >= 0 && h->n_rows <= (1 << 24), "linear_ce: n_rows must be in 0..2^24");
-  SUAVE_REQUIRE(h->n_rows * h->n_classes <= ((int64_t)1 << 40), "linear_ce: n_rows * n_classes must be at most 2^40");
+  SUAVE_REQUIRE(h->n_rows * h->n_classes <= ((int64_t)1 << 38), "linear_ce: n_rows * n_classes must be at most 2^38");  // (2^32 threads a launch)
   SUAVE_REQUIRE(h->ld_x >= h->dim && h->ld_weight >= h->dim, "linear_ce: a row stride is shorter than the row");
   SUAVE_REQUIRE(h->ld_x <= (1 << 22) && h->ld_weight <= (1 << 22), "linear_ce: row strides of x and weight must be at most 2^22 elements");
   SUAVE_REQUIRE(!h->dx || h->ld_dx >= h->dim, "linear_ce: ld_dx < dim");

@@ -227,6 +227,8 @@ class ManyClassHead:
             raise ValueError("ManyClassHead serves heads without hidden layers on a GPU device")
         w, b = clf.linear.weight, clf.linear.bias
         self.C, self.D = int(w.shape[0]), int(w.shape[1])
+        if self.C * (self.D + 1) > 1 << 30:
+            raise ValueError("ManyClassHead: at most 2^30 parameters (suave_adam_step counts them in 32 bits)")
         n = self.C * self.D
         self.flat = torch.cat([w.detach().reshape(-1), b.detach().reshape(-1)]).to(torch.float32).contiguous()
         w.data, b.data = self.flat[:n].view(self.C, self.D), self.flat[n:]
@@ -308,7 +310,14 @@ class QuantizedHead:
             with torch.no_grad():
                 x = self.clf.hidden_layers(x)
             self.clf.hidden_layers.train(was)
-        return ops.linear_quantized(x.contiguous(), self.weight, self.scale, bias=self.bias)
+        x = x.contiguous()
+        n, step = int(x.shape[0]), 1 << 20  # rows of a call
+        if n <= step:
+            return ops.linear_quantized(x, self.weight, self.scale, bias=self.bias)
+        out = torch.empty((n, int(self.weight.shape[0])), dtype=x.dtype, device=x.device)
+        for r in range(0, n, step):
+            ops.linear_quantized(x[r:r + step], self.weight, self.scale, bias=self.bias, out=out[r:r + step])
+        return out
 
 
 class TemperatureScaler:

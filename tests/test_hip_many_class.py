@@ -84,6 +84,23 @@ def test_heads_with_hidden_layers_are_refused():
         sup.QuantizedHead(sup.ClassificationHead(8, 5))
 
 
+def test_sizes_the_classes_state():
+    import torch
+    from suave_amd import supervised as sup
+
+    with torch.device("meta"):
+        big = sup.ClassificationHead(1 << 15, 1 << 15)
+    big.linear.weight = torch.nn.Parameter(torch.empty(1, device="cuda:0").expand(1 << 15, 1 << 15), requires_grad=False)
+    with pytest.raises(ValueError, match="2\\^30"):
+        sup.ManyClassHead(big)
+    # more rows than one call serves: the same as in two
+    clf = _head(3, 4, 0.0, False)
+    q = sup.QuantizedHead(clf)
+    x = torch.randn((1 << 20) + 5, 4, device="cuda:0")
+    a = q(x)
+    assert torch.equal(a[:1 << 20], q(x[:1 << 20])) and torch.equal(a[1 << 20:], q(x[1 << 20:]))
+
+
 @pytest.mark.parametrize("frozen", [(), ("decoder",), ("encoder", "decoder", "prior")])
 def test_engine_muon_step(frozen):
     import torch
@@ -179,7 +196,7 @@ def test_train_update_and_serve():
     sw, sx = w.abs().amax(1) / 127.0, x.abs().amax(1) / 127.0
     q = lambda a, s: torch.round(a.double() / torch.where(s == 0, torch.ones_like(s), s).double()[:, None])  # noqa: E731
     want = (q(x, sx) @ q(w, sw).t()) * sx.double()[:, None] * sw.double()[None] + clf.linear.bias.detach().double()
-    assert float((logits.double() - want).abs().max()) <= 3 * 2.0 ** -24 * float((want.abs() + clf.linear.bias.abs().max()).max())
+    assert float((logits.double() - want).abs().max()) <= 3 * 2.0 ** -24 * float((want.abs() + clf.linear.bias.detach().abs().max()).max())
     # and against the head itself: half a step of either scale per product
     full = x.double() @ w.double().t() + clf.linear.bias.double()
     bound = (x.double().abs().sum(1)[:, None] * sw.double()[None] / 2 + w.double().abs().sum(1)[None] * sx.double()[:, None] / 2

@@ -41,7 +41,7 @@ def _ce(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(dtype=2), "dtype"), (dict(n_classes=0), "n_classes"), (dict(n_classes=(1 << 24) + 1), "n_classes"), (dict(dim=0), "dim"),
     (dict(dim=32769), "dim"), (dict(n_rows=-1), "n_rows"), (dict(n_rows=(1 << 24) + 1), "n_rows"),
-    (dict(n_rows=1 << 20, n_classes=(1 << 20) + 1), "2^40"), (dict(ld_x=31), "stride"), (dict(ld_weight=31), "stride"),
+    (dict(n_rows=1 << 20, n_classes=(1 << 18) + 1), "2^38"), (dict(ld_x=31), "stride"), (dict(ld_weight=31), "stride"),
     (dict(ld_x=(1 << 22) + 1), "stride"), (dict(ld_dx=31), "ld_dx"), (dict(ld_dweight=31), "ld_dweight")])
 def test_linear_ce_sizes(lib, kw, text):
     n = C.c_size_t(0)
