@@ -312,3 +312,52 @@ def test_other_stream_and_captured_graph():
         torch.cuda.synchronize()
         eager = ops.linear_cross_entropy(x, w, y, bias=b, class_weight=cw)
         assert all(torch.equal(out[k], eager[k]) for k in eager)
+
+
+# float32 from 256 columns on, and few classes: other paths through the kernels than the sizes above
+@pytest.mark.parametrize("n,c,d", [(1, 300, 256), (33, 257, 300), (700, 1111, 261), (95, 5001, 512), (1100, 200, 40), (1025, 256, 256),
+                                   (2049, 3, 20), (1024, 256, 8)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_wide_rows_and_few_classes(n, c, d, dtype):
+    import torch
+    from suave_amd import operators as ops
+
+    dt = getattr(torch, dtype)
+    x, w, b, y, cw = _case(n, c, d, dt, c % 2 == 1, seed=n + c + d)
+    got = ops.linear_cross_entropy(x, w, y, bias=b, class_weight=cw, loss_scale=1.5)
+    _check(got, _reference(x, w, b, y, cw, scale=1.5), x, w, y)
+    again = ops.linear_cross_entropy(x, w, y, bias=b, class_weight=cw, loss_scale=1.5)
+    assert all(torch.equal(again[k], got[k]) for k in got)
+    only = ops.linear_cross_entropy(x, w, y, bias=b, class_weight=cw, grad=False)
+    assert torch.equal(only["row_loss"], got["row_loss"]) and torch.equal(only["loss"], got["loss"])
+
+
+@pytest.mark.parametrize("c,d", [(400, 256), (250, 24), (700, 300)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_masked_classes_and_rows_on_every_path(c, d, dtype):
+    """Strips of 64 classes at -inf or at the type's lowest value, a target among the former, rows left out that hold NaN."""
+    import torch
+    from suave_amd import operators as ops
+
+    dt = getattr(torch, dtype)
+    for low in (-float("inf"), torch.finfo(torch.float32).min):
+        x, w, b, y, _ = _case(50, c, d, dt, False, seed=4, drop=0)
+        b[64:192] = low
+        y = torch.where((y >= 64) & (y < 192), torch.full_like(y, 10), y)
+        y[7] = -1
+        keep = torch.tensor([i for i in range(c) if not 64 <= i < 192], device="cuda:0")
+        ref = _reference(x, w[keep], b[keep], torch.where(y >= 192, y - 128, y), None)
+        bad = x.clone()
+        bad[7] = float("nan")
+        got = ops.linear_cross_entropy(bad, w, y, bias=b)
+        full = dict(got, dweight=got["dweight"][keep], dbias=got["dbias"][keep])
+        got["lse"][7] = full["lse"][7] = float(ref["lse"][7])  # not defined for a row that is left out
+        _check(full, ref, x, w[keep], y)
+        assert bool((got["dweight"][64:192] == 0).all()) and bool((got["dbias"][64:192] == 0).all())
+    b[64:192] = -float("inf")
+    y[3] = 100
+    hit = ops.linear_cross_entropy(x, w, y, bias=b)
+    assert math.isinf(float(hit["row_loss"][3])) and float(hit["row_loss"][3]) > 0 and math.isinf(float(hit["loss"]))
+    assert bool(torch.isfinite(hit["dx"]).all()) and bool(torch.isfinite(hit["dweight"]).all())
+    # the target's entry of G is -1 / rows there: seen in the bias gradient
+    assert abs(float(hit["dbias"][100]) + 1.0 / 49) <= 2.0 ** -22
