@@ -214,12 +214,34 @@ __device__ __forceinline__ void write_results(const Group& g, const Mat& m, int 
   }
 }
 
-// X_0 in planes, pads zero; the sizes of X_0 .. X_steps
+// X_0 in planes, pads zero; the sizes of X_0 .. X_steps.  The norm is a chain of a few microseconds in every block, so two chunks
+// per thread are asked for in front of it and the grid fits the card in one round; the scaling is two exact-range binary32 steps (in
+// doubles the kernel was bound by their conversions: 2 x (1024 x 4096) bf16 18 us, this 11).
+constexpr int kPackBlocks = 512;  // per matrix
 template <int NP>
 __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
   const int i = find_mat(g, blockIdx.x);
   const Mat& m = g.m[i];
   const int b = blockIdx.x - g.begin[i], nb = g.begin[i + 1] - g.begin[i];
+  const int cp = (m.cols + 7) / 8 * 8, q = cp / 8;
+  const int64_t chunks = (int64_t)m.rows * q, step = (int64_t)nb * 256;
+  const int pit = pitch(m.cols, NP);
+  constexpr int U = 2;
+  float in[U][8];
+  int64_t r[U];
+  int c0[U];
+  auto load = [&](int64_t e0) {
+#pragma unroll
+    for (int h = 0; h < U; ++h) {
+      const int64_t e = e0 + h * step;
+      if (e >= chunks) continue;
+      r[h] = chunks < (1ll << 31) ? (int64_t)((uint32_t)e / (uint32_t)q) : e / q;
+      c0[h] = (int)(e - r[h] * q) * 8;
+      in_values(g, m, r[h], c0[h], in[h]);
+    }
+  };
+  int64_t e0 = (int64_t)b * 256 + threadIdx.x;
+  load(e0);
   __shared__ double sc, part[4];
   {
     double s = 0.0;
@@ -236,25 +258,26 @@ __global__ __launch_bounds__(256) void k_ortho_pack(Group g) {
     }
   }
   __syncthreads();
-  const double scale = sc;
-  const int cp = (m.cols + 7) / 8 * 8, q = cp / 8;
-  const int64_t chunks = (int64_t)m.rows * q;
-  const int pit = pitch(m.cols, NP);
-  for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
-    const int64_t r = chunks < (1ll << 31) ? (int64_t)((uint32_t)e / (uint32_t)q) : e / q;
-    const int c0 = (int)(e - r * q) * 8;
-    uint16_t hi[8], lo[8];
-    float in[8];
-    in_values(g, m, r, c0, in);
+  // scale = sm 2^se: the power of two first, so neither a subnormal U nor a huge scale leaves binary32
+  int se = 0;
+  const float sm = (float)frexp(sc, &se);
+  while (e0 < chunks) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float v = c0 + u < m.cols ? (float)((double)in[u] * scale) : 0.f;
-      if constexpr (NP == 2) planes(v, hi[u], lo[u]);
-      else hi[u] = f16_bits((_Float16)v);
+    for (int h = 0; h < U; ++h) {
+      if (e0 + h * step >= chunks) continue;
+      uint16_t hi[8], lo[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float v = c0[h] + u < m.cols ? ldexpf(in[h][u], se) * sm : 0.f;
+        if constexpr (NP == 2) planes(v, hi[u], lo[u]);
+        else hi[u] = f16_bits((_Float16)v);
+      }
+      char* o = m.x[0] + r[h] * pit + c0[h] * 2;
+      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+      if constexpr (NP == 2) *reinterpret_cast<uint4*>(o + cp * 2) = *reinterpret_cast<const uint4*>(lo);
     }
-    char* o = m.x[0] + r * pit + c0 * 2;
-    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
-    if constexpr (NP == 2) *reinterpret_cast<uint4*>(o + cp * 2) = *reinterpret_cast<const uint4*>(lo);
+    e0 += U * step;
+    load(e0);
   }
 }
 
@@ -303,9 +326,12 @@ __device__ __forceinline__ void upper_tile(int t, int T, int& tm, int& tn) {
   tn = tm + t;
 }
 
+// Waves per SIMD that a block's registers must leave room for: 1024 threads, or two blocks of 512, on a CU
+constexpr int min_waves(int threads, int parts) { return threads >= 1024 || parts > 1 ? 4 : 2; }
+
 // POLY 0: A from X; 1: B from A
 template <int NP, int BM, int WM, int WN, int POLY, int GROUPS, int PARTS>
-__global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_sym(Group g) {
+__global__ __launch_bounds__(64 * WM * WN * GROUPS, min_waves(64 * WM * WN * GROUPS, PARTS)) void k_ortho_sym(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   typedef Tile<kF16, NP, false, false, BM, BM, WM, WN> R;
   typedef Tile<kF16, NP, true, true, BM, BM, WM, WN> C;
@@ -369,7 +395,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
 
 // X <- B X (wide) or X B (tall); the last step writes the result or takes the step on the parameter
 template <int NP, int BM, int BN, int WM, int WN, bool LAST, int GROUPS>
-__global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_ortho_update(Group g) {
+__global__ __launch_bounds__(64 * WM * WN * GROUPS, min_waves(64 * WM * WN * GROUPS, 1)) void k_ortho_update(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   typedef Tile<kF16, NP, false, true, BM, BN, WM, WN> W;
   typedef Tile<kF16, NP, false, false, BM, BN, WM, WN> H;
@@ -393,23 +419,45 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, GROUPS > 1 ? 4 : 2) void k_o
   const int e = g.exps[m.id * (kMaxSteps + 1) + g.k], e1 = LAST ? 12 : g.exps[m.id * (kMaxSteps + 1) + g.k + 1];
   const float f = ldexpf(1.0f, max(e - e1 - 12, -126));
   const int cp = (m.cols + 7) / 8 * 8;
+  // a wave's planes leave in whole rows; blocks of several groups hold every other fragment only and store them as they are
+  constexpr bool kStaged = !LAST && GROUPS == 1;
+  typedef RowStage<uint16_t, W::NI * 16> Rows;
+  static_assert(!kStaged || WM * WN * NP * Rows::kBytes <= W::kLds, "the stages fit the tile's LDS");
+  char* stage = lds + wave * (NP * Rows::kBytes);
+  const int n_wave = n0 + wn * (W::NI * 16);
 #pragma unroll
   for (int mi = 0; mi < W::MI; ++mi) {
-    const int r = m0 + wm * (W::MI * 16) + 16 * mi + (lane & 15);
-    if (r >= m.rows) continue;
+    const int r0 = m0 + wm * (W::MI * 16) + 16 * mi, r = r0 + (lane & 15);
+    if (!kStaged && r >= m.rows) continue;
 #pragma unroll
     for (int j = 0; j < W::NI; ++j) {
       if (GROUPS > 1 && (W::MI * j + mi) % GROUPS != group) continue;
-      const int n = n0 + wn * (W::NI * 16) + 16 * j + 4 * (lane >> 4);
-      if (n >= (LAST ? m.cols : cp)) continue;
+      const int n = n_wave + 16 * j + 4 * (lane >> 4);
+      if (!kStaged && n >= (LAST ? m.cols : cp)) continue;
       float v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = acc[mi][j][u] * f;
-      if constexpr (!LAST) {
-        store_planes<NP>(m.x[(g.k & 1) ^ 1], px, m.cols, r, n, v);
-      } else {
+      if constexpr (LAST) {
         write_results(g, m, r, n, v);
+      } else if constexpr (kStaged) {
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float x = n + u < m.cols ? v[u] : 0.f;
+          if constexpr (NP == 2) planes(x, hi[u], lo[u]);
+          else hi[u] = f16_bits((_Float16)x);
+        }
+        Rows::put(stage, lane & 15, n - n_wave, hi);
+        if constexpr (NP == 2) Rows::put(stage + Rows::kBytes, lane & 15, n - n_wave, lo);
+      } else {
+        store_planes<NP>(m.x[(g.k & 1) ^ 1], px, m.cols, r, n, v);
       }
+    }
+    if constexpr (kStaged) {
+      const int rows = max(0, min(16, m.rows - r0)), cols = max(0, cp - n_wave);
+      char* o = m.x[(g.k & 1) ^ 1] + (int64_t)r0 * px + n_wave * 2;
+      Rows::flush(stage, o, px, rows, cols, lane);
+      if constexpr (NP == 2) Rows::flush(stage + Rows::kBytes, o + cp * 2, px, rows, cols, lane);
     }
   }
 }
@@ -844,7 +892,7 @@ int run_group(Group& g, char* ws, hipStream_t s) {
   int grid = set_begin(g, [](const Mat& m) { return norm_blocks(m.rows, m.cols); });
   hipLaunchKernelGGL(k_ortho_norm, dim3(grid), dim3(256), 0, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
-  grid = set_begin(g, [](const Mat& m) { return std::min<int64_t>(1024, std::max<int64_t>(1, ceil_div((int64_t)m.rows * ((m.cols + 7) / 8), 256))); });
+  grid = set_begin(g, [](const Mat& m) { return std::min<int64_t>(kPackBlocks, std::max<int64_t>(1, ceil_div((int64_t)m.rows * ((m.cols + 7) / 8), 256))); });
   hipLaunchKernelGGL(k_ortho_pack<NP>, dim3(grid), dim3(256), 0, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
   Group part[3];  // the matrices of a phase by groups 1, 2, 4
