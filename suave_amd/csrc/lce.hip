@@ -592,20 +592,22 @@ __global__ __launch_bounds__(256) void k_lce_scale(ScaleArgs a) {
   a.db[rb * a.db_ld + (c - cl * 8) + threadIdx.x] = s * (1.0f / g_scale(true));
 }
 
-// lse of 16 rows per block (1024 threads: 16 rows x 64 strip groups), their loss terms and weights.  The sums over all blocks are
-// left to the next launch: a ticket that lets the last block do it costs every block a release and an acquire at device scope
-// (4096 rows: 18 us, this 8).
+// lse of R rows per block (1024 threads: R rows x 1024 / R strip groups), their loss terms and weights: 16 rows, or 4 for batches that
+// would fill few CUs with 16 (33 x 100000: 6 us against 8).  The sums over all blocks are left to the next launch: a ticket that lets
+// the last block do it costs every block a release and an acquire at device scope (4096 rows: 18 us, this 7).
+template <int R>
 __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
-  __shared__ float2 ms[64][17];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t m = (int64_t)blockIdx.x * 16 + r;
+  constexpr int G = 1024 / R;
+  __shared__ float2 ms[G][R + 1];
+  const int r = threadIdx.x % R, q = threadIdx.x / R;
+  const int64_t m = (int64_t)blockIdx.x * R + r;
   float mx = -INFINITY, s = 0.f;
   if (m < a.n) {
     constexpr int U = 8;  // strips in flight
-    for (int t0 = q; t0 < a.n_strips; t0 += 64 * U) {
+    for (int t0 = q; t0 < a.n_strips; t0 += G * U) {
       float2 v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = t0 + 64 * u < a.n_strips ? a.strips[(int64_t)(t0 + 64 * u) * a.n + m] : make_float2(-INFINITY, 0.f);
+      for (int u = 0; u < U; ++u) v[u] = t0 + G * u < a.n_strips ? a.strips[(int64_t)(t0 + G * u) * a.n + m] : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (v[u].y == 0.f) continue;  // nothing of the strip counts (all -inf); NaN goes on
@@ -617,34 +619,33 @@ __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
   }
   ms[q][r] = make_float2(mx, s);
   __syncthreads();
-  if (threadIdx.x < 64) {  // four lanes per row, 16 groups each
-    const int part = threadIdx.x >> 4;
-    float M = -INFINITY, S = 0.f;
+  if (threadIdx.x >= 64) return;
+  const int part = threadIdx.x / R;  // 64 / R lanes per row, 16 groups each
+  float M = -INFINITY, S = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) M = fmaxf(M, ms[part * 16 + k][r].x);
-    M = fmaxf(M, __shfl_xor(M, 16, 64));
-    M = fmaxf(M, __shfl_xor(M, 32, 64));
+  for (int k = 0; k < 16; ++k) M = fmaxf(M, ms[part * 16 + k][r].x);
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (ms[part * 16 + k][r].y != 0.f) S += ms[part * 16 + k][r].y * __expf(ms[part * 16 + k][r].x - M);
-    S += __shfl_xor(S, 16, 64);
-    S += __shfl_xor(S, 32, 64);
-    double ce = 0.0, wsum = 0.0;
-    if (part == 0 && m < a.n) {
-      const float lse = S == 0.f ? -INFINITY : M + logf(S);
-      float l, w;
-      finish_row(a, m, lse, a.target_logit[m], l, a.row[m], w);
-      ce = l;
-      wsum = w;
-    }
-    for (int off = 8; off > 0; off >>= 1) {
-      ce += __shfl_xor(ce, off, 64);
-      wsum += __shfl_xor(wsum, off, 64);
-    }
-    if (threadIdx.x == 0) {
-      a.part[2 * blockIdx.x] = ce;
-      a.part[2 * blockIdx.x + 1] = wsum;
-    }
+  for (int off = R; off < 64; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (ms[part * 16 + k][r].y != 0.f) S += ms[part * 16 + k][r].y * __expf(ms[part * 16 + k][r].x - M);
+#pragma unroll
+  for (int off = R; off < 64; off <<= 1) S += __shfl_xor(S, off, 64);
+  double ce = 0.0, wsum = 0.0;
+  if (part == 0 && m < a.n) {
+    const float lse = S == 0.f ? -INFINITY : M + logf(S);
+    float l, w;
+    finish_row(a, m, lse, a.target_logit[m], l, a.row[m], w);
+    ce = l;
+    wsum = w;
+  }
+  for (int off = R / 2; off > 0; off >>= 1) {
+    ce += __shfl_xor(ce, off, 64);
+    wsum += __shfl_xor(wsum, off, 64);
+  }
+  if (threadIdx.x == 0) {
+    a.part[2 * blockIdx.x] = ce;
+    a.part[2 * blockIdx.x + 1] = wsum;
   }
 }
 
@@ -816,6 +817,8 @@ LogitTile logit_tile(int64_t n, int64_t classes) {
 // (1000 x 250 x 256: 38 us by 16 rows against 43; 4096 x 256 x 128: 54 against 48)
 LogitTile whole_tile(int64_t n) { return n <= 1024 ? kLow16 : kLow64; }
 
+int rows_per_block(int64_t n) { return n <= 1024 ? 4 : 16; }  // of k_lce_rows
+
 // Tile and K splits of the two gradient products of a piece.  A split takes whole multiples of 64 values of K, so a product of
 // K values has at most K / 64 of them; dW is not split when the classes come in several pieces (its rows are then plenty).
 void pick_grad(int64_t n, int cp, int dim, int planes, bool dx, bool dw, bool one_piece, Layout& L) {
@@ -871,7 +874,7 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   // 81, 4096 x 1000 x 16: 64 against 57)
   L.keep = f32 && grad && L.pieces == 1 && !L.whole && h.dim >= 256;
   L.db_rows = L.keep ? (int)ceil_div(n, kScaleRows) : (int)ceil_div(n, kLogitM[L.tile_g]) * kLogitWM[L.tile_g];
-  L.row_blocks = (int)ceil_div(n, L.whole ? kLogitM[L.tile_s] : 16);
+  L.row_blocks = (int)ceil_div(n, L.whole ? kLogitM[L.tile_s] : rows_per_block(n));
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
   L.scal = take(sizeof(Scalars));
@@ -1017,7 +1020,8 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     } else {
       if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
     }
-    hipLaunchKernelGGL(k_lce_rows, dim3(L.row_blocks), dim3(1024), 0, s, r);
+    if (rows_per_block(n) == 4) hipLaunchKernelGGL(k_lce_rows<4>, dim3(L.row_blocks), dim3(1024), 0, s, r);
+    else hipLaunchKernelGGL(k_lce_rows<16>, dim3(L.row_blocks), dim3(1024), 0, s, r);
     SUAVE_CHECK_HIP(hipGetLastError());
   }
   if (!grad || (L.whole && !products)) {

@@ -87,6 +87,18 @@ __device__ __forceinline__ void load8(const T* row, int k0, int cols, int vec, f
   }
 }
 
+__device__ __forceinline__ uint2 quantize8(const float (&u)[8], float s, float inv, bool finite, bool tiny) {
+  uint32_t k[8];
+  float off = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], inv, off);
+  if (!finite || tiny || off > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(!finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv));
+  }
+  return make_uint2(low_bytes(k[0], k[1], k[2], k[3]), low_bytes(k[4], k[5], k[6], k[7]));
+}
+
 // W waves share a row; a lane keeps P runs of 8 values, all loaded at once, and quantises them from its registers.  What a
 // row holds beyond W P 512 values is read twice.
 template <class T, int W, int P>
@@ -127,18 +139,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
   const bool finite = mx < 0x7f800000u, tiny = s < 1e-30f;
   const float inv = 1.0f / s;
   const int end = (a.cols + 15) / 16 * 16;
-  auto write = [&](int k0, const float (&u)[8]) {
-    uint32_t k[8];
-    float off = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], inv, off);
-    if (!finite || tiny || off > 0.4999f) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(!finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv));
-    }
-    const uint2 o = make_uint2(low_bytes(k[0], k[1], k[2], k[3]), low_bytes(k[4], k[5], k[6], k[7]));
-    *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = o;
-  };
+  auto write = [&](int k0, const float (&u)[8]) { *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = quantize8(u, s, inv, finite, tiny); };
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (p * kRun + t * 8 < end) write(p * kRun + t * 8, v[p]);
@@ -238,10 +239,47 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_linear_tile(ProductArgs a) {
 
 constexpr int kRowChannels = 64;
 
-// MT x 16 rows at most, 64 channels per block
-template <int MT>
-__global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a) {
+// Rows quantised inside k_linear_rows: a wave per row, 512 values at a time, read a second time (L2) for the rounding
+constexpr int kFusedRow = 1024, kFusedValues = 4096;  // longest row, all rows together
+template <class T>
+__device__ __forceinline__ void quantize_in_block(const QuantArgs& a, char* q, int pitch, float* scale) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int end = (a.cols + 15) / 16 * 16;
+  for (int r = wave; r < (int)a.rows; r += 4) {
+    const T* row = static_cast<const T*>(a.x) + r * a.ld;
+    float v[2][8];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      load8<T>(row, p * 512 + lane * 8, a.cols, a.vec, v[p]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[p][i]) & 0x7fffffffu);
+    }
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+    const float s = __fdiv_rn(__uint_as_float(mx), 127.0f), inv = 1.0f / s;
+    if (lane == 0) scale[r] = s;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if (p * 512 + lane * 8 < end) *reinterpret_cast<uint2*>(q + r * pitch + p * 512 + lane * 8) = quantize8(v[p], s, inv, mx < 0x7f800000u, s < 1e-30f);
+  }
+}
+
+// MT x 16 rows at most, 64 channels per block.  FUSED: the rows are quantised here, by every block for itself, instead of in a launch
+// of their own (1 x 1000 x 256: 14 us a call against 16, host included).
+template <int MT, bool FUSED>
+__global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a, QuantArgs x_in, int x_bf16) {
   __shared__ int part[4][4][MT * 4 * 64];  // [wave][channel tile][MT x 4 accumulators x lane]
+  __shared__ __attribute__((aligned(16))) char fused_q[FUSED ? kFusedValues + 16 * 32 : 16];
+  __shared__ float fused_scale[16];
+  if constexpr (FUSED) {
+    const int pitch = (a.K + 15) / 16 * 16 + 16;
+    if (x_bf16) quantize_in_block<uint16_t>(x_in, fused_q, pitch, fused_scale);
+    else quantize_in_block<float>(x_in, fused_q, pitch, fused_scale);
+    __syncthreads();
+    a.ldx = pitch;
+  }
+  const int8_t* xbase = FUSED ? reinterpret_cast<const int8_t*>(fused_q) : a.x;
+  const float* xscale = FUSED ? fused_scale : a.xs;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * kRowChannels;
@@ -254,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) wp[j] = a.w + (int64_t)min(n0 + 16 * j + r, a.N - 1) * a.ldw;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xp[i] = a.x + min<int64_t>(16 * i + r, a.M - 1) * a.ldx;
+  for (int i = 0; i < MT; ++i) xp[i] = xbase + min<int64_t>(16 * i + r, a.M - 1) * a.ldx;
   i32x4 acc[MT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -303,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_rows(ProductArgs a) {
   for (int i = 0; i < MT; ++i) {
     const int64_t m = 16 * i + r;
     if (m >= a.M) continue;
-    const float sx = a.xs[m];
+    const float sx = xscale[m];
     float v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -350,6 +388,10 @@ void launch_quantize(QuantArgs a, hipStream_t s) {
   }
 }
 
+int vec_rows(const void* x, int32_t dtype, int64_t ld) {
+  return (ld * (dtype == SUAVE_DTYPE_BF16 ? 2 : 4)) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 int check_call(const suave_linear_quantized_t* h) {
@@ -378,8 +420,7 @@ int launch_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t col
   SUAVE_REQUIRE(x && q && scale, "quantize_rows: x / q / scale is null");
   SUAVE_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0, "quantize_rows: q must be 16-byte aligned");
   QuantArgs a{x, ld_x, rows, cols, q, ld_q, scale, 0};
-  const int es = dtype == SUAVE_DTYPE_BF16 ? 2 : 4;
-  a.vec = (ld_x * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  a.vec = vec_rows(x, dtype, ld_x);
   if (dtype == SUAVE_DTYPE_BF16) launch_quantize<uint16_t>(a, s);
   else launch_quantize<float>(a, s);
   SUAVE_CHECK_HIP(hipGetLastError());
@@ -404,7 +445,6 @@ int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
   const int ldq = round_up(h->n_in, 16);
   int8_t* q = static_cast<int8_t*>(h->workspace);
   float* xs = reinterpret_cast<float*>(q + up256((size_t)h->n_rows * ldq));
-  if (int rc = launch_quantize_rows(h->x, h->dtype, h->n_rows, h->n_in, h->ld_x, q, ldq, xs, s)) return rc;
   ProductArgs a{};
   a.x = q; a.ldx = ldq; a.xs = xs; a.w = h->weight; a.ldw = h->ld_weight; a.ws = h->weight_scale; a.bias = h->bias;
   a.M = h->n_rows; a.N = h->n_out; a.K = h->n_in; a.out = h->out; a.ld_out = h->ld_out; a.bf16 = h->dtype == SUAVE_DTYPE_BF16;
@@ -416,11 +456,18 @@ int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
   // us against 74 by k_linear_rows, 64 x 100000 x 1000: 38 against 54); with fewer, blocks of 64 channels and K over the waves
   // (1 x 5000 x 4096: 21 us against 29).
   const bool many = (a.N + 255) / 256 >= 128;
+  if (a.M <= 16 && !many && a.K <= kFusedRow && a.M * a.K <= kFusedValues) {
+    QuantArgs x{h->x, h->ld_x, a.M, a.K, nullptr, 0, nullptr, vec_rows(h->x, h->dtype, h->ld_x)};
+    hipLaunchKernelGGL((k_linear_rows<1, true>), dim3(blocks), dim3(256), 0, s, a, x, a.bf16);
+    SUAVE_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
+  if (int rc = launch_quantize_rows(h->x, h->dtype, h->n_rows, h->n_in, h->ld_x, q, ldq, xs, s)) return rc;
   if (a.M <= 16 && many) return launch_tile<Tile<kI8, 1, false, false, 16, 256, 1, 4>>(a, s);
   if (a.M <= 64 && many) return launch_tile<Tile<kI8, 1, false, false, 64, 256, 1, 4>>(a, s);
-  if (a.M <= 16) hipLaunchKernelGGL(k_linear_rows<1>, dim3(blocks), dim3(256), 0, s, a);
-  else if (a.M <= 32) hipLaunchKernelGGL(k_linear_rows<2>, dim3(blocks), dim3(256), 0, s, a);
-  else if (a.M <= 64) hipLaunchKernelGGL(k_linear_rows<4>, dim3(blocks), dim3(256), 0, s, a);
+  if (a.M <= 16) hipLaunchKernelGGL((k_linear_rows<1, false>), dim3(blocks), dim3(256), 0, s, a, QuantArgs{}, 0);
+  else if (a.M <= 32) hipLaunchKernelGGL((k_linear_rows<2, false>), dim3(blocks), dim3(256), 0, s, a, QuantArgs{}, 0);
+  else if (a.M <= 64) hipLaunchKernelGGL((k_linear_rows<4, false>), dim3(blocks), dim3(256), 0, s, a, QuantArgs{}, 0);
   else {
     // the tile with the smallest estimated time
     int best = kT64;
