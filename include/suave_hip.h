@@ -314,7 +314,7 @@ typedef struct suave_linear_ce_t {
 int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes);
 int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
 
-/* 8-bit rows with one scale each: scale[r] = max |x_r| / 127 (binary32), q[r, k] = x[r, k] / scale[r] rounded to the
+/* 8-bit rows with one scale each: scale[r] = max |x_r| (1/127) in binary32, q[r, k] = x[r, k] / scale[r] rounded to the
  * nearest integer, ties to even, exactly.  A row of zeros has scale 0; a row with an infinity or a NaN has a non-finite
  * scale and q = 0.  q: 16-byte aligned, ld_q a multiple of 16; the bytes of a row from cols to the next multiple of 16
  * are written as zero.  Strides in elements. */

@@ -1,9 +1,10 @@
 // Matrix product in 8-bit integers with a scale per row of either operand (per token and per output channel): the serving
 // form of a linear layer.
 //
-//   s_r = max_k |x_rk| / 127     q_rk = rint(x_rk / s_r)     out_rn = s_r w_n sum_k q_rk Q_nk + b_n
+//   s_r = max_k |x_rk| (1/127)   q_rk = rint(x_rk / s_r)     out_rn = s_r w_n sum_k q_rk Q_nk + b_n
 //
-// k_quantize_rows writes q and s.  The scale is the correctly rounded binary32 quotient and q the exact nearest integer of
+// k_quantize_rows writes q and s.  The scale is the binary32 product with the binary32 1/127 -- what torch makes of amax / 127.0 on
+// the device, so scales laid out with it agree in every bit -- and q the exact nearest integer of
 // x / s (ties to even): the quotient by the reciprocal decides except next to a half-integer, where the sign of the exactly
 // rounded x - (q +- 1/2) s does; so q does not depend on how the division is evaluated.  A row of zeros has scale 0, a row
 // that holds an infinity or a NaN gets that as its scale and q = 0: its outputs are NaN.
@@ -41,6 +42,7 @@ struct QuantArgs {
 // Adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits.  The quotient by the reciprocal is off
 // by at most 127 * 3 * 2^-24 < 3e-5: away from a half-integer it decides.
 constexpr float kRound = 12582912.0f;
+constexpr float kStep = 1.0f / 127.0f;
 __device__ __forceinline__ uint32_t quantize_near(float x, float inv, float& off) {
   const float t = fmaf(x, inv, kRound);
   off = fmaxf(off, fabsf(fmaf(x, inv, kRound - t)));
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
     for (int i = 0; i < W; ++i) mx = max(mx, part[w0 + i]);
   }
   if (!in) return;
-  const float s = __fdiv_rn(__uint_as_float(mx), 127.0f);
+  const float s = __uint_as_float(mx) * kStep;
   if (t == 0) a.scale[r] = s;
   const bool finite = mx < 0x7f800000u, tiny = s < 1e-30f;
   const float inv = 1.0f / s;
@@ -256,7 +258,7 @@ __device__ __forceinline__ void quantize_in_block(const QuantArgs& a, char* q, i
       for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[p][i]) & 0x7fffffffu);
     }
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
-    const float s = __fdiv_rn(__uint_as_float(mx), 127.0f), inv = 1.0f / s;
+    const float s = __uint_as_float(mx) * kStep, inv = 1.0f / s;
     if (lane == 0) scale[r] = s;
 #pragma unroll
     for (int p = 0; p < 2; ++p)

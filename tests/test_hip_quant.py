@@ -17,7 +17,7 @@ def _quantized(x):
     """(q, scale) of the definition, int64 / float32, on the host in float64."""
     x = x.double().cpu().numpy()
     with np.errstate(all="ignore"):
-        s = (np.abs(x).max(axis=1).astype(np.float32) / np.float32(127)).astype(np.float32)
+        s = (np.abs(x).max(axis=1).astype(np.float32) * (np.float32(1) / np.float32(127))).astype(np.float32)
         ok = np.isfinite(s) & (s > 0)
         q = np.where(ok[:, None], np.rint(x / np.where(ok, s, 1).astype(np.float64)[:, None]), 0.0)
     return np.clip(q, -127, 127).astype(np.int64), s
@@ -45,7 +45,7 @@ def test_borders_ties_and_odd_rows():
 
     rows = []
     for amax in (127.0, 1.0, 3.0, 0.37, 1e30, 1e-30, 1e-38, 1e-42, 3e-45):
-        s = np.float32(np.float32(amax) / np.float32(127))
+        s = np.float32(np.float32(amax) * (np.float32(1) / np.float32(127)))
         half = (np.arange(-127, 127) + 0.5) * np.float64(s)
         v = half.astype(np.float32)
         rows.append(np.concatenate([[amax], v, np.nextafter(v, np.float32(1e38)), np.nextafter(v, np.float32(-1e38))]).astype(np.float32))
@@ -177,3 +177,26 @@ def test_other_stream_and_captured_graph():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, ops.linear_quantized(x, w, ws))
+
+
+def test_many_rows_against_torch_on_the_device():
+    """Scales and integers as torch gives them on the device (amax / 127.0, the quotient decided in 64 bits), over enough rows that
+    quotients fall next to half-integers."""
+    import torch
+    from suave_amd import operators as ops
+
+    g = torch.Generator(device="cuda:0").manual_seed(11)
+    for dt in (torch.float32, torch.bfloat16):
+        x = torch.randn((3000, 1000), generator=g, device="cuda:0").to(dt)
+        q, s = ops.quantize_rows(x)
+        ts = x.float().abs().amax(dim=1) / 127.0
+        assert torch.equal(s, ts)
+        assert torch.equal(q.double(), torch.round(x.double() / ts.double()[:, None]))
+    # the same rows a few at a time, where the product quantises them itself
+    x = torch.randn((16, 250), generator=g, device="cuda:0")
+    one = torch.eye(250, device="cuda:0").mul(127).to(torch.int8)
+    w = torch.zeros((250, 256), dtype=torch.int8, device="cuda:0")
+    w[:, :250] = one
+    ts = x.abs().amax(dim=1) / 127.0
+    got = ops.linear_quantized(x, w[:, :250], torch.ones(250, device="cuda:0"))
+    assert torch.equal(got, torch.round(x.double() / ts.double()[:, None]).float() * 127 * ts[:, None])
