@@ -3,15 +3,18 @@
 //   l_ic = x_i . W_c + b_c      lse_i = log sum_c exp l_ic      ce_i = w[y_i] (lse_i - l_i,y_i)      loss = sum ce / sum w[y]
 //   G_ic = s w[y_i] / sum w (exp(l_ic - lse_i) - [c = y_i])     dx = G W       dW = G^T x            db = sum_i G_i
 //
-// Two sweeps over the classes.  The first computes logit tiles on the matrix pipe and keeps of each 64-class strip of a row
+// In general two sweeps over the classes.  The first computes logit tiles on the matrix pipe and keeps of each 64-class strip of a row
 // its maximum and its sum of exponentials (8 bytes for 64 logits) and the target's logit; the strips of a row are then joined.
 // The second computes the tiles again, now against the known lse, and writes G for one piece of the classes at a time (bounded
 // scratch), which two products turn into dx (summed over the pieces in fp32) and dW.  8 n C D flops instead of 6: the price of
 // not keeping the logits.
 //
-// bf16 operands are multiplied as they are, G is rounded to bf16 for its two products (relative 2^-9 of each entry, below the
-// rounding of the bf16 results); db and every sum stay fp32.  fp32 operands are scaled by a power of two per tensor, cut into
-// two fp16 planes once per call (mma.h), G likewise: binary32's own accuracy on the fp16 pipe.
+// fp32 operands are scaled by a power of two per tensor, cut into two fp16 planes once per call (mma.h), G likewise: binary32's own
+// accuracy on the fp16 pipe.  bf16 operands are multiplied as they are and G is rounded to bf16 for its two products: relative
+// 2^-9 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
+// anything, and where a class has one row their rounding is as large as the result's own; then the operands are copied
+// into one fp16 plane (exact for bf16 values down to 2^-28 of the tensor's largest), and G rounded to fp16 (2^-12): 3 passes over W
+// more (4096 x 32000 x 1024: 1081 us against 1020; 33 x 100000 x 2048: 747 against 471).  db and every sum stay fp32.
 //
 // Rows with a negative target are left out whatever they hold (x is copied with those rows zero); a target >= C makes its row's
 // loss NaN, and with it the mean and the gradients.  No atomics: partial sums are written out and added in a fixed order.
@@ -35,13 +38,20 @@ constexpr int64_t kScanElems = 65536;  // x and W together: up to here every pac
 constexpr size_t kPieceBytes = (size_t)192 << 20;  // G of one piece: what the 256 MB memory-side cache holds beside its operands
 
 struct Scalars {
-  float x_scale, w_scale;    // powers of two the planes were multiplied by (1 for bf16)
+  float x_scale, w_scale;    // powers of two the fp16 operands were multiplied by (1 for bf16 ones)
   float g_unit;              // loss_scale * max_w / total / g_scale: what one unit of the stored G is worth
-  float max_w;               // largest |class weight| (1 for bf16 and without class weights): G is stored relative to it
+  float max_w;               // largest |class weight| (1 without gradients and without class weights): G is stored relative to it
 };
 
-// G is stored relative to the largest row weight (entries in [-1, 1]) times 2^14: fp16's hi plane is normal down to 2^-28
-__host__ __device__ constexpr float g_scale(bool planes) { return planes ? 16384.0f : 1.0f; }
+// G is stored relative to the largest row weight (entries in [-1, 1]), in fp16 times 2^14: normal down to 2^-28
+__host__ __device__ constexpr float g_scale(int type) { return type == kF16 ? 16384.0f : 1.0f; }
+// a value in one plane, or two
+template <int TYPE, int NP>
+__device__ __forceinline__ void g_bits(float v, uint16_t& hi, uint16_t& lo) {
+  if constexpr (NP == 2) planes(v, hi, lo);
+  else if constexpr (TYPE == kF16) hi = f16_bits((_Float16)v);
+  else hi = bf16_bits(v);
+}
 
 struct PackArgs {
   const void* src[2];        // x, W
@@ -65,31 +75,34 @@ __device__ __forceinline__ int64_t row_of(int64_t chunk, int64_t chunks, int q) 
   return chunks <= 0xffffffffll ? (int64_t)((uint32_t)chunk / (uint32_t)q) : chunk / q;
 }
 
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(uint16_t v) { return bf16_value(v); }
 __device__ __forceinline__ float finite_abs(float v) {
   v = fabsf(v);
   return v < INFINITY ? v : 0.f;  // (a NaN compares false)
 }
 
 // largest finite |value| of x (rows that count) or W: the share of thread `first` of `step`, in chunks of eight
+template <class T>
 __device__ __forceinline__ float scan_rows(const PackArgs& a, int t, int64_t first, int64_t step) {
-  const float* src = static_cast<const float*>(a.src[t]);
+  const T* src = static_cast<const T*>(a.src[t]);
   const int64_t ld = a.ld[t];
   const int q = (a.D + 7) / 8;
   const int64_t chunks = a.rows[t] * q;
   float m = 0.f;
   constexpr int U = 4;  // chunks in flight
   for (int64_t e0 = first; e0 < chunks; e0 += U * step) {
-    float v[U][8];
+    T v[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+      for (int i = 0; i < 8; ++i) v[u][i] = (T)0;
       const int64_t e = e0 + u * step;
       if (e >= chunks) continue;
       const int64_t r = row_of(e, chunks, q);
       const int d0 = (int)(e - r * q) * 8;
       if (t == 0 && a.targets[r] < 0) continue;
-      const float* p = src + r * ld;
+      const T* p = src + r * ld;
       if (a.D >= 8) load8(p + min(d0, a.D - 8), v[u]);  // (the last chunk may repeat some of the one before)
       else
         for (int i = 0; i < a.D; ++i) v[u][i] = p[i];
@@ -97,7 +110,7 @@ __device__ __forceinline__ float scan_rows(const PackArgs& a, int t, int64_t fir
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[u][i]));
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(as_float(v[u][i])));
   }
   return m;
 }
@@ -109,11 +122,12 @@ __device__ __forceinline__ float block_max(float m, float* part) {  // 256 threa
   return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
+template <class T>
 __global__ __launch_bounds__(256) void k_lce_amax(PackArgs a) {
   __shared__ float part[4];
   const int t = (int)blockIdx.x >= kAmaxBlocks, b = blockIdx.x - t * kAmaxBlocks;
   const int64_t first = (int64_t)b * 256 + threadIdx.x, step = (int64_t)kAmaxBlocks * 256;
-  const float m = block_max(scan_rows(a, t, first, step), part);
+  const float m = block_max(scan_rows<T>(a, t, first, step), part);
   if (threadIdx.x == 0) a.amax[blockIdx.x] = m;
   if (t == 0) {
     float w = 0.f;
@@ -132,16 +146,17 @@ __device__ __forceinline__ float plane_scale(float amax) {
   return ldexpf(1.0f, min(14 - e, 120));
 }
 
-template <class T, bool PLANES>
+// PLANES 1, 2: scaled fp16; 0: as it is
+template <class T, int PLANES>
 __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
   const int t = (int)blockIdx.x >= a.blocks0;
   const int b = blockIdx.x - (t ? a.blocks0 : 0), nb = t ? (int)gridDim.x - a.blocks0 : a.blocks0;
   float scale = 1.0f, max_w = 1.0f;
-  if constexpr (PLANES) {
+  if constexpr (PLANES > 0) {
     __shared__ float part[4];
     float m = 0.f, w = 0.f;
     if (a.scan) {
-      m = scan_rows(a, t, threadIdx.x, 256);
+      m = scan_rows<T>(a, t, threadIdx.x, 256);
       if (t == 0 && a.class_weight)
         for (int c = threadIdx.x; c < a.C; c += 256) w = fmaxf(w, finite_abs(a.class_weight[c]));
     } else {
@@ -188,12 +203,12 @@ __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
     uint16_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (PLANES) planes(v[i] * scale, hi[i], lo[i]);
+      if constexpr (PLANES > 0) g_bits<kF16, PLANES>(as_float(v[i]) * scale, hi[i], lo[i]);
       else hi[i] = v[i];
     }
     char* o = a.dst[t] + r * a.dst_ld[t] + d0 * 2;
     *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
-    if constexpr (PLANES) *reinterpret_cast<uint4*>(o + (size_t)a.Dp * 2) = *reinterpret_cast<const uint4*>(lo);
+    if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(o + (size_t)a.Dp * 2) = *reinterpret_cast<const uint4*>(lo);
   }
 }
 
@@ -326,8 +341,7 @@ __device__ __forceinline__ void write_gradients(const LogitArgs& a, const typena
       for (int u = 0; u < 4; ++u) {
         const float gv = counts ? p[j][u] * rw.y : 0.f;
         cs[j][u] += gv;
-        if constexpr (P) planes(gv * g_scale(true), hi[u], lo[u]);
-        else hi[u] = bf16_bits(gv);
+        g_bits<T::TYPE, T::NP>(gv * g_scale(T::TYPE), hi[u], lo[u]);
       }
       Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
       if constexpr (P) Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
@@ -448,12 +462,12 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
       s += __shfl_xor(s, 32, 64);
       if constexpr (SWEEP == 3) {
         typedef RowStage<uint16_t, kStrip> Rows;
-        char* stage = lds + kTabs + wave * (2 * Rows::kBytes);
+        char* stage = lds + kTabs + wave * (T::NP * Rows::kBytes);
 #pragma unroll
         for (int j = 0; j < T::NI; ++j) {
           uint16_t hi[4], lo[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) planes(v[j][u] * g_scale(true), hi[u], lo[u]);
+          for (int u = 0; u < 4; ++u) planes(v[j][u] * g_scale(kF16), hi[u], lo[u]);
           Rows::put(stage, lane & 15, 16 * j + 4 * g, hi);
           Rows::put(stage + Rows::kBytes, lane & 15, 16 * j + 4 * g, lo);
         }
@@ -572,7 +586,7 @@ __global__ __launch_bounds__(256) void k_lce_scale(ScaleArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float v = ((float)__builtin_bit_cast(_Float16, ph[i]) + (float)__builtin_bit_cast(_Float16, pl[i])) * f;
-        if (i == at) v = (__expf(tl[u] - rw[u].x) - 1.0f) * (rw[u].y * g_scale(true));
+        if (i == at) v = (__expf(tl[u] - rw[u].x) - 1.0f) * (rw[u].y * g_scale(kF16));
         if (zero) v = i == at && rw[u].y != 0.f ? v : 0.f;
         cs[i] += v;
         planes(v, oh[i], ol[i]);
@@ -589,7 +603,7 @@ __global__ __launch_bounds__(256) void k_lce_scale(ScaleArgs a) {
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
-  a.db[rb * a.db_ld + (c - cl * 8) + threadIdx.x] = s * (1.0f / g_scale(true));
+  a.db[rb * a.db_ld + (c - cl * 8) + threadIdx.x] = s * (1.0f / g_scale(kF16));
 }
 
 // lse of R rows per block (1024 threads: R rows x 1024 / R strip groups), their loss terms and weights: 16 rows, or 4 for batches that
@@ -853,7 +867,7 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.n_strips = (int)ceil_div(h.n_classes, kStrip);
   L.ldp = (int64_t)L.Dp * 2 * np;
   L.plane = (uint32_t)(L.Dp * 2);
-  L.pack_w = f32 || h.dim % 8 != 0 || h.ld_weight % 8 != 0 || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+  L.pack_w = f32 || (grad && h.class_weight) || h.dim % 8 != 0 || h.ld_weight % 8 != 0 || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
   const int64_t per_class = n * 2 * np;
   // (at most 2^20 classes: 256 rows of a piece lie within the 2^31 bytes a tile addresses)
   const int64_t piece = std::min<int64_t>(1 << 20, std::max<int64_t>(kClassPad, (int64_t)(kPieceBytes / per_class) / kClassPad * kClassPad));
@@ -870,8 +884,8 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.dw_direct = L.dw_splits == 1 && !L.whole;  // (in one sweep the unit of G is not known before the gradients' launch ends)
   L.tile_s = L.whole ? whole_tile(n) : logit_tile(n, h.n_classes);
   L.tile_g = L.whole ? L.tile_s : logit_tile(n, cp);
-  // (pays where the second product costs more than the pass over G: 1777 x 20011 x 501: 493 us against 576, 4096 x 1000 x 256: 82 against
-  // 81, 4096 x 1000 x 16: 64 against 57)
+  // (pays where the second product costs more than the pass over G: fp32 1777 x 20011 x 501: 493 us against 576, 4096 x 1000 x 256: 82
+  // against 81, 4096 x 1000 x 16: 64 against 57.  Two planes only: db is summed from what is kept)
   L.keep = f32 && grad && L.pieces == 1 && !L.whole && h.dim >= 256;
   L.db_rows = L.keep ? (int)ceil_div(n, kScaleRows) : (int)ceil_div(n, kLogitM[L.tile_g]) * kLogitWM[L.tile_g];
   L.row_blocks = (int)ceil_div(n, L.whole ? kLogitM[L.tile_s] : rows_per_block(n));
@@ -965,78 +979,18 @@ int launch_grads(const GradArgs& dx, const GradArgs& dw, TileId tile, int totals
   }
 }
 
+// What follows the statistics where gradients are wanted: G piece by piece, its two products, the results
 template <int TYPE, int NP>
-int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
-  constexpr bool F = NP == 2;
-  const bool grad = h.dx || h.dweight || h.dbias;
+int run_gradients(const suave_linear_ce_t& h, const Layout& L, LogitArgs& a, bool products, hipStream_t s) {
+  const bool bf = h.dtype == SUAVE_DTYPE_BF16;
   const int64_t n = h.n_rows;
   char* ws = static_cast<char*>(h.workspace);
-  Scalars* scal = reinterpret_cast<Scalars*>(ws + L.scal);
-  PackArgs p{};
-  p.src[0] = h.x; p.src[1] = h.weight; p.ld[0] = h.ld_x; p.ld[1] = h.ld_weight; p.rows[0] = n; p.rows[1] = h.n_classes;
-  p.dst[0] = ws + L.xp; p.dst[1] = L.pack_w ? ws + L.wp : nullptr; p.dst_ld[0] = p.dst_ld[1] = L.ldp;
-  p.D = h.dim; p.Dp = L.Dp; p.targets = h.targets; p.amax = reinterpret_cast<float*>(ws + L.amax); p.scal = scal;
-  p.class_weight = F ? h.class_weight : nullptr;
-  p.scan = (n + h.n_classes) * h.dim <= kScanElems;
-  p.bias = h.bias; p.bias_pad = reinterpret_cast<float*>(ws + L.bias); p.C = h.n_classes; p.C_pad = L.C_pad;
-  if (F && !p.scan) {
-    hipLaunchKernelGGL(k_lce_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, s, p);
-    SUAVE_CHECK_HIP(hipGetLastError());
-  }
-  p.blocks0 = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(n * (L.Dp / 8), 256), 1024));
-  const int64_t wblocks = L.pack_w ? ceil_div((int64_t)h.n_classes * (L.Dp / 8), 256) : ceil_div(L.C_pad, 256);
-  const int grid = p.blocks0 + (int)std::max<int64_t>(1, std::min<int64_t>(wblocks, 4096));
-  if (F) hipLaunchKernelGGL((k_lce_pack<float, true>), dim3(grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_lce_pack<uint16_t, false>), dim3(grid), dim3(256), 0, s, p);
-  SUAVE_CHECK_HIP(hipGetLastError());
-
-  LogitArgs a{};
-  a.x = ws + L.xp; a.ldx = L.ldp;
-  a.w = L.pack_w ? ws + L.wp : static_cast<const char*>(h.weight);
-  a.ldw = L.pack_w ? L.ldp : h.ld_weight * 2;
-  a.plane = L.plane; a.n = n; a.C = h.n_classes; a.D = h.dim; a.c0 = 0; a.c1 = h.n_classes; a.scal = scal;
-  a.bias = p.bias_pad; a.targets = h.targets;
-  a.strips = reinterpret_cast<float2*>(ws + L.strips);
-  a.target_logit = reinterpret_cast<float*>(ws + L.target);
-  a.row = reinterpret_cast<const float2*>(ws + L.row);
-
-  RowArgs& r = a.rows;
-  r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
-  r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
-  r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part); r.scal = scal;
-  a.total = TotalArgs{r.part, L.row_blocks, h.weight_sum, h.loss_scale, h.loss_rows, g_scale(F), h.loss, h.loss_sum, scal};
-  a.db_ld = L.C_pad;
-  a.ldg = L.ldg; a.g_plane = L.g_plane;
-  if (grad) {
-    a.g = ws + L.g;
-    a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
-  }
-  const bool products = h.dx || h.dweight;
-  if (L.whole) {
-    if (int rc = launch_whole<TYPE, NP>(a, L.tile_s, s)) return rc;
-  } else {
-    if constexpr (F) {
-      if (int rc = L.keep ? launch_logits<TYPE, NP, 3>(a, L.tile_s, s) : launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
-    } else {
-      if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
-    }
-    if (rows_per_block(n) == 4) hipLaunchKernelGGL(k_lce_rows<4>, dim3(L.row_blocks), dim3(1024), 0, s, r);
-    else hipLaunchKernelGGL(k_lce_rows<16>, dim3(L.row_blocks), dim3(1024), 0, s, r);
-    SUAVE_CHECK_HIP(hipGetLastError());
-  }
-  if (!grad || (L.whole && !products)) {
-    hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(256), 0, s, a.total);
-    SUAVE_CHECK_HIP(hipGetLastError());
-    if (!grad) return 0;
-  }
-
+  const Scalars* scal = a.scal;
   if (L.keep) {
     const ScaleArgs k{a.g, L.ldg, L.g_plane, n, L.n_strips, L.C_pad / 256, a.strips, a.row, a.target_logit, h.targets, a.db, a.db_ld, a.total};
     hipLaunchKernelGGL(k_lce_scale, dim3((unsigned)(1 + ceil_div(n, kScaleRows) * k.groups)), dim3(256), 0, s, k);
     SUAVE_CHECK_HIP(hipGetLastError());
   }
-
-  const bool bf = !F;
   auto vec_ok = [&](const void* ptr, int64_t ld) {
     return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) & (bf ? 7 : 15)) == 0;
   };
@@ -1072,7 +1026,7 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
       if (int rc = launch_grads<TYPE, NP>(gx, gw, L.grad_tile, L.whole, a.total, s)) return rc;
   }
   FinishArgs f{};
-  f.scal = scal; f.out_bf16 = bf; f.ld_slab = L.Dp; f.N = h.dim; f.gs = g_scale(F);
+  f.scal = scal; f.out_bf16 = bf; f.ld_slab = L.Dp; f.N = h.dim; f.gs = g_scale(TYPE);
   int blocks = 0;
   if (h.dx) {
     f.slab[0] = reinterpret_cast<float*>(ws + L.dx_slab); f.n_slabs[0] = L.dx_splits; f.slab_stride[0] = n * L.Dp; f.rows[0] = n;
@@ -1095,6 +1049,77 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
     SUAVE_CHECK_HIP(hipGetLastError());
   }
   return 0;
+}
+
+
+template <int TYPE, int NP>
+int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
+  constexpr bool F = TYPE == kF16;  // scaled fp16
+  const bool bf = h.dtype == SUAVE_DTYPE_BF16;
+  const bool grad = h.dx || h.dweight || h.dbias;
+  const int64_t n = h.n_rows;
+  char* ws = static_cast<char*>(h.workspace);
+  Scalars* scal = reinterpret_cast<Scalars*>(ws + L.scal);
+  PackArgs p{};
+  p.src[0] = h.x; p.src[1] = h.weight; p.ld[0] = h.ld_x; p.ld[1] = h.ld_weight; p.rows[0] = n; p.rows[1] = h.n_classes;
+  p.dst[0] = ws + L.xp; p.dst[1] = L.pack_w ? ws + L.wp : nullptr; p.dst_ld[0] = p.dst_ld[1] = L.ldp;
+  p.D = h.dim; p.Dp = L.Dp; p.targets = h.targets; p.amax = reinterpret_cast<float*>(ws + L.amax); p.scal = scal;
+  p.class_weight = F ? h.class_weight : nullptr;
+  p.scan = (n + h.n_classes) * h.dim <= kScanElems;
+  p.bias = h.bias; p.bias_pad = reinterpret_cast<float*>(ws + L.bias); p.C = h.n_classes; p.C_pad = L.C_pad;
+  if (F && !p.scan) {
+    if (bf) hipLaunchKernelGGL(k_lce_amax<uint16_t>, dim3(2 * kAmaxBlocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(k_lce_amax<float>, dim3(2 * kAmaxBlocks), dim3(256), 0, s, p);
+    SUAVE_CHECK_HIP(hipGetLastError());
+  }
+  p.blocks0 = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(n * (L.Dp / 8), 256), 1024));
+  const int64_t wblocks = L.pack_w ? ceil_div((int64_t)h.n_classes * (L.Dp / 8), 256) : ceil_div(L.C_pad, 256);
+  const int grid = p.blocks0 + (int)std::max<int64_t>(1, std::min<int64_t>(wblocks, 4096));
+  if (NP == 2) hipLaunchKernelGGL((k_lce_pack<float, 2>), dim3(grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((k_lce_pack<uint16_t, F ? 1 : 0>), dim3(grid), dim3(256), 0, s, p);
+  SUAVE_CHECK_HIP(hipGetLastError());
+
+  LogitArgs a{};
+  a.x = ws + L.xp; a.ldx = L.ldp;
+  a.w = L.pack_w ? ws + L.wp : static_cast<const char*>(h.weight);
+  a.ldw = L.pack_w ? L.ldp : h.ld_weight * 2;
+  a.plane = L.plane; a.n = n; a.C = h.n_classes; a.D = h.dim; a.c0 = 0; a.c1 = h.n_classes; a.scal = scal;
+  a.bias = p.bias_pad; a.targets = h.targets;
+  a.strips = reinterpret_cast<float2*>(ws + L.strips);
+  a.target_logit = reinterpret_cast<float*>(ws + L.target);
+  a.row = reinterpret_cast<const float2*>(ws + L.row);
+
+  RowArgs& r = a.rows;
+  r.strips = a.strips; r.n_strips = L.n_strips; r.n = n; r.targets = h.targets; r.C = h.n_classes;
+  r.class_weight = h.class_weight; r.target_logit = a.target_logit; r.row_loss = h.row_loss; r.lse_out = h.lse;
+  r.row = reinterpret_cast<float2*>(ws + L.row); r.part = reinterpret_cast<double*>(ws + L.part); r.scal = scal;
+  a.total = TotalArgs{r.part, L.row_blocks, h.weight_sum, h.loss_scale, h.loss_rows, g_scale(TYPE), h.loss, h.loss_sum, scal};
+  a.db_ld = L.C_pad;
+  a.ldg = L.ldg; a.g_plane = L.g_plane;
+  if (grad) {
+    a.g = ws + L.g;
+    a.db = h.dbias ? reinterpret_cast<float*>(ws + L.db) : nullptr;
+  }
+  const bool products = h.dx || h.dweight;
+  if (L.whole) {
+    if (int rc = launch_whole<TYPE, NP>(a, L.tile_s, s)) return rc;
+  } else {
+    if constexpr (NP == 2) {
+      if (int rc = L.keep ? launch_logits<TYPE, NP, 3>(a, L.tile_s, s) : launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    } else {
+      if (int rc = launch_logits<TYPE, NP, 0>(a, L.tile_s, s)) return rc;
+    }
+    if (rows_per_block(n) == 4) hipLaunchKernelGGL(k_lce_rows<4>, dim3(L.row_blocks), dim3(1024), 0, s, r);
+    else hipLaunchKernelGGL(k_lce_rows<16>, dim3(L.row_blocks), dim3(1024), 0, s, r);
+    SUAVE_CHECK_HIP(hipGetLastError());
+  }
+  if (!grad || (L.whole && !products)) {
+    hipLaunchKernelGGL(k_lce_total, dim3(1), dim3(256), 0, s, a.total);
+    SUAVE_CHECK_HIP(hipGetLastError());
+    if (!grad) return 0;
+  }
+
+  return run_gradients<TYPE, NP>(h, L, a, products, s);
 }
 
 }  // namespace
@@ -1139,7 +1164,9 @@ int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s) {
   make_layout(*h, L);
   SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_ce: workspace is null or not 256-byte aligned");
   SUAVE_REQUIRE(h->workspace_bytes >= L.total, "linear_ce: workspace too small (suave_linear_ce_workspace_bytes)");
-  return h->dtype == SUAVE_DTYPE_F32 ? run_linear_ce<kF16, 2>(*h, L, s) : run_linear_ce<kBf16, 1>(*h, L, s);
+  if (h->dtype == SUAVE_DTYPE_F32) return run_linear_ce<kF16, 2>(*h, L, s);
+  const bool grad = h->dx || h->dweight || h->dbias;
+  return grad && h->class_weight ? run_linear_ce<kF16, 1>(*h, L, s) : run_linear_ce<kBf16, 1>(*h, L, s);
 }
 
 }  // namespace suave
