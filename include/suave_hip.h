@@ -350,8 +350,9 @@ int suave_linear_quantized(const suave_linear_quantized_t* call, void* stream);
  * X <- (a I + b A + c A A) X with A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315), on the shorter side; after five steps
  * the singular values of the result lie in about 0.7 .. 1.2 where U's were not negligible.  All matrices of the list go
  * through the same launches.  in / out have the type dtype and may be the same matrix, otherwise they must not overlap;
- * rows contiguous, strides in elements.  F32: binary32-grade products; BF16: fp16 products with fp32 sums.  A zero matrix
- * gives zero; an infinity or a NaN makes its whole matrix NaN.  Sides at most 32768 (short) and 2^20 (long).  The list is
+ * rows contiguous, strides in elements.  F32, and BF16 with a short side below 128: binary32-grade products; other BF16:
+ * fp16 products with fp32 sums.  A zero matrix gives zero; an infinity or a NaN makes its whole matrix NaN.  Sides at most
+ * 32768 (short) and 2^20 (long).  The list is
  * host memory and is read before the call returns.  workspace: 256-byte aligned; one call at a time uses it. */
 typedef struct suave_ortho_matrix_t {
   const void* in;

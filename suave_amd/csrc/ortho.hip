@@ -9,7 +9,7 @@
 // call go through the same launches: three per step for the whole list.
 //
 // Arithmetic (mma.h).  fp32 matrices: every factor as two fp16 planes, which keeps binary32's accuracy -- the iteration
-// multiplies small singular directions, and rounding noise in them, by up to a^5 = 485.  bf16 matrices: one fp16 plane (11 bits;
+// multiplies small singular directions, and rounding noise in them, by up to a^5 = 485.  bf16 matrices from a short side of 128 on: one fp16 plane (11 bits;
 // the result is rounded to 8): a relative error of about 1.3e-3 where the rounding of the result is 1.7e-3.  Factors are stored times a power of two:
 // X times 2^(12 - e), A times 2^(12 - 2 e), B times 2^12, with 2^e the size of X (e = 0 unless |U|_F is below eps): entries of
 // X are at most about 1.3 in magnitude, and start at 1 / sqrt(rows cols), which 2^12 keeps clear of fp16's subnormals.
@@ -754,14 +754,20 @@ size_t head_bytes() { return up256(sizeof(double) * kMaxMats * kNormBlocks) + up
 
 bool is_small(int rows, int cols, int np) { return small_shape(rows, cols, np).bytes <= kSmallLds; }
 
-// The matrices that do not fit one block go through the launches in groups of kMaxMats, one group after the other in the same
-// workspace
+// Planes of a matrix: float32 two.  bfloat16 one, an error (fp16's 2^-12 through the steps) that adds little to the result's own rounding
+// -- but on short sides it does not average out: 4 x 400 was 4 times, 96 x 39 1.6 times as far off as that rounding alone, from 128
+// on it is 1.3 times at most.  Short sides take two; they are bound by latency.
+constexpr int kOnePlaneSide = 128;
+int planes_of(int rows, int cols, bool bf16) { return bf16 && std::min(rows, cols) >= kOnePlaneSide ? 1 : 2; }
+
+// The matrices that do not fit one block go through the launches in groups of kMaxMats of the same planes, one group after the
+// other in the same workspace
 template <class F>
-size_t workspace_bytes(int n, int np, F shape) {
+size_t workspace_bytes(int n, int np, bool bf16, F shape) {
   size_t most = 0, b = 0;
   int in_group = 0;
   for (int i = 0; i < n; ++i) {
-    if (is_small(shape(i).first, shape(i).second, np)) continue;
+    if (planes_of(shape(i).first, shape(i).second, bf16) != np || is_small(shape(i).first, shape(i).second, np)) continue;
     if (in_group == kMaxMats) { b = 0; in_group = 0; }
     b += mat_bytes(shape(i).first, shape(i).second, np);
     ++in_group;
@@ -941,6 +947,7 @@ int run_list(int n, const Group& base, F fill, char* ws, hipStream_t s) {
   for (int i = 0; i < n; ++i) {
     Mat m{};
     fill(i, m);
+    if (planes_of(m.rows, m.cols, base.bf16) != NP) continue;
     const bool sm = is_small(m.rows, m.cols, NP);
     Group& g = sm ? small : large;
     g.m[g.n++] = m;
@@ -972,7 +979,9 @@ int orthogonalize_workspace(const suave_ortho_matrix_t* mats, int32_t n, int32_t
   SUAVE_REQUIRE(n >= 0 && (n == 0 || mats) && bytes, "orthogonalize: null argument");
   for (int i = 0; i < n; ++i)
     if (int rc = check_dims(mats[i].rows, mats[i].cols)) return rc;
-  *bytes = workspace_bytes(n, dtype == SUAVE_DTYPE_F32 ? 2 : 1, [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); });
+  const bool bf16 = dtype == SUAVE_DTYPE_BF16;
+  auto shape = [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); };
+  *bytes = std::max(workspace_bytes(n, 2, bf16, shape), bf16 ? workspace_bytes(n, 1, bf16, shape) : 0);
   return 0;
 }
 
@@ -991,14 +1000,15 @@ int launch_orthogonalize(const suave_ortho_matrix_t* mats, int32_t n, int32_t dt
   auto fill = [&](int i, Mat& m) {
     m.in = mats[i].in; m.out = mats[i].out; m.ld_in = mats[i].ld_in; m.ld_out = mats[i].ld_out; m.rows = mats[i].rows; m.cols = mats[i].cols;
   };
-  return base.bf16 ? run_list<1>(n, base, fill, static_cast<char*>(ws), s) : run_list<2>(n, base, fill, static_cast<char*>(ws), s);
+  if (int rc = run_list<2>(n, base, fill, static_cast<char*>(ws), s)) return rc;
+  return base.bf16 ? run_list<1>(n, base, fill, static_cast<char*>(ws), s) : 0;
 }
 
 int muon_workspace(const suave_muon_matrix_t* mats, int32_t n, size_t* bytes) {
   SUAVE_REQUIRE(n >= 0 && (n == 0 || mats) && bytes, "muon_step: null argument");
   for (int i = 0; i < n; ++i)
     if (int rc = check_dims(mats[i].rows, mats[i].cols)) return rc;
-  *bytes = workspace_bytes(n, 2, [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); });
+  *bytes = workspace_bytes(n, 2, false, [&](int i) { return std::make_pair(mats[i].rows, mats[i].cols); });
   return 0;
 }
 

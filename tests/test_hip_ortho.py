@@ -249,3 +249,18 @@ def test_other_stream_and_captured_graph():
         ops.muon_step(p2, us, m2, lr=0.05)
         assert all(torch.equal(x, y) for x, y in zip(out, ops.orthogonalize(us)))
         assert all(torch.equal(x, y) for x, y in zip(p + m, p2 + m2))
+
+
+@pytest.mark.parametrize("r,c", [(1, 5), (3, 50), (4, 400), (8, 8), (40, 500), (96, 39), (127, 300), (1000, 77)])
+def test_short_sides_in_bfloat16_are_off_by_their_rounding_alone(r, c):
+    """Up to 127 the bfloat16 iteration is binary32's: with d its error, the result is bf16(O + d), so it is off by at most
+    |bf16(O) - O| + 3 |d| (rounding moves by at most |d| where its argument does, twice, and d itself)."""
+    import torch
+    from suave_amd import operators as ops
+
+    u = _random(r, c, r + c, torch.bfloat16)
+    want = _exact(u)
+    got = ops.orthogonalize([u, _random(200, 300, 1, torch.bfloat16)])[0]
+    norm = torch.linalg.matrix_norm
+    assert float(norm(got.double() - want)) <= float(norm(want.bfloat16().double() - want)) + 3 * _tolerance(u.float(), want)
+    assert torch.equal(got, ops.orthogonalize([u])[0])
