@@ -742,6 +742,136 @@ __global__ __launch_bounds__(64 * kSmallWaves) void k_ortho_small(Group g) {
   }
 }
 
+// ---- short sides up to 16 -------------------------------------------------------------------------------------------
+// X_k = P_k X_0 with P_k = B_k .. B_1, and every B is a polynomial of A_0 = X_0 X_0^T: the whole iteration is one of s x s matrices,
+// all of which commute, and U is read once and multiplied once.  In doubles throughout: P is large where U is small (3.44^5), so
+// P U cancels.  A block per matrix, U in LDS.  Short sides are where the roundings of planes do not average out: 3 x 40 f32 is off by
+// 5e-8 here, by 1.6e-6 in two fp16 planes; 16 x 2000 f32: 57 us, against 126 by launches.  Up to 32 the s x s products take longer than the
+// matrix pipe's whole iteration (32 x 32: 54 us against 15).
+constexpr int kTinyThreads = 512, kTinySide = 16, kTinyValues = 35840;
+int tiny_pitch(int l) { return l | 1; }  // odd: the rows of a column fall on distinct banks
+bool is_tiny(int rows, int cols) {
+  const int s = std::min(rows, cols), l = std::max(rows, cols);
+  return s <= kTinySide && (int64_t)s * tiny_pitch(l) <= kTinyValues;
+}
+int tiny_lds(int s, int l) { return 4 * kTinySide * (kTinySide + 1) * 8 + s * tiny_pitch(l) * 4; }
+
+__global__ __launch_bounds__(kTinyThreads) void k_ortho_tiny(Group g) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const Mat& m = g.m[blockIdx.x];
+  constexpr int S = kTinySide;
+  constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;  // (binary32's differ by up to 2^-25: more than all the rest)
+  constexpr int W = S + 1;                 // row pitch of the s x s matrices: a column falls on distinct banks
+  constexpr int R = S / 8;                 // a wave holds the S x S sums as 8 x 8 lanes of R x R
+  constexpr int kWaves = kTinyThreads / 64;
+  const int rows = m.rows, cols = m.cols, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool tall = rows > cols;
+  const int s = tall ? cols : rows, l = tall ? rows : cols, pitch = l | 1;
+  double* A = reinterpret_cast<double*>(lds);
+  double* B = A + S * W;
+  double* P = B + S * W;
+  double* T = P + S * W;
+  float* U = reinterpret_cast<float*>(T + S * W);
+  auto at = [](int i) { return i / S * W + i % S; };  // entry i of the S x S
+  for (int i = tid; i < S * S; i += kTinyThreads) {
+    A[at(i)] = 0.0;
+    P[at(i)] = i / S == i % S ? 1.0 : 0.0;
+  }
+  // U[i][k]: i the short side; eight loads in flight per thread
+  const int total = s * l;
+  for (int e0 = tid; e0 < total; e0 += 8 * kTinyThreads) {
+    float v[8], mo[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = e0 + u * kTinyThreads, r = e / cols, c = e - r * cols;
+      v[u] = mo[u] = 0.f;
+      if (e < total) {
+        if (g.bf16) v[u] = bf16_value(static_cast<const uint16_t*>(m.in)[(int64_t)r * m.ld_in + c]);
+        else v[u] = static_cast<const float*>(m.in)[(int64_t)r * m.ld_in + c];
+        if (g.muon) mo[u] = m.mom[(int64_t)r * m.ld_mom + c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = e0 + u * kTinyThreads, r = e / cols, c = e - r * cols;
+      if (e >= total) continue;
+      if (g.muon) {
+        const float mn = fmaf(g.momentum, mo[u], v[u]);
+        m.mom[(int64_t)r * m.ld_mom + c] = mn;
+        v[u] = g.nesterov ? fmaf(g.momentum, mn, v[u]) : mn;
+      }
+      U[(tall ? c : r) * pitch + (tall ? r : c)] = v[u];
+    }
+  }
+  __syncthreads();
+  {  // U U^T: every wave its columns, then the waves' sums in their order (rows past s repeat the last one and are not used)
+    const int i0 = R * (lane >> 3), j0 = R * (lane & 7);
+    double acc[R][R];
+#pragma unroll
+    for (int a = 0; a < R; ++a)
+#pragma unroll
+      for (int b = 0; b < R; ++b) acc[a][b] = 0.0;
+    for (int k = wave; k < l; k += kWaves) {
+      double x[R], y[R];
+#pragma unroll
+      for (int a = 0; a < R; ++a) {
+        x[a] = (double)U[min(i0 + a, s - 1) * pitch + k];
+        y[a] = (double)U[min(j0 + a, s - 1) * pitch + k];
+      }
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int b = 0; b < R; ++b) acc[a][b] = fma(x[a], y[b], acc[a][b]);
+    }
+    for (int w = 0; w < kWaves; ++w) {
+      if (w == wave) {
+#pragma unroll
+        for (int a = 0; a < R; ++a)
+#pragma unroll
+          for (int b = 0; b < R; ++b)
+            if (i0 + a < s && j0 + b < s) A[(i0 + a) * W + j0 + b] += acc[a][b];
+      }
+      __syncthreads();
+    }
+  }
+  double sum = 0.0;
+  for (int i = 0; i < s; ++i) sum += A[i * W + i];
+  const double f = isfinite(sum) ? 1.0 / (sqrt(sum) + (double)g.eps) : (double)NAN;  // anything not finite: the whole result is NaN
+  __syncthreads();
+  for (int i = tid; i < S * S; i += kTinyThreads) A[at(i)] *= f * f;
+  __syncthreads();
+  // entry (i0, j0) of a product of two of them by 256 threads (the second factor is symmetric: rows of both)
+  static_assert(S * S == 256 && kTinyThreads == 512, "two products at a time");
+  const int half = tid >> 8, i0 = (tid & 255) / S, j0 = tid % S, own = i0 * W + j0;
+  auto product = [&](const double* x, const double* y) {
+    double d = 0.0;
+#pragma unroll
+    for (int k = 0; k < S; ++k) d = fma(x[i0 * W + k], y[j0 * W + k], d);
+    return d;
+  };
+  for (int step = 0; step < g.steps; ++step) {
+    if (half == 0) B[own] = fma(kC, product(A, A), kB * A[own]) + (i0 == j0 ? kA : 0.0);
+    __syncthreads();
+    const double d = product(half == 0 ? A : P, B);  // A B beside P B
+    __syncthreads();
+    (half == 0 ? T : P)[own] = d;
+    __syncthreads();
+    if (half == 0) A[own] = product(T, B);
+    __syncthreads();
+  }
+  for (int k = tid; k < l; k += kTinyThreads) {
+    double x[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) x[i] = i < s ? (double)U[i * pitch + k] * f : 0.0;
+    for (int r = 0; r < s; ++r) {
+      double y = 0.0;
+#pragma unroll
+      for (int i = 0; i < S; ++i) y = fma(P[r * W + i], x[i], y);
+      write_result(g, m, tall ? k : r, tall ? r : k, (float)y);
+    }
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -752,7 +882,7 @@ size_t mat_bytes(int rows, int cols, int np) {
 }
 size_t head_bytes() { return up256(sizeof(double) * kMaxMats * kNormBlocks) + up256(sizeof(int32_t) * kMaxMats * (kMaxSteps + 1)); }
 
-bool is_small(int rows, int cols, int np) { return small_shape(rows, cols, np).bytes <= kSmallLds; }
+bool is_small(int rows, int cols, int np) { return is_tiny(rows, cols) || small_shape(rows, cols, np).bytes <= kSmallLds; }
 
 // Planes of a matrix: float32 two.  bfloat16 one, an error (fp16's 2^-12 through the steps) that adds little to the result's own rounding
 // -- but on short sides it does not average out: 4 x 400 was 4 times, 96 x 39 1.6 times as far off as that rounding alone, from 128
@@ -929,12 +1059,18 @@ int run_group(Group& g, char* ws, hipStream_t s) {
 // `fill(i, mat)` describes matrix i; `base` holds what the matrices of the call share
 template <int NP, class F>
 int run_list(int n, const Group& base, F fill, char* ws, hipStream_t s) {
-  Group small = base, large = base;
-  small.n = large.n = 0;
-  auto flush = [&](Group& g, bool is_small_group) {
+  enum { kTiny, kSmall, kLarge, kKinds };
+  Group groups[kKinds] = {base, base, base};
+  for (Group& g : groups) g.n = 0;
+  auto flush = [&](int kind) {
+    Group& g = groups[kind];
     if (g.n == 0) return 0;
     int rc;
-    if (is_small_group) {
+    if (kind == kTiny) {
+      int lds = 0;
+      for (int i = 0; i < g.n; ++i) lds = std::max(lds, tiny_lds(std::min(g.m[i].rows, g.m[i].cols), std::max(g.m[i].rows, g.m[i].cols)));
+      rc = launch<k_ortho_tiny>(g, g.n, kTinyThreads, lds, s);
+    } else if (kind == kSmall) {
       int lds = 0;
       for (int i = 0; i < g.n; ++i) lds = std::max(lds, small_shape(g.m[i].rows, g.m[i].cols, NP).bytes);
       rc = launch<k_ortho_small<NP>>(g, g.n, 64 * kSmallWaves, lds, s);
@@ -948,14 +1084,15 @@ int run_list(int n, const Group& base, F fill, char* ws, hipStream_t s) {
     Mat m{};
     fill(i, m);
     if (planes_of(m.rows, m.cols, base.bf16) != NP) continue;
-    const bool sm = is_small(m.rows, m.cols, NP);
-    Group& g = sm ? small : large;
+    const int kind = is_tiny(m.rows, m.cols) ? kTiny : is_small(m.rows, m.cols, NP) ? kSmall : kLarge;
+    Group& g = groups[kind];
     g.m[g.n++] = m;
     if (g.n == kMaxMats)
-      if (int rc = flush(g, sm)) return rc;
+      if (int rc = flush(kind)) return rc;
   }
-  if (int rc = flush(small, true)) return rc;
-  return flush(large, false);
+  for (int kind = 0; kind < kKinds; ++kind)
+    if (int rc = flush(kind)) return rc;
+  return 0;
 }
 
 int check_dims(int32_t rows, int32_t cols) {

@@ -264,3 +264,28 @@ def test_short_sides_in_bfloat16_are_off_by_their_rounding_alone(r, c):
     norm = torch.linalg.matrix_norm
     assert float(norm(got.double() - want)) <= float(norm(want.bfloat16().double() - want)) + 3 * _tolerance(u.float(), want)
     assert torch.equal(got, ops.orthogonalize([u])[0])
+
+
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 39), (42, 1), (3, 392), (16, 16), (16, 2239), (16, 2240), (2240, 16), (7, 3000), (52, 4)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_short_sides_up_to_sixteen_are_rounded_once(r, c, dtype):
+    """Up to 16 the whole iteration is one of small matrices in doubles: the result is off by its own rounding (half a step, 2^-24 or
+    2^-8 relative), or by the general bound where the matrix is too long for that."""
+    import torch
+    from suave_amd import operators as ops
+
+    dt = getattr(torch, dtype)
+    u = _random(r, c, 7 * r + c, dt)
+    want, (got,) = _exact(u), ops.orthogonalize([u])
+    if min(r, c) * (max(r, c) | 1) <= 35840:
+        half = torch.finfo(dt).eps / 2
+        # the doubles' own errors, 2^-53 times 3.4445^5, are lost in it
+        assert bool(((got.double() - want).abs() <= half * want.abs() * (1 + 1e-6) + 1e-11).all())
+    else:
+        _check(got, u)
+    p, m = torch.zeros(r, c, device="cuda:0"), torch.zeros(r, c, device="cuda:0")
+    ops.muon_step([p], [u.float()], [m], lr=1.0, momentum=0.5, nesterov=True)
+    assert torch.equal(m, u.float())
+    s = math.sqrt(max(1.0, r / c))
+    tol = s * 2 * _tolerance((1.5 * u.double()).float(), want) + 2.0 ** -23 * s * float(torch.linalg.matrix_norm(want))
+    assert float(torch.linalg.matrix_norm(p.double() + s * want)) <= tol
