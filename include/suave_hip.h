@@ -310,8 +310,8 @@ typedef struct suave_linear_ce_t {
   void* workspace;
   size_t workspace_bytes;
 } suave_linear_ce_t;
-/* Bytes of workspace for a call with these fields (the pointers of weight and outputs count: which of them are NULL, and
- * weight's alignment; workspace itself is not looked at). */
+/* Bytes of workspace for a call with these fields (the pointers of weight, class_weight and outputs count: which of them are
+ * NULL, and weight's alignment; workspace itself is not looked at). */
 int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes);
 int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
 
