@@ -40,7 +40,7 @@ struct QuantArgs {
 };
 
 // Adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits.  The quotient by the reciprocal is off
-// by at most 127 * 3 * 2^-24 < 3e-5: away from a half-integer it decides.
+// by at most 127 * 2^-24 < 8e-6: away from a half-integer it decides.
 constexpr float kRound = 12582912.0f;
 constexpr float kStep = 1.0f / 127.0f;
 __device__ __forceinline__ uint32_t quantize_near(float x, float inv, float& off) {
@@ -52,20 +52,12 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
   return __builtin_amdgcn_perm(cd, ab, 0x05040100u);
 }
-__device__ __forceinline__ int quantize_exact(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t quantize_exact(float x, float s, float inv) {
   const float k = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
   const float up = fmaf(-(k + 0.5f), s, x), down = fmaf(-(k - 0.5f), s, x);  // signs are exact: one rounding each
-  const int ki = (int)k;
-  const int odd = ki & 1;
-  int r = ki;
-  if (up > 0.f || (up == 0.f && odd)) r = ki + 1;
-  if (down < 0.f || (down == 0.f && odd)) r = ki - 1;
-  return min(max(r, -127), 127);
-}
-// scales next to or below binary32's smallest normal number: the reciprocal or the residuals above may leave the range
-__device__ __forceinline__ int quantize_tiny(float x, float s) {
-  if (!(s > 0.f)) return 0;
-  return (int)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0);
+  const int ki = (int)k, odd = ki & 1;
+  const int r = ki + ((up > 0.f) | ((up == 0.f) & odd)) - ((down < 0.f) | ((down == 0.f) & odd));
+  return (uint32_t)min(max(r, -127), 127);
 }
 
 template <class T> __device__ __forceinline__ float as_float(T v);
@@ -89,14 +81,35 @@ __device__ __forceinline__ void load8(const T* row, int k0, int cols, int vec, f
   }
 }
 
-__device__ __forceinline__ uint2 quantize8(const float (&u)[8], float s, float inv, bool finite, bool tiny) {
+// What a row's largest |x| (bits) gives: its scale, and how its values are quantised.  Rows whose scale is next to or below binary32's
+// smallest normal number are taken 2^100 times larger, values and scale, which is exact: neither the reciprocal nor the
+// residuals leave the range then.
+struct RowScale {
+  float scale, s, inv;
+  bool tiny, none;  // none: nothing to quantise (zeros, or an infinity or a NaN among them): q = 0
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t mx) {
+  RowScale r;
+  r.scale = __uint_as_float(mx) * kStep;
+  r.tiny = r.scale < 1e-30f;
+  r.s = r.tiny ? r.scale * 0x1p100f : r.scale;
+  r.none = mx >= 0x7f800000u || r.s == 0.f;
+  r.inv = 1.0f / r.s;
+  return r;
+}
+__device__ __forceinline__ uint2 quantize8(float (&u)[8], const RowScale& r) {
+  if (r.none) return make_uint2(0, 0);
+  if (r.tiny) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] *= 0x1p100f;
+  }
   uint32_t k[8];
   float off = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], inv, off);
-  if (!finite || tiny || off > 0.4999f) {
+  for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], r.inv, off);
+  if (off > 0.49998f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(!finite ? 0 : tiny ? quantize_tiny(u[i], s) : quantize_exact(u[i], s, inv));
+    for (int i = 0; i < 8; ++i) k[i] = quantize_exact(u[i], r.s, r.inv);
   }
   return make_uint2(low_bytes(k[0], k[1], k[2], k[3]), low_bytes(k[4], k[5], k[6], k[7]));
 }
@@ -136,12 +149,10 @@ __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
     for (int i = 0; i < W; ++i) mx = max(mx, part[w0 + i]);
   }
   if (!in) return;
-  const float s = __uint_as_float(mx) * kStep;
-  if (t == 0) a.scale[r] = s;
-  const bool finite = mx < 0x7f800000u, tiny = s < 1e-30f;
-  const float inv = 1.0f / s;
+  const RowScale rs = row_scale(mx);
+  if (t == 0) a.scale[r] = rs.scale;
   const int end = (a.cols + 15) / 16 * 16;
-  auto write = [&](int k0, const float (&u)[8]) { *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = quantize8(u, s, inv, finite, tiny); };
+  auto write = [&](int k0, float (&u)[8]) { *reinterpret_cast<uint2*>(a.q + r * a.ldq + k0) = quantize8(u, rs); };
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (p * kRun + t * 8 < end) write(p * kRun + t * 8, v[p]);
@@ -258,11 +269,11 @@ __device__ __forceinline__ void quantize_in_block(const QuantArgs& a, char* q, i
       for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[p][i]) & 0x7fffffffu);
     }
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
-    const float s = __uint_as_float(mx) * kStep, inv = 1.0f / s;
-    if (lane == 0) scale[r] = s;
+    const RowScale rs = row_scale(mx);
+    if (lane == 0) scale[r] = rs.scale;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      if (p * 512 + lane * 8 < end) *reinterpret_cast<uint2*>(q + r * pitch + p * 512 + lane * 8) = quantize8(v[p], s, inv, mx < 0x7f800000u, s < 1e-30f);
+      if (p * 512 + lane * 8 < end) *reinterpret_cast<uint2*>(q + r * pitch + p * 512 + lane * 8) = quantize8(v[p], rs);
   }
 }
 
