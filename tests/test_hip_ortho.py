@@ -289,3 +289,17 @@ def test_short_sides_up_to_sixteen_are_rounded_once(r, c, dtype):
     s = math.sqrt(max(1.0, r / c))
     tol = s * 2 * _tolerance((1.5 * u.double()).float(), want) + 2.0 ** -23 * s * float(torch.linalg.matrix_norm(want))
     assert float(torch.linalg.matrix_norm(p.double() + s * want)) <= tol
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shapes", [[(1024, 4096), (4096, 1024)], [(700, 3001), (650, 2900), (2500, 690), (1000, 2000)]])
+def test_long_lists_of_large_matrices_are_each_matrix_alone(shapes, dtype):
+    """More blocks than CUs: other tiles, the same sums, so the same bits; and the definition."""
+    import torch
+    from suave_amd import operators as ops
+
+    us = [_random(r, c, 3 * r + c, getattr(torch, dtype)) for r, c in shapes]
+    together = ops.orthogonalize(us)
+    for u, got in zip(us, together):
+        assert torch.equal(got, ops.orthogonalize([u])[0])
+    _check(together[-1], us[-1])
