@@ -278,7 +278,7 @@ int suave_elbo_joint_backward(const suave_plan* plan, const float* params, const
  * hold -inf (a class that is never predicted); other non-finite inputs make what they touch non-finite.
  * F32: products of binary32 grade (two fp16 planes per operand and tensor scale; elements 2^28 times smaller than their
  * tensor's largest lose relative accuracy).  BF16: fp32 accumulation, the logit gradient rounded once: to bf16, or with
- * class weights to fp16 (the operands are then copied into fp16 with a tensor scale, as above).
+ * class weights or up to 8 rows to fp16 (the operands are then copied into fp16 with a tensor scale, as above).
  * Outputs that are NULL are not computed.  dx / dweight have the type of x / weight and are overwritten, multiplied by
  * loss_scale like dbias; *loss is overwritten, *loss_sum += loss * loss_rows.  Results do not depend on anything but the
  * arguments (no atomics).  Strides in elements.  No output may overlap an input.  workspace: 256-byte aligned; one call at

@@ -12,7 +12,7 @@
 // fp32 operands are scaled by a power of two per tensor, cut into two fp16 planes once per call (mma.h), G likewise: binary32's own
 // accuracy on the fp16 pipe.  bf16 operands are multiplied as they are and G is rounded to bf16 for its two products: relative
 // 2^-9 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
-// anything, and where a class has one row their rounding is as large as the result's own; then the operands are copied
+// anything, and where a class has one row their rounding is as large as the result's own; then (and for up to 8 rows) the operands are copied
 // into one fp16 plane (exact for bf16 values down to 2^-28 of the tensor's largest), and G rounded to fp16 (2^-12): 3 passes over W
 // more (4096 x 32000 x 1024: 1081 us against 1020; 33 x 100000 x 2048: 747 against 471).  db and every sum stay fp32.
 //
@@ -857,6 +857,10 @@ void pick_grad(int64_t n, int cp, int dim, int planes, bool dx, bool dw, bool on
   }
 }
 
+// Whether a bf16 call's gradients go through fp16 (the head of this file): with class weights, and with few rows, where a row of
+// dweight is one entry of G times one row of x and may happen to round exactly (1 x 1000 x 500: off by 5.6e-4 instead of 3.4e-4)
+bool bf16_in_half(const suave_linear_ce_t& h) { return (h.dx || h.dweight || h.dbias) && (h.class_weight || h.n_rows <= 8); }
+
 void make_layout(const suave_linear_ce_t& h, Layout& L) {
   const bool f32 = h.dtype == SUAVE_DTYPE_F32;
   const int np = f32 ? 2 : 1;
@@ -867,7 +871,7 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   L.n_strips = (int)ceil_div(h.n_classes, kStrip);
   L.ldp = (int64_t)L.Dp * 2 * np;
   L.plane = (uint32_t)(L.Dp * 2);
-  L.pack_w = f32 || (grad && h.class_weight) || h.dim % 8 != 0 || h.ld_weight % 8 != 0 || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
+  L.pack_w = f32 || bf16_in_half(h) || h.dim % 8 != 0 || h.ld_weight % 8 != 0 || (reinterpret_cast<uintptr_t>(h.weight) & 15) != 0;
   const int64_t per_class = n * 2 * np;
   // (at most 2^20 classes: 256 rows of a piece lie within the 2^31 bytes a tile addresses)
   const int64_t piece = std::min<int64_t>(1 << 20, std::max<int64_t>(kClassPad, (int64_t)(kPieceBytes / per_class) / kClassPad * kClassPad));
@@ -1165,8 +1169,7 @@ int launch_linear_ce(const suave_linear_ce_t* h, hipStream_t s) {
   SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_ce: workspace is null or not 256-byte aligned");
   SUAVE_REQUIRE(h->workspace_bytes >= L.total, "linear_ce: workspace too small (suave_linear_ce_workspace_bytes)");
   if (h->dtype == SUAVE_DTYPE_F32) return run_linear_ce<kF16, 2>(*h, L, s);
-  const bool grad = h->dx || h->dweight || h->dbias;
-  return grad && h->class_weight ? run_linear_ce<kF16, 1>(*h, L, s) : run_linear_ce<kBf16, 1>(*h, L, s);
+  return bf16_in_half(*h) ? run_linear_ce<kF16, 1>(*h, L, s) : run_linear_ce<kBf16, 1>(*h, L, s);
 }
 
 }  // namespace suave
