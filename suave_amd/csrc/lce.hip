@@ -7,13 +7,14 @@
 // its maximum and its sum of exponentials (8 bytes for 64 logits) and the target's logit; the strips of a row are then joined.
 // The second computes the tiles again, now against the known lse, and writes G for one piece of the classes at a time (bounded
 // scratch), which two products turn into dx (summed over the pieces in fp32) and dW.  8 n C D flops instead of 6: the price of
-// not keeping the logits.
+// not keeping the logits.  Two cases need one sweep: up to 256 classes a tile holds whole rows, and fp32 rows of 256 columns and more whose
+// G is one piece keep the first sweep's exponentials in its place and rescale them.
 //
 // fp32 operands are scaled by a power of two per tensor, cut into two fp16 planes once per call (mma.h), G likewise: binary32's own
 // accuracy on the fp16 pipe.  bf16 operands are multiplied as they are and G is rounded to bf16 for its two products: relative
-// 2^-9 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
+// 2^-8 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
 // anything, and where a class has one row their rounding is as large as the result's own; then (and for up to 8 rows) the operands are copied
-// into one fp16 plane (exact for bf16 values down to 2^-28 of the tensor's largest), and G rounded to fp16 (2^-12): 3 passes over W
+// into one fp16 plane (exact for bf16 values down to 2^-28 of the tensor's largest), and G rounded to fp16 (2^-11): 3 passes over W
 // more (4096 x 32000 x 1024: 1081 us against 1020; 33 x 100000 x 2048: 747 against 471).  db and every sum stay fp32.
 //
 // Rows with a negative target are left out whatever they hold (x is copied with those rows zero); a target >= C makes its row's

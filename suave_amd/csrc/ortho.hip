@@ -884,7 +884,7 @@ size_t head_bytes() { return up256(sizeof(double) * kMaxMats * kNormBlocks) + up
 
 bool is_small(int rows, int cols, int np) { return is_tiny(rows, cols) || small_shape(rows, cols, np).bytes <= kSmallLds; }
 
-// Planes of a matrix: float32 two.  bfloat16 one, an error (fp16's 2^-12 through the steps) that adds little to the result's own rounding
+// Planes of a matrix: float32 two.  bfloat16 one, an error (fp16's 2^-11 through the steps) that adds little to the result's own rounding
 // -- but on short sides it does not average out: 4 x 400 was 4 times, 96 x 39 1.6 times as far off as that rounding alone, from 128
 // on it is 1.3 times at most.  Short sides take two; they are bound by latency.
 constexpr int kOnePlaneSide = 128;

@@ -7,11 +7,9 @@ fp16 plane (X, A and B times 2^12) for bfloat16 ones -- and exact products in be
 elsewhere, may be FOUR times as far from float64 in the 2-norm (two independent errors of that size differ by sqrt(2); the three
 plane products add sqrt(3) 2^-24), plus the rounding of the result (2^-8 for bfloat16).  Single entries: 64 times that rms.
 
-A matrix with few directions may be rounded luckily by that iteration, so what the LAST step alone may add is allowed on top,
-per singular direction sigma <= 1.2, lambda = sigma^2 <= 1.45: in binary32 two roundings of each term of
-(a + b lambda + c lambda^2) sigma: 2 (3.44 + 6.93 + 4.28) 1.2 2^-24 = 35 2^-24; with fp16 factors, one rounding each of B (|B| <=
-3.44), of A (slope |b + 2 c lambda| <= 4.78 at lambda) and of X (slope of the step <= 3.9): (3.44 + 1.45 * 4.78 + 3.9) 1.2 2^-12 = 17 2^-12.
-That is sqrt(s) times as much in the 2-norm of a matrix with short side s (fp16: only up to s = 8, where nothing averages)."""
+A matrix with few directions may be rounded luckily by that iteration, so what the LAST step alone may add in binary32 is allowed on
+top, per singular direction sigma <= 1.2, lambda = sigma^2 <= 1.45: two roundings of each term of (a + b lambda + c lambda^2) sigma:
+2 (3.44 + 6.93 + 4.28) 1.2 2^-24 = 35 2^-24.  That is sqrt(s) times as much in the 2-norm of a matrix with short side s."""
 
 import math
 
@@ -50,7 +48,7 @@ def _tolerance(u, want, steps=5, eps=1e-7):
         rnd = lambda t: t.float().double()  # noqa: E731
     off = float(torch.linalg.matrix_norm(_iterate(u, steps, eps, rnd) - want))
     size, s, bf = float(torch.linalg.matrix_norm(want)), min(u.shape), u.dtype == torch.bfloat16
-    last = (17 * 2.0 ** -12 if s <= 8 else 0.0) if bf else 35 * 2.0 ** -24
+    last = 35 * 2.0 ** -24
     return 4 * off + last * math.sqrt(s) + (4 * 2.0 ** -24 + (2.0 ** -8 if bf else 2.0 ** -24)) * size
 
 
