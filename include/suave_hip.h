@@ -316,8 +316,9 @@ int suave_linear_ce_workspace_bytes(const suave_linear_ce_t* call, size_t* bytes
 int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
 
 /* 8-bit rows with one scale each: scale[r] = max |x_r| (1/127) in binary32, q[r, k] = x[r, k] / scale[r] rounded to the
- * nearest integer, ties to even, exactly.  A row of zeros has scale 0; a row with an infinity or a NaN has a non-finite
- * scale and q = 0.  q: 16-byte aligned, ld_q a multiple of 16; the bytes of a row from cols to the next multiple of 16
+ * nearest integer, ties to even, exactly, and at most 127 in magnitude (only a row whose scale is subnormal, which has few bits,
+ * reaches past that before).  A row of zeros, or one so small that its scale rounds to zero, has scale 0 and q = 0; a row with an
+ * infinity or a NaN has a non-finite scale and q = 0.  q: 16-byte aligned, ld_q a multiple of 16; the bytes of a row from cols to the next multiple of 16
  * are written as zero.  Strides in elements. */
 int suave_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,
                         float* scale, void* stream);

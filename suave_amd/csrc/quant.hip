@@ -83,7 +83,8 @@ __device__ __forceinline__ void load8(const T* row, int k0, int cols, int vec, f
 
 // What a row's largest |x| (bits) gives: its scale, and how its values are quantised.  Rows whose scale is next to or below binary32's
 // smallest normal number are taken 2^100 times larger, values and scale, which is exact: neither the reciprocal nor the
-// residuals leave the range then.
+// residuals leave the range then.  A subnormal scale has few bits -- largest |x| 190 2^-149: 1.496 2^-149 rounds to 2^-149 -- so values
+// reach 190 steps there; they saturate at 127.
 struct RowScale {
   float scale, s, inv;
   bool tiny, none;  // none: nothing to quantise (zeros, or an infinity or a NaN among them): q = 0
@@ -107,7 +108,7 @@ __device__ __forceinline__ uint2 quantize8(float (&u)[8], const RowScale& r) {
   float off = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) k[i] = quantize_near(u[i], r.inv, off);
-  if (off > 0.49998f) {
+  if (r.tiny || off > 0.49998f) {  // (tiny: quantize_near keeps the low byte of any integer, quantize_exact saturates)
 #pragma unroll
     for (int i = 0; i < 8; ++i) k[i] = quantize_exact(u[i], r.s, r.inv);
   }

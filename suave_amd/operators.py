@@ -226,7 +226,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x`` [rows, cols] (float32 / bfloat16) in 8 bits with one scale per row (``suave_quantize_rows``): ``(q, scale)``
-    with ``q`` int8 [rows, cols], the nearest integers of ``x / scale`` (rows start at multiples of 16 bytes), and ``scale``
+    with ``q`` int8 [rows, cols], the nearest integers of ``x / scale`` within +-127 (rows start at multiples of 16 bytes), and ``scale``
     float32 [rows] = max |x| (1/127), as torch divides by 127.0 on the device.  The form ``linear_quantized`` takes a layer's weight in."""
 
     dev = _device_of("x", x)

@@ -1,0 +1,53 @@
+"""Calls of suave_amd.operators at the edges of their ranges: rows of subnormal numbers."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+STEP = 2.0 ** -149  # binary32's smallest number
+
+
+def _subnormal_rows(cols):
+    """Rows of both signs whose largest element is m STEP: their scale, m / 127 STEP rounded, has few bits, and m / scale reaches 190."""
+    rows = []
+    for m in (1, 63, 64, 65, 100, 127, 128, 150, 190, 191, 300, 317, 500, 5000, 16000, 16129, 20000, 10 ** 6):
+        for sign in (1, -1):
+            j = np.rint(np.linspace(-m, m, cols)).astype(np.int64)
+            j[cols // 2] = m
+            rows.append(sign * j)
+    return np.stack(rows).astype(np.float64) * STEP
+
+
+def _definition(x):
+    """q (-127 .. 127) and scale of float64 rows that binary32 holds."""
+    s = (np.abs(x).max(axis=1).astype(np.float32) * (np.float32(1) / np.float32(127))).astype(np.float32)
+    ok = s > 0
+    q = np.where(ok[:, None], np.rint(x / np.where(ok, s, 1).astype(np.float64)[:, None]), 0.0)
+    return np.clip(q, -127, 127), s
+
+
+@pytest.mark.parametrize("cols", [8, 61, 700, 5000])
+def test_subnormal_rows_saturate(cols):
+    import torch
+    from suave_amd import operators as ops
+
+    x = _subnormal_rows(cols)
+    wq, ws = _definition(x)
+    t = torch.from_numpy(x.astype(np.float32)).cuda()
+    assert np.array_equal(t.cpu().numpy().astype(np.float64), x)
+    q, s = ops.quantize_rows(t)
+    assert np.array_equal(s.cpu().numpy(), ws)
+    assert np.array_equal(q.cpu().numpy().astype(np.float64), wq)
+    # q through the product with 127 times the identity: 127 q s, rounded once (127 127 7874 STEP, of the largest row, has 27 bits)
+    if cols > 700:
+        return
+    eye = torch.zeros((cols, (cols + 15) // 16 * 16), dtype=torch.int8, device="cuda:0")
+    eye[:, :cols] = torch.eye(cols, device="cuda:0").mul(127).to(torch.int8)
+    one = torch.ones(cols, device="cuda:0")
+    want = (127.0 * wq * ws.astype(np.float64)[:, None]).astype(np.float32)
+    n = len(x)
+    for rows in ([range(i, min(i + 5, n)) for i in range(0, n, 5)] + [range(n), [i % n for i in range(100)]]):  # few rows: quantised inside the product
+        rows = list(rows)
+        got = ops.linear_quantized(t[rows].contiguous(), eye[:, :cols], one)
+        assert np.array_equal(got.cpu().numpy(), want[rows]), len(rows)
