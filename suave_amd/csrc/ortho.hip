@@ -4,7 +4,7 @@
 //
 // drives every singular value of U towards 1 (after five steps into about 0.7 .. 1.2) and keeps the singular vectors.  X is
 // kept in the orientation of U; A and B live on the short side, so a tall U uses A = X^T X and X <- X B.  A and B are
-// symmetric: only tiles on and above the diagonal are computed, the others are written as their mirror image, which takes a
+// symmetric: only tiles on and above the diagonal are computed, what lies below it is written as the mirror image, which takes a
 // step from 2 s^2 l + 2 s^3 + 2 s^2 l to s^2 l + s^3 + 2 s^2 l flops (s the short side, l the long one).  All matrices of a
 // call go through the same launches: three per step for the whole list.
 //
@@ -313,6 +313,34 @@ __device__ __forceinline__ void store_mirror(char* base, int pit, int cols, int 
   }
 }
 
+// (m, n .. n + 3) of a symmetric matrix and their mirror image.  Each pair of elements comes from the one above the diagonal: in two planes
+// the two sums differ in the order of their cross terms, and which of them a tile computes depends on its size.
+// `side`: fragments above (1), on (0) or below (-1) the diagonal.
+template <int NP>
+__device__ __forceinline__ void store_symmetric(char* base, int pit, int s, int m, int n, const float (&v)[4], int side) {
+  if (side > 0) {
+    store_planes<NP>(base, pit, s, m, n, v);
+    store_mirror<NP>(base, pit, s, m, n, v);
+  } else if (side == 0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = n + u;
+      if (c < m) continue;
+      const float x = c < s ? v[u] : 0.f;
+      uint16_t hi, lo = 0;
+      if constexpr (NP == 2) planes(x, hi, lo);
+      else hi = f16_bits((_Float16)x);
+      auto put = [&](int r, int k) {
+        char* o = base + (int64_t)r * pit + k * 2;
+        *reinterpret_cast<uint16_t*>(o) = hi;
+        if constexpr (NP == 2) *reinterpret_cast<uint16_t*>(o + (s + 7) / 8 * 16) = lo;
+      };
+      put(m, c);
+      if (c > m && c < s) put(c, m);
+    }
+  }
+}
+
 template <class T, int GROUPS, int PARTS>
 __device__ __forceinline__ void run_tile(char* lds, const Operand& A, const Operand& B, int K, typename T::acc_t (&acc)[T::MI][T::NI]) {
   if constexpr (GROUPS > 1) T::template run_split<GROUPS, PARTS>(lds, A, B, K, acc);
@@ -368,7 +396,8 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, min_waves(64 * WM * WN * GRO
     for (int j = 0; j < R::NI; ++j) {
       if (GROUPS > 1 && (R::MI * j + mi) % GROUPS != group) continue;
       const int n = n0 + wn * (R::NI * 16) + 16 * j + 4 * (lane >> 4);
-      if (n >= sp) continue;
+      const int above = (n0 + wn * (R::NI * 16) + 16 * j) - (m0 + wm * (R::MI * 16) + 16 * mi), side = (above > 0) - (above < 0);
+      if (n >= sp || side < 0) continue;
       float v[4];
       if (POLY) {
         uint16_t hi[4], lo[4];
@@ -381,13 +410,11 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, min_waves(64 * WM * WN * GRO
           if (NP == 2) av += (float)__builtin_bit_cast(_Float16, lo[u]);
           v[u] = fmaf(fc, acc[mi][j][u], fb * av) + (r == n + u ? kNsA * kS : 0.f);
         }
-        store_planes<NP>(m.b, ps, s, r, n, v);
-        if (tm != tn) store_mirror<NP>(m.b, ps, s, r, n, v);
+        store_symmetric<NP>(m.b, ps, s, r, n, v, side);
       } else {
 #pragma unroll
         for (int u = 0; u < 4; ++u) v[u] = acc[mi][j][u] * (1.0f / kS);
-        store_planes<NP>(m.a, ps, s, r, n, v);
-        if (tm != tn) store_mirror<NP>(m.a, ps, s, r, n, v);
+        store_symmetric<NP>(m.a, ps, s, r, n, v, side);
       }
     }
   }
@@ -923,8 +950,8 @@ double launch_us(double blocks_per_cu, int64_t steps, int planes, int tile, int 
 }
 // Into how many groups of waves the blocks of a matrix's product cut K (Tile::run_split: a step of the block costs a CU as much as
 // that many steps of the tile and takes as long as one; about two steps more join the sums): 4 on 64 x 64 tiles, 2 on 96 x 96, 1 on
-// any.  Decided by the matrix alone, so that its result does not depend on what else is in the list: the order of the sums does
-// not depend on the tile, only on the groups.
+// any.  Decided by the matrix alone, so that its result does not depend on what else is in the list: the order of the sums of an
+// element does not depend on the tile, only on the groups, and symmetric results are computed above the diagonal only.
 int groups_of(const Mat& m, Phase p, int planes) {
   const int64_t steps = steps_of(m, p, planes);
   double us = 1e30;

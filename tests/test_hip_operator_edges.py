@@ -1,4 +1,4 @@
-"""Calls of suave_amd.operators at the edges of their ranges: rows of subnormal numbers."""
+"""Calls of suave_amd.operators at the edges of their ranges: rows of subnormal numbers, lists that share a choice of tile."""
 
 import numpy as np
 import pytest
@@ -51,3 +51,22 @@ def test_subnormal_rows_saturate(cols):
         rows = list(rows)
         got = ops.linear_quantized(t[rows].contiguous(), eye[:, :cols], one)
         assert np.array_equal(got.cpu().numpy(), want[rows]), len(rows)
+
+
+def _random(r, c, seed, dtype):
+    import torch
+
+    g = torch.Generator(device="cuda:0").manual_seed(seed)
+    return (torch.randn((r, c), generator=g, device="cuda:0") * 1e-3).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shapes", [[(3000, 3000), (3000, 3000)], [(2300, 3000), (1100, 2600), (3000, 2300)], [(1500, 1500), (2900, 2100)]])
+def test_a_matrix_is_the_same_in_any_list(shapes, dtype):
+    """Sizes whose tile depends on how much work the list holds: every matrix has the bits that it has alone."""
+    import torch
+    from suave_amd import operators as ops
+
+    us = [_random(r, c, 5 * r + c + i, getattr(torch, dtype)) for i, (r, c) in enumerate(shapes)]
+    for u, got in zip(us, ops.orthogonalize(us)):
+        assert torch.equal(got, ops.orthogonalize([u])[0]), tuple(u.shape)
