@@ -543,7 +543,8 @@ struct RowStage {
   }
 };
 
-// Dynamic LDS beyond 64 KB has to be allowed once per kernel and device; `done` is the caller's record for one kernel.
+// Dynamic LDS beyond 64 KB has to be allowed once per kernel and device; `done` is the caller's record for one kernel.  bytes: the most
+// that ANY launch of the kernel asks for (later calls do not raise it).
 inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
   if (bytes <= 64 * 1024) return hipSuccess;
   int dev = 0;

@@ -781,7 +781,9 @@ bool is_tiny(int rows, int cols) {
   const int s = std::min(rows, cols), l = std::max(rows, cols);
   return s <= kTinySide && (int64_t)s * tiny_pitch(l) <= kTinyValues;
 }
-int tiny_lds(int s, int l) { return 4 * kTinySide * (kTinySide + 1) * 8 + s * tiny_pitch(l) * 4; }
+constexpr int kTinyFixed = 4 * kTinySide * (kTinySide + 1) * 8, kTinyLds = kTinyFixed + kTinyValues * 4;
+static_assert(kTinyLds <= 160 * 1024 && kSmallLds <= 160 * 1024, "a CU's LDS");
+int tiny_lds(int s, int l) { return kTinyFixed + s * tiny_pitch(l) * 4; }
 
 __global__ __launch_bounds__(kTinyThreads) void k_ortho_tiny(Group g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -978,10 +980,12 @@ int pick_tile(const Group& g, Phase p, int planes) {
   return best;
 }
 
+// `most`: the largest lds of any launch of the kernel, where it depends on the matrices
 template <auto kernel>
-int launch(Group& g, int grid, int threads, int lds, hipStream_t s) {
+int launch(Group& g, int grid, int threads, int lds, hipStream_t s, int most = 0) {
   static std::atomic<uint64_t> done{0};
-  SUAVE_CHECK_HIP(allow_lds(reinterpret_cast<const void*>(kernel), lds, done));
+  SUAVE_REQUIRE(most == 0 || lds <= most, "orthogonalize: a launch asks for more LDS than its kernel was allowed");
+  SUAVE_CHECK_HIP(allow_lds(reinterpret_cast<const void*>(kernel), most ? most : lds, done));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, s, g);
   SUAVE_CHECK_HIP(hipGetLastError());
   return 0;
@@ -1096,11 +1100,11 @@ int run_list(int n, const Group& base, F fill, char* ws, hipStream_t s) {
     if (kind == kTiny) {
       int lds = 0;
       for (int i = 0; i < g.n; ++i) lds = std::max(lds, tiny_lds(std::min(g.m[i].rows, g.m[i].cols), std::max(g.m[i].rows, g.m[i].cols)));
-      rc = launch<k_ortho_tiny>(g, g.n, kTinyThreads, lds, s);
+      rc = launch<k_ortho_tiny>(g, g.n, kTinyThreads, lds, s, kTinyLds);
     } else if (kind == kSmall) {
       int lds = 0;
       for (int i = 0; i < g.n; ++i) lds = std::max(lds, small_shape(g.m[i].rows, g.m[i].cols, NP).bytes);
-      rc = launch<k_ortho_small<NP>>(g, g.n, 64 * kSmallWaves, lds, s);
+      rc = launch<k_ortho_small<NP>>(g, g.n, 64 * kSmallWaves, lds, s, kSmallLds);
     } else {
       rc = run_group<NP>(g, ws, s);
     }

@@ -70,3 +70,16 @@ def test_a_matrix_is_the_same_in_any_list(shapes, dtype):
     us = [_random(r, c, 5 * r + c + i, getattr(torch, dtype)) for i, (r, c) in enumerate(shapes)]
     for u, got in zip(us, ops.orthogonalize(us)):
         assert torch.equal(got, ops.orthogonalize([u])[0]), tuple(u.shape)
+
+
+def test_growing_sizes_of_one_block():
+    """Matrices that go through one block, their LDS growing from call to call past 64 KB: what an earlier call was allowed is not enough."""
+    import torch
+    from suave_amd import operators as ops
+
+    from tests.test_hip_ortho import _check
+
+    for shapes in ([(40, 40)], [(65, 64)], [(63, 130)], [(128, 128)], [(16, 1100)], [(16, 1800)], [(16, 2239)], [(100, 90), (128, 128)]):
+        us = [_random(r, c, r + c, torch.float32) for r, c in shapes]
+        for u, got in zip(us, ops.orthogonalize(us)):
+            _check(got, u)
