@@ -319,7 +319,7 @@ int suave_linear_ce(const suave_linear_ce_t* call, void* stream);
  * nearest integer, ties to even, exactly, and at most 127 in magnitude (only a row whose scale is subnormal, which has few bits,
  * reaches past that before).  A row of zeros, or one so small that its scale rounds to zero, has scale 0 and q = 0; a row with an
  * infinity or a NaN has a non-finite scale and q = 0.  q: 16-byte aligned, ld_q a multiple of 16; the bytes of a row from cols to the next multiple of 16
- * are written as zero.  Strides in elements. */
+ * are written as zero.  q and scale may not overlap x.  Strides in elements. */
 int suave_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,
                         float* scale, void* stream);
 
@@ -327,7 +327,8 @@ int suave_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t cols
  * sum_k q[r, k] weight[n, k] + bias[n], where q, s are suave_quantize_rows of x, made in the call.  The sums are exact in
  * 32 bits.  x and out have the type dtype; weight: 16-byte aligned, ld_weight a multiple of 16 (suave_quantize_rows of the
  * layer's rows; the bytes of a row from n_in to the next multiple of 16 are read, and do not matter).
- * A row of x with an infinity or a NaN gives NaN.  workspace: 256-byte aligned. */
+ * A row of x with an infinity or a NaN gives NaN.  out may not overlap an input.  workspace: 256-byte aligned; one call at a time
+ * uses it. */
 typedef struct suave_linear_quantized_t {
   int32_t dtype;
   int32_t n_out;

@@ -454,6 +454,9 @@ int launch_linear_quantized(const suave_linear_quantized_t* h, hipStream_t s) {
   if (h->n_rows == 0) return 0;
   SUAVE_REQUIRE(h->x && h->weight && h->weight_scale && h->out, "linear_quantized: x / weight / weight_scale / out is null");
   SUAVE_REQUIRE((reinterpret_cast<uintptr_t>(h->weight) & 15) == 0, "linear_quantized: weight must be 16-byte aligned");
+  // (few short rows are quantised by every block for itself, while others already write out)
+  for (const void* in : {h->x, static_cast<const void*>(h->weight), static_cast<const void*>(h->weight_scale), static_cast<const void*>(h->bias)})
+    SUAVE_REQUIRE(h->out != in, "linear_quantized: the output is an input");
   SUAVE_REQUIRE(h->workspace && (reinterpret_cast<uintptr_t>(h->workspace) & 255) == 0, "linear_quantized: workspace is null or not 256-byte aligned");
   SUAVE_REQUIRE(h->workspace_bytes >= need, "linear_quantized: workspace too small (suave_linear_quantized_workspace_bytes)");
   const int ldq = round_up(h->n_in, 16);

@@ -246,7 +246,7 @@ def linear_quantized(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     """``x @ (weight * weight_scale[:, None]).T + bias`` with ``x`` quantised per row in the call and exact integer sums
     (``suave_linear_quantized``).  ``x`` [rows, in] float32 / bfloat16 and the result [rows, out] of the same type;
     ``weight`` int8 [out, in] and ``weight_scale`` float32 [out] as ``quantize_rows`` gives them: rows 16-byte aligned, a
-    row stride that is a multiple of 16."""
+    row stride that is a multiple of 16.  ``out`` may not overlap an input."""
 
     dev = _device_of("x", x)
     ld = _matrix("x", x, dev, tuple(_DTYPES))

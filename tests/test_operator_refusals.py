@@ -163,3 +163,19 @@ def test_python_checks_without_a_gpu():
     with pytest.raises(ValueError, match="lr"):
         ops.muon_step([x], [x], [x], lr=[0.1, 0.2])
     assert ops.orthogonalize([]) == [] and ops.muon_step([], [], [], lr=0.1) is None
+
+
+def test_linear_quantized_outputs_that_are_inputs(lib):
+    """In place: blocks that still quantise x would read what others have written."""
+
+    def h(**kw):
+        s = LinearQuantizedT()
+        base = dict(dtype=0, n_out=20, n_in=20, n_rows=3, x=P, ld_x=20, weight=2 * P, ld_weight=32, weight_scale=3 * P, bias=6 * P, out=4 * P,
+                    ld_out=20, workspace=5 * P, workspace_bytes=1 << 40)
+        base.update(kw)
+        for k, v in base.items():
+            setattr(s, k, v)
+        return s
+
+    for other in ("x", "weight", "weight_scale", "bias"):
+        _refused(lib, lib.suave_linear_quantized(C.byref(h(**{other: 4 * P})), None), "output is an input")
