@@ -372,7 +372,7 @@ int suave_orthogonalize(const suave_ortho_matrix_t* matrices_host, int32_t n_mat
 /* One Muon step on a list of float32 weight matrices (hidden layers; biases and the rest stay with suave_adam_step):
  *   momentum <- mu momentum + grad;   U = nesterov ? grad + mu momentum : momentum
  *   param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) orthogonalize(U)
- * param and momentum are updated in place; no matrix of the list may overlap another. */
+ * param and momentum are updated in place; neither may overlap anything else in the list (gradients are only read). */
 typedef struct suave_muon_matrix_t {
   float* param;
   const float* grad;

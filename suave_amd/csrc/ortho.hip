@@ -1193,9 +1193,13 @@ int launch_muon(const suave_muon_matrix_t* mats, int32_t n, float momentum, int 
     SUAVE_REQUIRE(h.ld_param >= h.cols && h.ld_grad >= h.cols && h.ld_momentum >= h.cols, "muon_step: a row stride is shorter than the row");
     SUAVE_REQUIRE(std::isfinite(h.lr) && h.lr >= 0.f, "muon_step: lr must not be negative");
     SUAVE_REQUIRE(h.param != h.grad && h.param != h.momentum && h.grad != h.momentum, "muon_step: param, grad and momentum must be three matrices");
-    for (int j = 0; j < i; ++j)
-      SUAVE_REQUIRE(h.param != mats[j].param && h.momentum != mats[j].momentum && h.param != mats[j].momentum && h.momentum != mats[j].param,
+    for (int j = 0; j < i; ++j) {
+      const suave_muon_matrix_t& o = mats[j];
+      SUAVE_REQUIRE(h.param != o.param && h.momentum != o.momentum && h.param != o.momentum && h.momentum != o.param,
                     "muon_step: a matrix is in the list twice");
+      SUAVE_REQUIRE(h.grad != o.param && h.grad != o.momentum && o.grad != h.param && o.grad != h.momentum,
+                    "muon_step: a gradient is another matrix's param or momentum");
+    }
   }
   Group base{};
   base.eps = eps; base.steps = steps; base.muon = 1; base.momentum = momentum; base.nesterov = nesterov;

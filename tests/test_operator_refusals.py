@@ -179,3 +179,18 @@ def test_linear_quantized_outputs_that_are_inputs(lib):
 
     for other in ("x", "weight", "weight_scale", "bias"):
         _refused(lib, lib.suave_linear_quantized(C.byref(h(**{other: 4 * P})), None), "output is an input")
+
+
+def test_muon_gradients_that_are_written(lib):
+    def call(*mats):
+        arr = (MuonMatrixT * len(mats))()
+        for a, kw in zip(arr, mats):
+            for k, v in dict(dict(ld_param=8, ld_grad=8, ld_momentum=8, rows=5, cols=8, lr=0.1), **kw).items():
+                setattr(a, k, v)
+        return lib.suave_muon_step(arr, len(mats), 0.9, 1, 0.0, 5, 1e-7, 9 * P, 1 << 40, None)
+
+    one = dict(param=P, grad=2 * P, momentum=3 * P)
+    for grad in (P, 3 * P):
+        other = dict(param=5 * P, grad=grad, momentum=6 * P)
+        _refused(lib, call(one, other), "another matrix's")
+        _refused(lib, call(other, one), "another matrix's")
