@@ -1123,23 +1123,24 @@ class SUAVE:
         if not self._is_fitted or self._classifier is None or self._classes is None:
             raise RuntimeError(f"Model must be fitted before calling {what}")
 
-    def _compute_logits(self, X: pd.DataFrame) -> np.ndarray:
-        """_compute_logits (model.py:3449-3486): classifier on the posterior-mean latent."""
+    def _compute_logits(self, X: pd.DataFrame, served: bool = True) -> np.ndarray:
+        """_compute_logits (model.py:3449-3486): classifier on the posterior-mean latent.  ``served=False``: the classifier itself,
+        also while 8-bit weights serve."""
 
         table = self._table(X.loc[:, list(self.schema.feature_names)])
         if table.n_rows == 0:
             return np.empty((0, len(self._classes)), np.float32)
         self._classifier.eval()
-        served = self._quantized_head
-        if served is not None and served.clf is self._classifier:
-            return served(self._posterior_mean(table)).cpu().numpy()
+        quantized = self._quantized_head if served else None
+        if quantized is not None and quantized.clf is self._classifier:
+            return quantized(self._posterior_mean(table)).cpu().numpy()
         with torch.no_grad():
             return self._classifier(self._posterior_mean(table)).cpu().numpy()
 
     def quantize_classifier(self, enable: bool = True) -> "SUAVE":
-        """Serve the classifier's logits (``predict``, ``predict_proba``, ``calibrate``) from 8-bit weights
-        (``supervised.QuantizedHead``) until the next ``fit`` or ``quantize_classifier(False)``.  Not saved with the model;
-        off by default."""
+        """Serve the classifier's logits (``predict``, ``predict_proba``) from 8-bit weights (``supervised.QuantizedHead``) until
+        the next ``fit`` or ``quantize_classifier(False)``.  Not saved with the model; off by default.  ``calibrate`` keeps fitting
+        its temperature, which outlives the 8-bit weights, to the classifier itself."""
 
         self._ensure_classifier("quantize_classifier")
         self._quantized_head = sup.QuantizedHead(self._classifier) if enable else None
@@ -1299,7 +1300,7 @@ class SUAVE:
         self._ensure_classifier("calibrate")
         if len(X) != len(y):
             raise ValueError("X and y must have matching first dimensions")
-        logits = self._compute_logits(X)
+        logits = self._compute_logits(X, served=False)
         self._temperature_scaler.fit(logits, self._map_targets(np.asarray(y)))
         self._is_calibrated = True
         return self

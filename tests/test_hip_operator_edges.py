@@ -1,4 +1,5 @@
-"""Calls of suave_amd.operators at the edges of their ranges: rows of subnormal numbers, lists that share a choice of tile."""
+"""Calls of suave_amd.operators at the edges of their ranges: rows of subnormal numbers, lists that share a choice of tile, and
+what a served model keeps."""
 
 import numpy as np
 import pytest
@@ -83,3 +84,29 @@ def test_growing_sizes_of_one_block():
         us = [_random(r, c, r + c, torch.float32) for r, c in shapes]
         for u, got in zip(us, ops.orthogonalize(us)):
             _check(got, u)
+
+
+def test_calibration_is_of_the_classifier_itself(tmp_path):
+    """The temperature outlives the 8-bit weights (quantize_classifier(False), save): fitted while they serve, it is the one fitted without."""
+    import pandas as pd
+    from suave_amd.model import SUAVE
+    from suave_amd.types import Schema
+
+    rng = np.random.default_rng(1)
+    n = 300
+    df = pd.DataFrame({"a": rng.normal(size=n), "c": rng.integers(0, 3, n)})
+    y = (df["a"].to_numpy() > 0.2).astype(int) + df["c"].to_numpy()
+    m = SUAVE(Schema({"a": {"type": "real"}, "c": {"type": "cat", "n_classes": 3}}), behaviour="supervised", latent_dim=8, n_components=2,
+              hidden_dims=(32, 16), random_state=0)
+    m.fit(df, y=y, warmup_epochs=1, kl_warmup_epochs=1, head_epochs=2, finetune_epochs=1, decoder_refine_epochs=1)
+    m.calibrate(df, y)
+    want, proba = m._temperature_scaler.state_dict(), m.predict_proba(df)
+    m.quantize_classifier()
+    assert not np.array_equal(m.predict_proba(df), proba)
+    m._temperature_scaler = type(m._temperature_scaler)()  # (a fit starts from the temperature it finds)
+    m.calibrate(df, y)
+    assert m._temperature_scaler.state_dict() == want
+    path = m.save(tmp_path / "m.pt") or tmp_path / "m.pt"
+    assert np.array_equal(SUAVE.load(path).predict_proba(df), proba)
+    m.quantize_classifier(False)
+    assert np.array_equal(m.predict_proba(df), proba)
