@@ -276,9 +276,11 @@ int suave_elbo_joint_backward(const suave_plan* plan, const float* params, const
  * out: it adds nothing anywhere, whatever x holds there, and its dx is zero; targets[i] >= n_classes makes the row's
  * loss NaN and with it the mean and the gradients.  A batch with no weight has loss 0 and zero gradients.  bias may
  * hold -inf (a class that is never predicted); other non-finite inputs make what they touch non-finite.
- * F32: products of binary32 grade (two fp16 planes per operand and tensor scale; elements 2^28 times smaller than their
- * tensor's largest lose relative accuracy).  BF16: fp32 accumulation, the logit gradient rounded once: to bf16, or with
- * class weights or up to 8 rows to fp16 (the operands are then copied into fp16 with a tensor scale, as above).
+ * F32: x, weight and the logit gradient enter their products as two fp16 planes under a power-of-two scale: a value is held to 2^-23
+ * of itself, but no finer than 2^-38 of the largest that shares its scale.  Scales are those of the tensors, except that in the logits a
+ * row of x or of weight 256 times smaller than the tensor's largest has its own, so no row's size reaches another's loss; the
+ * logit gradient's is that of the largest class weight.  BF16: fp32 accumulation, the logit gradient rounded once: to bf16, or with
+ * class weights or up to 8 rows to fp16 (the operands are then copied into fp16, scaled as above).
  * Outputs that are NULL are not computed.  dx / dweight have the type of x / weight and are overwritten, multiplied by
  * loss_scale like dbias; *loss is overwritten, *loss_sum += loss * loss_rows.  Results do not depend on anything but the
  * arguments (no atomics).  Strides in elements.  No output may overlap an input.  workspace: 256-byte aligned; one call at

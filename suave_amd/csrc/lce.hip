@@ -10,8 +10,8 @@
 // not keeping the logits.  Two cases need one sweep: up to 256 classes a tile holds whole rows, and fp32 rows of 256 columns and more whose
 // G is one piece keep the first sweep's exponentials in its place and rescale them.
 //
-// fp32 operands are scaled by a power of two per tensor, cut into two fp16 planes once per call (mma.h), G likewise: binary32's own
-// accuracy on the fp16 pipe.  bf16 operands are multiplied as they are and G is rounded to bf16 for its two products: relative
+// fp32 operands are scaled by a power of two per tensor (in the logits: also per row where rows differ much, pack_row_scale), cut into two
+// fp16 planes once per call (mma.h), G likewise: binary32's own accuracy on the fp16 pipe.  bf16 operands are multiplied as they are and G is rounded to bf16 for its two products: relative
 // 2^-8 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
 // anything, and where a class has one row their rounding is as large as the result's own; then (and for up to 8 rows) the operands are copied
 // into one fp16 plane (exact for bf16 values down to 2^-28 of the tensor's largest), and G rounded to fp16 (2^-11): 3 passes over W
@@ -39,7 +39,8 @@ constexpr int64_t kScanElems = 65536;  // x and W together: up to here every pac
 constexpr size_t kPieceBytes = (size_t)192 << 20;  // G of one piece: what the 256 MB memory-side cache holds beside its operands
 
 struct Scalars {
-  float x_scale, w_scale;    // powers of two the fp16 operands were multiplied by (1 for bf16 ones)
+  float x_scale, w_scale;    // powers of two the tensors' fp16 operands are multiplied by (1 for bf16 ones)
+  int x_split, w_split;      // rows of x / W far below the tensor's largest have scales of their own in the logits' operand (pack_row_scale)
   float g_unit;              // loss_scale * max_w / total / g_scale: what one unit of the stored G is worth
   float max_w;               // largest |class weight| (1 without gradients and without class weights): G is stored relative to it
 };
@@ -58,12 +59,14 @@ struct PackArgs {
   const void* src[2];        // x, W
   int64_t ld[2];             // elements
   int64_t rows[2];
-  char* dst[2];              // null: not packed
+  char* dst[2];              // null: not packed.  The operands of the logits
+  char* same[2];             // null: not wanted.  Those of the gradients' products where the rows of dst differ in scale: one scale
+  float* unit[2];            // [n], [C_pad]: what one unit of a row of dst is worth
   int64_t dst_ld[2];         // bytes
   int blocks0;               // blocks of tensor 0
   int D, Dp;
   const int32_t* targets;    // rows of tensor 0 with a negative target are zero
-  float* amax;               // [3][kAmaxBlocks]: x, W, class weights
+  float* amax;               // [5][kAmaxBlocks]: largest of x, W, class weights; smallest row (by its largest element) of x, W
   int scan;                  // no k_lce_amax launch: the blocks look for the maxima themselves
   const float* class_weight;
   Scalars* scal;
@@ -83,59 +86,105 @@ __device__ __forceinline__ float finite_abs(float v) {
   return v < INFINITY ? v : 0.f;  // (a NaN compares false)
 }
 
-// largest finite |value| of x (rows that count) or W: the share of thread `first` of `step`, in chunks of eight
+// lanes that share a row of q chunks of eight: a power of two, up to a wave
+__device__ __forceinline__ int row_lanes(int q) { return q >= 64 ? 64 : q <= 1 ? 1 : 1 << (32 - __builtin_clz(q - 1)); }
+
+// the maximum over the `L` neighbouring lanes that share a row, in each of them: within 16 lanes without LDS
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float row_max(float v, int L) {
+  if (L > 1) v = max_dpp<0xb1>(v);   // lane ^ 1
+  if (L > 2) v = max_dpp<0x4e>(v);   // lane ^ 2
+  if (L > 4) v = max_dpp<0x141>(v);  // mirrored within 8: the other four
+  if (L > 8) v = max_dpp<0x140>(v);  // mirrored within 16: the other eight
+  if (L > 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+  if (L > 32) v = fmaxf(v, __shfl_xor(v, 32, 64));
+  return v;
+}
+
+// chunk c (eight values, c < ceil(D / 8)) of a row, zeros past D
 template <class T>
-__device__ __forceinline__ float scan_rows(const PackArgs& a, int t, int64_t first, int64_t step) {
+__device__ __forceinline__ void load_chunk(const PackArgs& a, const T* row, int c, T (&v)[8]) {
+  const int d0 = c * 8;
+  if (d0 + 8 <= a.D) {
+    load8(row + d0, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = d0 + i < a.D ? row[d0 + i] : (T)0;
+  }
+}
+
+// Largest finite |value| of each row of x (of those that count) or W: mx their largest, mn the smallest that is not zero.  `block` of
+// `blocks`; row_lanes lanes share a row, four rows in flight.
+template <class T>
+__device__ __forceinline__ void scan_rows(const PackArgs& a, int t, int block, int blocks, float& mx, float& mn) {
   const T* src = static_cast<const T*>(a.src[t]);
-  const int64_t ld = a.ld[t];
-  const int q = (a.D + 7) / 8;
-  const int64_t chunks = a.rows[t] * q;
-  float m = 0.f;
-  constexpr int U = 4;  // chunks in flight
-  for (int64_t e0 = first; e0 < chunks; e0 += U * step) {
-    T v[U][8];
+  const int q = (a.D + 7) / 8, L = row_lanes(q), l = threadIdx.x & (L - 1);
+  const int64_t rows = a.rows[t], step = (int64_t)blocks * (256 / L), mine = threadIdx.x / L;
+  constexpr int U = 4;
+  for (int64_t base = (int64_t)block * (256 / L); base < rows; base += U * step) {  // (the same number of turns for every lane of a wave)
+    float m[U];
+    const T* row[U];
+    bool in[U], gone[U];  // (rows without a target are read like the others: a load that waits for the target takes twice as long)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const int64_t r = base + mine + u * step;
+      in[u] = r < rows;
+      row[u] = src + (in[u] ? r : 0) * a.ld[t];
+      gone[u] = t == 0 && in[u] && a.targets[r] < 0;
+      m[u] = 0.f;
+    }
+    for (int c = l; c < q; c += L) {
+      T v[U][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = (T)0;
-      const int64_t e = e0 + u * step;
-      if (e >= chunks) continue;
-      const int64_t r = row_of(e, chunks, q);
-      const int d0 = (int)(e - r * q) * 8;
-      if (t == 0 && a.targets[r] < 0) continue;
-      const T* p = src + r * ld;
-      if (a.D >= 8) load8(p + min(d0, a.D - 8), v[u]);  // (the last chunk may repeat some of the one before)
-      else
-        for (int i = 0; i < a.D; ++i) v[u][i] = p[i];
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = (T)0;
+        if (!in[u]) continue;
+        if (a.D >= 8) load8(row[u] + min(c * 8, a.D - 8), v[u]);  // (the last chunk may repeat some of the one before)
+        else load_chunk(a, row[u], c, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[u] = fmaxf(m[u], finite_abs(as_float(v[u][i])));
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(as_float(v[u][i])));
+    for (int u = 0; u < U; ++u) {
+      m[u] = row_max(gone[u] ? 0.f : m[u], L);
+      mx = fmaxf(mx, m[u]);
+      if (m[u] > 0.f) mn = fminf(mn, m[u]);
+    }
   }
-  return m;
 }
-__device__ __forceinline__ float block_max(float m, float* part) {  // 256 threads; every thread gets the maximum
-  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+__device__ __forceinline__ float wave_max(float v) { return row_max(v, 64); }
+// 256 threads; every thread gets the maxima of a and w and the minimum of b
+__device__ __forceinline__ void block_extremes(float& a, float& b, float& w, float (&part)[3][4]) {
+  a = wave_max(a);
+  b = wave_max(-b);
+  w = wave_max(w);
+  if ((threadIdx.x & 63) == 0) { part[0][threadIdx.x >> 6] = a; part[1][threadIdx.x >> 6] = b; part[2][threadIdx.x >> 6] = w; }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  a = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
+  b = -fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
+  w = fmaxf(fmaxf(part[2][0], part[2][1]), fmaxf(part[2][2], part[2][3]));
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void k_lce_amax(PackArgs a) {
-  __shared__ float part[4];
+  __shared__ float part[3][4];
   const int t = (int)blockIdx.x >= kAmaxBlocks, b = blockIdx.x - t * kAmaxBlocks;
-  const int64_t first = (int64_t)b * 256 + threadIdx.x, step = (int64_t)kAmaxBlocks * 256;
-  const float m = block_max(scan_rows<T>(a, t, first, step), part);
-  if (threadIdx.x == 0) a.amax[blockIdx.x] = m;
-  if (t == 0) {
-    float w = 0.f;
-    if (a.class_weight)
-      for (int64_t c = first; c < a.C; c += step) w = fmaxf(w, finite_abs(a.class_weight[c]));
-    w = block_max(w, part);
-    if (threadIdx.x == 0) a.amax[2 * kAmaxBlocks + b] = w;
+  float m = 0.f, mn = INFINITY, w = 0.f;
+  if (t == 0 && a.class_weight)
+    for (int64_t c = (int64_t)b * 256 + threadIdx.x; c < a.C; c += (int64_t)kAmaxBlocks * 256) w = fmaxf(w, finite_abs(a.class_weight[c]));
+  scan_rows<T>(a, t, b, kAmaxBlocks, m, mn);
+  block_extremes(m, mn, w, part);
+  if (threadIdx.x == 0) {
+    a.amax[blockIdx.x] = m;
+    a.amax[3 * kAmaxBlocks + blockIdx.x] = mn;
+    if (t == 0) a.amax[2 * kAmaxBlocks + b] = w;
   }
 }
 
@@ -147,69 +196,121 @@ __device__ __forceinline__ float plane_scale(float amax) {
   return ldexpf(1.0f, min(14 - e, 120));
 }
 
+// A tensor has ONE scale as long as its rows are of a size: fp16 holds both planes of what lies up to 2^14 below the largest element in
+// full.  Rows of x are independent in the logits, though, and so are the classes: a row whose largest element is kSplit times smaller than
+// the tensor's gets a scale of its own there, or one large row would cost all others their low planes (64 x 1000 x 32 with one
+// row 10^6 times the others: their lse off by 3.7e-5 instead of 2.5e-6).  The gradients' products add over these rows (dW over x's, dx
+// over W's), so they take operands of one scale: what a small row loses there is 2^-38 of the largest.  Looking for such rows and
+// the units' way through the epilogue cost 4096 x 1000 x 128 two microseconds of 59, 1777 x 20011 x 501 nine of 476.
+constexpr float kSplit = 256.0f;
+__device__ __forceinline__ bool split_rows(float mx, float mn) { return mn < mx * (1.0f / kSplit); }
+__device__ __forceinline__ float pack_row_scale(float row_max, float mx, float scale) {
+  return row_max > 0.f && row_max < mx * (1.0f / kSplit) ? plane_scale(row_max) : scale;
+}
+template <class T, int PLANES>
+__device__ __forceinline__ void store_chunk(char* o, const T (&v)[8], float scale, int Dp) {
+  uint16_t hi[8], lo[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (PLANES > 0) g_bits<kF16, PLANES>(as_float(v[i]) * scale, hi[i], lo[i]);
+    else hi[i] = v[i];
+  }
+  *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+  if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(o + (size_t)Dp * 2) = *reinterpret_cast<const uint4*>(lo);
+}
+
 // PLANES 1, 2: scaled fp16; 0: as it is
 template <class T, int PLANES>
 __global__ __launch_bounds__(256) void k_lce_pack(PackArgs a) {
   const int t = (int)blockIdx.x >= a.blocks0;
   const int b = blockIdx.x - (t ? a.blocks0 : 0), nb = t ? (int)gridDim.x - a.blocks0 : a.blocks0;
-  float scale = 1.0f, max_w = 1.0f;
+  float scale = 1.0f, max_w = 1.0f, largest = 0.f;
+  bool split = false;
   if constexpr (PLANES > 0) {
-    __shared__ float part[4];
-    float m = 0.f, w = 0.f;
+    __shared__ float part[3][4];
+    float m = 0.f, mn = INFINITY, w = 0.f;
     if (a.scan) {
-      m = scan_rows<T>(a, t, threadIdx.x, 256);
+      scan_rows<T>(a, t, 0, 1, m, mn);
       if (t == 0 && a.class_weight)
         for (int c = threadIdx.x; c < a.C; c += 256) w = fmaxf(w, finite_abs(a.class_weight[c]));
     } else {
       for (int i = threadIdx.x; i < kAmaxBlocks; i += 256) {
         m = fmaxf(m, a.amax[t * kAmaxBlocks + i]);
+        mn = fminf(mn, a.amax[(3 + t) * kAmaxBlocks + i]);
         w = fmaxf(w, a.amax[2 * kAmaxBlocks + i]);
       }
     }
-    scale = plane_scale(block_max(m, part));
-    w = block_max(w, part);
+    block_extremes(m, mn, w, part);
+    largest = m;
+    split = split_rows(m, mn);
+    scale = plane_scale(m);
     max_w = a.class_weight && w > 0.f ? w : 1.0f;
   }
   if (b == 0 && threadIdx.x == 0) {
     if (t == 0) {
       a.scal->x_scale = scale;
+      a.scal->x_split = split;
       a.scal->max_w = max_w;
     } else {
       a.scal->w_scale = scale;
+      a.scal->w_split = split;
     }
   }
   if (t) {
     for (int64_t c = (int64_t)b * 256 + threadIdx.x; c < a.C_pad; c += (int64_t)nb * 256)
       a.bias_pad[c] = c < a.C ? (a.bias ? a.bias[c] : 0.f) : -INFINITY;
   }
+  if constexpr (PLANES > 0) {
+    const int64_t units = t ? a.C_pad : a.rows[0], from = split ? a.rows[t] : 0;  // (rows of their own scale say theirs below)
+    for (int64_t r = from + (int64_t)b * 256 + threadIdx.x; r < units; r += (int64_t)nb * 256) a.unit[t][r] = 1.0f / scale;
+  }
   if (a.dst[t] == nullptr) return;
   const T* src = static_cast<const T*>(a.src[t]);
   const int q = a.Dp / 8;  // 16-byte chunks of a row
-  const int64_t chunks = a.rows[t] * q, ld = a.ld[t];
+  const int64_t rows = a.rows[t], ld = a.ld[t];
+  if constexpr (PLANES > 0) {
+    if (split) {  // row_lanes lanes share a row: its maximum, then its planes (read again, from L2)
+      const int L = row_lanes(q), l = threadIdx.x & (L - 1), per = 256 / L;
+      for (int64_t base = (int64_t)b * per; base < rows; base += (int64_t)nb * per) {
+        const int64_t r = base + threadIdx.x / L;
+        const bool in = r < rows && !(t == 0 && a.targets[r] < 0);
+        const T* p = src + (in ? r : 0) * ld;
+        float m = 0.f;
+        for (int c = l; in && c < q; c += L) {
+          T v[8];
+          load_chunk(a, p, c, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(as_float(v[i])));
+        }
+        m = row_max(m, L);
+        if (r >= rows) continue;
+        const float rs = pack_row_scale(m, largest, scale);
+        if (l == 0) a.unit[t][r] = 1.0f / rs;
+        for (int c = l; c < q; c += L) {
+          T v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = (T)0;
+          if (in) load_chunk(a, p, c, v);
+          const int64_t o = r * a.dst_ld[t] + c * 16;
+          store_chunk<T, PLANES>(a.dst[t] + o, v, rs, a.Dp);
+          if (a.same[t]) store_chunk<T, PLANES>(a.same[t] + o, v, scale, a.Dp);
+        }
+      }
+      return;
+    }
+  }
+  const int64_t chunks = rows * q;
   for (int64_t e = (int64_t)b * 256 + threadIdx.x; e < chunks; e += (int64_t)nb * 256) {
     const int64_t r = row_of(e, chunks, q);
-    const int d0 = (int)(e - r * q) * 8;
-    const bool gone = t == 0 && a.targets[r] < 0;
-    const T* p = src + r * ld + d0;
+    const int c = (int)(e - r * q);
     T v[8];
+    const bool gone = t == 0 && a.targets[r] < 0;
+    load_chunk(a, src + r * ld, c, v);
+    if (gone) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (T)0;
-    if (!gone) {
-      if (d0 + 8 <= a.D) load8(p, v);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (d0 + i < a.D) v[i] = p[i];
+      for (int i = 0; i < 8; ++i) v[i] = (T)0;
     }
-    uint16_t hi[8], lo[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (PLANES > 0) g_bits<kF16, PLANES>(as_float(v[i]) * scale, hi[i], lo[i]);
-      else hi[i] = v[i];
-    }
-    char* o = a.dst[t] + r * a.dst_ld[t] + d0 * 2;
-    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
-    if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(o + (size_t)a.Dp * 2) = *reinterpret_cast<const uint4*>(lo);
+    store_chunk<T, PLANES>(a.dst[t] + r * a.dst_ld[t] + c * 16, v, scale, a.Dp);
   }
 }
 
@@ -287,6 +388,8 @@ struct LogitArgs {
   int group;
   const Scalars* scal;
   const float* bias;               // padded
+  const float* x_unit;             // [n], scaled fp16 operands: what one unit of a row of x is worth
+  const float* w_unit;             // padded
   const int32_t* targets;
   // first sweep
   float2* strips;                  // [strip][n] (max, sum exp(l - max))
@@ -301,10 +404,18 @@ struct LogitArgs {
   RowArgs rows;                    // whole rows in one tile
 };
 
+// the units are powers of two
+template <int TYPE>
+__device__ __forceinline__ float logit(float acc, float x_unit, float w_unit, float bias) {
+  if constexpr (TYPE == kF16) return fmaf(acc, x_unit * w_unit, bias);
+  else return acc + bias;
+}
+
 // G of a tile from its logits and its rows' (lse, weight), and the column sums that db is made of
 template <class T>
-__device__ __forceinline__ void write_gradients(const LogitArgs& a, const typename T::acc_t (&acc)[T::MI][T::NI], const float4 (&bias)[T::NI], float unit,
-                                                int tm, int cw, const float2* row_tab, const int* target_tab, char* stages) {
+__device__ __forceinline__ void write_gradients(const LogitArgs& a, const typename T::acc_t (&acc)[T::MI][T::NI], const float4 (&bias)[T::NI],
+                                                const float4 (&unit)[T::NI], int tm, int cw, const float2* row_tab, const int* target_tab,
+                                                const float* unit_tab, char* stages) {
   constexpr bool P = T::NP == 2;
   typedef RowStage<uint16_t, kStrip> Rows;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, g = lane >> 4;
@@ -320,12 +431,14 @@ __device__ __forceinline__ void write_gradients(const LogitArgs& a, const typena
     const int m0 = wm * (T::MI * 16) + 16 * i, ml = m0 + (lane & 15);
     const float2 rw = row_tab[ml];
     const int at = target_tab[ml] - cw;
+    const float x_unit = T::TYPE == kF16 ? unit_tab[ml] : 1.0f;
     float p[T::NI][4];
 #pragma unroll
     for (int j = 0; j < T::NI; ++j) {
       const float* bj = reinterpret_cast<const float*>(&bias[j]);
+      const float* wj = reinterpret_cast<const float*>(&unit[j]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[j][u] = __expf(fmaf(acc[i][j][u], unit, bj[u]) - rw.x);
+      for (int u = 0; u < 4; ++u) p[j][u] = __expf(logit<T::TYPE>(acc[i][j][u], x_unit, wj[u], bj[u]) - rw.x);
     }
     if (__any(at >= 0 && at < kStrip)) {
 #pragma unroll
@@ -399,7 +512,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
   const int my_target = has_row ? a.targets[m_base + t] : -1;
   float2 my_row = make_float2(0.f, 0.f);
   if (SWEEP == 1 && has_row) my_row = a.row[m_base + t];
-  const float unit = 1.0f / (a.scal->x_scale * a.scal->w_scale);  // a power of two
+  constexpr bool kScaled = T::TYPE == kF16;
+  const float my_x_unit = kScaled && has_row ? a.x_unit[m_base + t] : 0.f;
+  const float my_w_unit = kScaled && t < T::BN ? a.w_unit[c_base + t] : 0.f;
   const Operand A{a.x + m_base * a.ldx, (uint32_t)a.ldx, (int)min<int64_t>(T::BM, a.n - m_base), a.plane};
   const Operand B{a.w + (int64_t)c_base * a.ldw, (uint32_t)a.ldw, a.C - c_base, a.plane};
   typename T::acc_t acc[T::MI][T::NI];
@@ -411,32 +526,43 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
   float2* row_tab = reinterpret_cast<float2*>(lds);
   float* bias_tab = reinterpret_cast<float*>(row_tab + T::BM);
   int* target_tab = reinterpret_cast<int*>(bias_tab + T::BN);
-  float2* strip_tab = reinterpret_cast<float2*>(target_tab + T::BM);  // whole rows only
+  float* w_unit_tab = reinterpret_cast<float*>(target_tab + T::BM);  // scaled operands only
+  float* x_unit_tab = w_unit_tab + (kScaled ? T::BN : 0);
+  float2* strip_tab = reinterpret_cast<float2*>(x_unit_tab + (kScaled ? T::BM : 0));  // whole rows only
   float* logit_tab = reinterpret_cast<float*>(strip_tab + T::WN * T::BM);
-  constexpr int kTabs = T::BM * 12 + T::BN * 4 + (SWEEP == 2 ? T::BM * (8 * T::WN + 4) : 0);
+  constexpr int kTabs = T::BM * 12 + T::BN * 4 + (kScaled ? (T::BM + T::BN) * 4 : 0) + (SWEEP == 2 ? T::BM * (8 * T::WN + 4) : 0);
   static_assert(kTabs % 16 == 0 && kTabs + T::WM * T::WN * T::NP * RowStage<uint16_t, kStrip>::kBytes <= T::kLds, "tables and stages fit the tile's LDS");
-  if (t < T::BN) bias_tab[t] = my_bias;
+  if (t < T::BN) {
+    bias_tab[t] = my_bias;
+    if (kScaled) w_unit_tab[t] = my_w_unit;
+  }
   if (t < T::BM) {
     target_tab[t] = my_target;
+    if (kScaled) x_unit_tab[t] = my_x_unit;
     if (SWEEP == 1) row_tab[t] = my_row;
   }
   __syncthreads();
   const int cw = c_base + wn * kStrip;
-  float4 bias[T::NI];
+  float4 bias[T::NI], unit[T::NI];
 #pragma unroll
-  for (int j = 0; j < T::NI; ++j) bias[j] = *reinterpret_cast<const float4*>(bias_tab + wn * kStrip + 16 * j + 4 * g);
+  for (int j = 0; j < T::NI; ++j) {
+    bias[j] = *reinterpret_cast<const float4*>(bias_tab + wn * kStrip + 16 * j + 4 * g);
+    unit[j] = kScaled ? *reinterpret_cast<const float4*>(w_unit_tab + wn * kStrip + 16 * j + 4 * g) : make_float4(1.f, 1.f, 1.f, 1.f);
+  }
   if constexpr (SWEEP != 1) {
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
       const int ml = wm * (T::MI * 16) + 16 * i + (lane & 15);
       const int64_t m = m_base + ml;
+      const float x_unit = kScaled ? x_unit_tab[ml] : 1.0f;
       float v[T::NI][4], mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
         const float* bj = reinterpret_cast<const float*>(&bias[j]);
+        const float* wj = reinterpret_cast<const float*>(&unit[j]);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          v[j][u] = fmaf(acc[i][j][u], unit, bj[u]);
+          v[j][u] = logit<T::TYPE>(acc[i][j][u], x_unit, wj[u], bj[u]);
           mx = fmaxf(mx, v[j][u]);
         }
       }
@@ -518,7 +644,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_lce_logits(LogitArgs a) {
     __syncthreads();
   }
   if constexpr (SWEEP == 1 || SWEEP == 2) {
-    write_gradients<T>(a, acc, bias, unit, tm, cw, row_tab, target_tab, lds + kTabs);
+    write_gradients<T>(a, acc, bias, unit, tm, cw, row_tab, target_tab, x_unit_tab, lds + kTabs);
   }
 }
 
@@ -667,17 +793,17 @@ __global__ __launch_bounds__(1024) void k_lce_rows(RowArgs a) {
 struct GradArgs {
   const char* a; int64_t lda; uint32_t a_plane;
   const char* b; int64_t ldb; uint32_t b_plane;
+  const char* b_same;          // what takes b's place where b's rows differ in scale (Scalars), or null
   int64_t M;
   int N, K, splits, group;     // split s takes K range [s, s + 1) * round_up(ceil(K / splits), 64)
   float* slab; int64_t slab_stride; int ld_slab;  // fp32 [splits][M][ld_slab]; null: out is written
   int accumulate;              // add to what the slab holds (an earlier piece of the classes)
   void* out; int64_t ld_out;   // T_out [M][N]
   int out_bf16, out_vec;       // out_vec: rows may be stored four elements at a time
-  const Scalars* scal;
   int which;                   // 0: dx (the classes' operand is W), 1: dW (x)
 };
 
-__device__ __forceinline__ float grad_factor(const Scalars* s, int which) { return s->g_unit / (which ? s->x_scale : s->w_scale); }
+__device__ __forceinline__ float grad_factor(const Scalars& s, int which) { return s.g_unit / (which ? s.x_scale : s.w_scale); }
 
 __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4], int n_valid, int bf16, int vec) {
   if (bf16) {
@@ -699,7 +825,7 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
 }
 
 template <class T>
-__device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* lds) {
+__device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* lds, const Scalars& scal) {
   const int tiles_m = (int)((a.M + T::BM - 1) / T::BM), tiles_n = (a.N + T::BN - 1) / T::BN;
   const int per = tiles_m * tiles_n;
   const int split = block / per;
@@ -709,16 +835,17 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
   const int n_base = tn * T::BN;
   const int kper = ((a.K + a.splits - 1) / a.splits + 63) / 64 * 64;
   const int k0 = min(split * kper, a.K), k1 = min(k0 + kper, a.K);
+  const char* b_base = a.b_same && (a.which ? scal.x_split : scal.w_split) ? a.b_same : a.b;
   Operand A, B;
   if (T::ACOL) A = Operand{a.a + (int64_t)k0 * a.lda + m_base * 2, (uint32_t)a.lda, (int)min<int64_t>((a.M - m_base + 7) / 8 * 16, 1 << 20), a.a_plane};
   else A = Operand{a.a + m_base * a.lda + (int64_t)k0 * 2, (uint32_t)a.lda, (int)min<int64_t>(T::BM, a.M - m_base), a.a_plane};
-  if (T::BCOL) B = Operand{a.b + (int64_t)k0 * a.ldb + (int64_t)n_base * 2, (uint32_t)a.ldb, (a.N - n_base + 7) / 8 * 16, a.b_plane};
-  else B = Operand{a.b + (int64_t)n_base * a.ldb + (int64_t)k0 * 2, (uint32_t)a.ldb, a.N - n_base, a.b_plane};
+  if (T::BCOL) B = Operand{b_base + (int64_t)k0 * a.ldb + (int64_t)n_base * 2, (uint32_t)a.ldb, (a.N - n_base + 7) / 8 * 16, a.b_plane};
+  else B = Operand{b_base + (int64_t)n_base * a.ldb + (int64_t)k0 * 2, (uint32_t)a.ldb, a.N - n_base, a.b_plane};
   typename T::acc_t acc[T::MI][T::NI];
   T::run(lds, A, B, k1 - k0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const float f = a.slab ? 1.0f : grad_factor(a.scal, a.which);
+  const float f = a.slab ? 1.0f : grad_factor(scal, a.which);
 #pragma unroll
   for (int i = 0; i < T::MI; ++i) {
     const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
@@ -747,14 +874,15 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
 template <class TX, class TW>
 __global__ __launch_bounds__(TX::kThreads, 2) void k_lce_grads(GradArgs dx, GradArgs dw, int dx_blocks, int totals, TotalArgs total) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const Scalars scal = *total.scal;  // (asked for first; where this launch makes g_unit, nothing here uses it)
   const int block = (int)blockIdx.x - totals;
   if (block < 0) {  // finishes the loss instead: nothing else in this launch needs it
     double* d = reinterpret_cast<double*>(lds);
     total_loss(total, *reinterpret_cast<double(*)[4]>(d), *reinterpret_cast<double(*)[4]>(d + 4));
   } else if (block < dx_blocks) {
-    grad_tile<TX>(dx, block, lds);
+    grad_tile<TX>(dx, block, lds, scal);
   } else {
-    grad_tile<TW>(dw, block - dx_blocks, lds);
+    grad_tile<TW>(dw, block - dx_blocks, lds, scal);
   }
 }
 
@@ -783,7 +911,7 @@ __global__ __launch_bounds__(256) void k_lce_finish(FinishArgs a) {
   }
   const int w = (int)blockIdx.x >= a.blk1;
   const int64_t b = blockIdx.x - (w ? a.blk1 : 0), nb = w ? a.blk2 - a.blk1 : a.blk1;
-  const float f = grad_factor(a.scal, w);
+  const float f = grad_factor(*a.scal, w);
   const int q = a.ld_slab / 4;
   for (int64_t e = b * 256 + threadIdx.x; e < a.rows[w] * q; e += nb * 256) {
     const int64_t r = e / q;
@@ -802,7 +930,7 @@ __global__ __launch_bounds__(256) void k_lce_finish(FinishArgs a) {
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 struct Layout {  // offsets into the workspace, bytes
-  size_t scal, amax, bias, xp, wp, strips, target, row, part, g, db, dx_slab, dw_slab, total;
+  size_t scal, amax, bias, x_unit, w_unit, xp, wp, x_same, w_same, strips, target, row, part, g, db, dx_slab, dw_slab, total;
   int Dp, C_pad, n_strips, piece, pieces;
   int dx_splits, dw_splits;
   int64_t ldp, ldg;      // bytes
@@ -897,10 +1025,15 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
   L.scal = take(sizeof(Scalars));
-  L.amax = take(sizeof(float) * 3 * kAmaxBlocks);
+  L.amax = take(sizeof(float) * 5 * kAmaxBlocks);
   L.bias = take(sizeof(float) * L.C_pad);
   L.xp = take((size_t)n * L.ldp);
   L.wp = L.pack_w ? take((size_t)h.n_classes * L.ldp) : 0;
+  L.x_unit = L.w_unit = L.x_same = L.w_same = 0;
+  if (f32 || bf16_in_half(h)) {
+    L.x_unit = take(sizeof(float) * n);
+    L.w_unit = take(sizeof(float) * L.C_pad);
+  }
   L.strips = take(sizeof(float2) * (size_t)L.n_strips * n);
   L.target = take(sizeof(float) * n);
   L.row = take(sizeof(float2) * n);
@@ -911,6 +1044,10 @@ void make_layout(const suave_linear_ce_t& h, Layout& L) {
     L.db = take(sizeof(float) * (size_t)L.db_rows * L.C_pad);
     if (h.dx) L.dx_slab = take(sizeof(float) * (size_t)L.dx_splits * n * L.Dp);
     if (h.dweight && !L.dw_direct) L.dw_slab = take(sizeof(float) * (size_t)L.dw_splits * h.n_classes * L.Dp);
+  }
+  if (f32 || bf16_in_half(h)) {
+    if (h.dweight) L.x_same = take((size_t)n * L.ldp);
+    if (h.dx) L.w_same = take((size_t)h.n_classes * L.ldp);
   }
   L.total = o;
 }
@@ -1011,21 +1148,23 @@ int run_gradients(const suave_linear_ce_t& h, const Layout& L, LogitArgs& a, boo
       GradArgs& g = gx;
       g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
       g.b = a.w + (int64_t)a.c0 * a.ldw; g.ldb = a.ldw; g.b_plane = L.plane;
+      g.b_same = TYPE == kF16 ? ws + L.w_same + (int64_t)a.c0 * L.ldp : nullptr;
       g.M = n; g.N = h.dim; g.K = cp; g.splits = L.dx_splits;
       g.slab = reinterpret_cast<float*>(ws + L.dx_slab); g.slab_stride = n * L.Dp; g.ld_slab = L.Dp; g.accumulate = piece > 0;
-      g.scal = scal; g.which = 0;
+      g.which = 0;
     }
     if (h.dweight) {
       GradArgs& g = gw;
       g.a = a.g; g.lda = L.ldg; g.a_plane = L.g_plane;
       g.b = a.x; g.ldb = L.ldp; g.b_plane = L.plane;
+      g.b_same = TYPE == kF16 ? ws + L.x_same : nullptr;
       g.M = cp; g.N = h.dim; g.K = (int)n; g.splits = L.dw_splits;
       if (!L.dw_direct) {
         g.slab = reinterpret_cast<float*>(ws + L.dw_slab); g.slab_stride = (int64_t)h.n_classes * L.Dp; g.ld_slab = L.Dp;
       }
       g.out = static_cast<char*>(h.dweight) + (int64_t)a.c0 * h.ld_dweight * (bf ? 2 : 4); g.ld_out = h.ld_dweight;
       g.out_bf16 = bf; g.out_vec = vec_ok(h.dweight, h.ld_dweight);
-      g.scal = scal; g.which = 1;
+      g.which = 1;
     }
     if (products)
       if (int rc = launch_grads<TYPE, NP>(gx, gw, L.grad_tile, L.whole, a.total, s)) return rc;
@@ -1068,6 +1207,11 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   PackArgs p{};
   p.src[0] = h.x; p.src[1] = h.weight; p.ld[0] = h.ld_x; p.ld[1] = h.ld_weight; p.rows[0] = n; p.rows[1] = h.n_classes;
   p.dst[0] = ws + L.xp; p.dst[1] = L.pack_w ? ws + L.wp : nullptr; p.dst_ld[0] = p.dst_ld[1] = L.ldp;
+  if (F) {
+    for (int t = 0; t < 2; ++t) p.unit[t] = reinterpret_cast<float*>(ws + (t ? L.w_unit : L.x_unit));
+    p.same[0] = h.dweight ? ws + L.x_same : nullptr;
+    p.same[1] = h.dx ? ws + L.w_same : nullptr;
+  }
   p.D = h.dim; p.Dp = L.Dp; p.targets = h.targets; p.amax = reinterpret_cast<float*>(ws + L.amax); p.scal = scal;
   p.class_weight = F ? h.class_weight : nullptr;
   p.scan = (n + h.n_classes) * h.dim <= kScanElems;
@@ -1089,7 +1233,7 @@ int run_linear_ce(const suave_linear_ce_t& h, const Layout& L, hipStream_t s) {
   a.w = L.pack_w ? ws + L.wp : static_cast<const char*>(h.weight);
   a.ldw = L.pack_w ? L.ldp : h.ld_weight * 2;
   a.plane = L.plane; a.n = n; a.C = h.n_classes; a.D = h.dim; a.c0 = 0; a.c1 = h.n_classes; a.scal = scal;
-  a.bias = p.bias_pad; a.targets = h.targets;
+  a.bias = p.bias_pad; a.targets = h.targets; a.x_unit = p.unit[0]; a.w_unit = p.unit[1];
   a.strips = reinterpret_cast<float2*>(ws + L.strips);
   a.target_logit = reinterpret_cast<float*>(ws + L.target);
   a.row = reinterpret_cast<const float2*>(ws + L.row);
