@@ -45,7 +45,9 @@ struct Scalars {
   float max_w;               // largest |class weight| (1 without gradients and without class weights): G is stored relative to it
 };
 
-// G is stored relative to the largest row weight (entries in [-1, 1]), in fp16 times 2^14: normal down to 2^-28
+// G is stored relative to the largest row weight (entries in [-1, 1]), in fp16 times 2^14: normal down to 2^-28 in one plane; in two off by
+// 2^-23 of itself, or 2^-39 of the largest.  A class that no row gives a chance (p = 2^-20) has its row of dW to 2^-19 of itself, then,
+// and one with p below 2^-39 has zeros there.
 __host__ __device__ constexpr float g_scale(int type) { return type == kF16 ? 16384.0f : 1.0f; }
 // a value in one plane, or two
 template <int TYPE, int NP>
@@ -663,7 +665,7 @@ constexpr int kScaleRows = 32;
 
 // G from the exponentials of a sweep that kept them, in place: exp(l - strip's max) exp(strip's max - lse) instead of a second product.
 // A block takes 32 rows x 256 classes, a thread eight neighbouring classes of every eighth row.  Only for planes, whose rounding
-// (2^-22) may be made twice, and where all the classes are one piece.  Bound by the memory-side cache: 1777 x 20011 50 us for 285 MB,
+// (2^-23) may be made twice, and where all the classes are one piece.  Bound by the memory-side cache: 1777 x 20011 50 us for 285 MB,
 // against 177 us for the second sweep at 501 columns (and 34 more in the first one for the writing).  The first block finishes the loss.
 __global__ __launch_bounds__(256) void k_lce_scale(ScaleArgs a) {
   __shared__ double tot[8];

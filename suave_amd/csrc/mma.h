@@ -2,9 +2,11 @@
 // product (quant.hip):  acc[m][n] = sum_k A[m][k] B[n][k]  for one BM x BN tile of a block.
 //
 // Mathematics: the matrix pipe multiplies bf16, fp16 or int8 fragments into fp32 / int32 accumulators.  A binary32
-// operand enters as TWO fp16 planes, x = hi + lo (each 11 bits, round to nearest: |x - hi - lo| <= 2^-24 |x| while the
-// caller's power-of-two scale keeps lo clear of fp16's subnormals), and a product is hi hi + hi lo + lo hi: the dropped
-// lo lo term is below 2^-24 of the product as well, so the result carries binary32's own error.
+// operand enters as TWO fp16 planes of 11 bits, x = hi + lo, each rounded to nearest.  For 2^e <= |x| < 2^(e+1): |x - hi| <= 2^(e-11), so lo
+// is off by 2^(e-23) at most and |x - hi - lo| <= 2^-23 |x|.  That takes |x| >= 1/4; below it lo is subnormal and off by up to 2^-25 whatever
+// x is, which the caller's power-of-two scale keeps far below its largest values.  A product is hi hi + hi lo + lo hi; the dropped lo lo is
+// at most 2^-22 of it.  These are worst cases of single products, 2 to 4 times binary32's; they have either sign, and a sum of many
+// is off by what binary32's own rounding of it is off by.
 //
 // Operands come in two storage forms.  "Row" form: [rows][K], K contiguous.  "Column" form: [K][rows], rows contiguous
 // (the gradient products read the same stored matrices along their other axis); those fragments are transposed on the
