@@ -269,8 +269,11 @@ int suave_elbo_joint_backward(const suave_plan* plan, const float* params, const
 
 /* Linear layer + class-weighted softmax cross entropy for heads beyond suave_head_step's 64 classes (heads.py:62-91 with
  * F.cross_entropy; also the last layer of a head with hidden layers), with its gradients, without keeping the
- * [n_rows, n_classes] logits: scratch grows with n_rows * n_classes / 8 bytes (statistics of 64-class strips) plus one
- * piece of the logit gradient (at most 192 MiB, or 256 classes of it).
+ * [n_rows, n_classes] logits.  Scratch (suave_linear_ce_workspace_bytes gives the size) is n_rows * n_classes / 8 bytes of statistics of
+ * 64-class strips and copies of the operands in the storage of the products, 4 bytes per element for F32 and 2 for BF16: x, and weight
+ * unless BF16 can be read as it is.  Gradients add a second copy of either for F32 and for BF16 that goes through fp16, up to
+ * n_rows * n_classes / 4 bytes of partial sums of dbias, one piece of the logit gradient (at most 192 MiB, or 256 classes of it) and up to 32
+ * partial results each, in fp32, of dx and dweight (large ones: one of dx, none of dweight).
  *   loss = sum_i w[y_i] (log sum_c exp l_ic - l_i,y_i) / weight_sum,   l = x weight^T + bias
  * weight_sum = sum_i w[y_i], or *weight_sum if given (data parallelism: the GLOBAL batch).  targets[i] < 0 leaves row i
  * out: it adds nothing anywhere, whatever x holds there, and its dx is zero; targets[i] >= n_classes makes the row's
