@@ -15,7 +15,7 @@
 // 2^-8 at most, and next to nothing at the entries p - 1 of the targets, which lie next to -1.  With class weights those entries are
 // anything, and where a class has one row their rounding is as large as the result's own; then (and for up to 8 rows) the operands are copied
 // into one fp16 plane (exact for bf16 values down to 2^-28 of the row's largest, or the tensor's), and G rounded to fp16 (2^-11): 3 passes
-// over W more (4096 x 32000 x 1024: 1081 us against 1020; 33 x 100000 x 2048: 747 against 471).  db and every sum stay fp32.
+// over W more (4096 x 32000 x 1024: 1059 us against 990; 33 x 100000 x 2048: 746 against 446).  db and every sum stay fp32.
 //
 // Rows with a negative target are left out whatever they hold (x is copied with those rows zero); a target >= C makes its row's
 // loss NaN, and with it the mean and the gradients.  No atomics: partial sums are written out and added in a fixed order.
