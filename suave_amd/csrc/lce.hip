@@ -203,7 +203,7 @@ __device__ __forceinline__ float plane_scale(float amax) {
 // the tensor's gets a scale of its own there, or one large row would cost all others their low planes (64 x 1000 x 32 with one
 // row 10^6 times the others: their lse off by 3.7e-5 instead of 2.5e-6).  The gradients' products add over these rows (dW over x's, dx
 // over W's), so they take operands of one scale: what a small row loses there is 2^-38 of the largest.  Looking for such rows and
-// the units' way through the epilogue cost 4096 x 1000 x 128 two microseconds of 59, 1777 x 20011 x 501 nine of 476.
+// the units' way through the epilogue cost 4096 x 1000 x 128 one microsecond of 60, 1777 x 20011 x 501 five of 466.
 constexpr float kSplit = 256.0f;
 __device__ __forceinline__ bool split_rows(float mx, float mn) { return mn < mx * (1.0f / kSplit); }
 __device__ __forceinline__ float pack_row_scale(float row_max, float mx, float scale) {
@@ -827,7 +827,7 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
 }
 
 template <class T>
-__device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* lds, const Scalars& scal) {
+__device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* lds, int b_split, const Scalars* scal) {
   const int tiles_m = (int)((a.M + T::BM - 1) / T::BM), tiles_n = (a.N + T::BN - 1) / T::BN;
   const int per = tiles_m * tiles_n;
   const int split = block / per;
@@ -837,7 +837,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
   const int n_base = tn * T::BN;
   const int kper = ((a.K + a.splits - 1) / a.splits + 63) / 64 * 64;
   const int k0 = min(split * kper, a.K), k1 = min(k0 + kper, a.K);
-  const char* b_base = a.b_same && (a.which ? scal.x_split : scal.w_split) ? a.b_same : a.b;
+  const char* b_base = a.b_same && b_split ? a.b_same : a.b;
   Operand A, B;
   if (T::ACOL) A = Operand{a.a + (int64_t)k0 * a.lda + m_base * 2, (uint32_t)a.lda, (int)min<int64_t>((a.M - m_base + 7) / 8 * 16, 1 << 20), a.a_plane};
   else A = Operand{a.a + m_base * a.lda + (int64_t)k0 * 2, (uint32_t)a.lda, (int)min<int64_t>(T::BM, a.M - m_base), a.a_plane};
@@ -847,7 +847,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
   T::run(lds, A, B, k1 - k0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const float f = a.slab ? 1.0f : grad_factor(scal, a.which);
+  const float f = a.slab ? 1.0f : grad_factor(*scal, a.which);
 #pragma unroll
   for (int i = 0; i < T::MI; ++i) {
     const int64_t m = m_base + wm * (T::MI * 16) + 16 * i + (lane & 15);
@@ -876,15 +876,15 @@ __device__ __forceinline__ void grad_tile(const GradArgs& a, int block, char* ld
 template <class TX, class TW>
 __global__ __launch_bounds__(TX::kThreads, 2) void k_lce_grads(GradArgs dx, GradArgs dw, int dx_blocks, int totals, TotalArgs total) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const Scalars scal = *total.scal;  // (asked for first; where this launch makes g_unit, nothing here uses it)
+  const int x_split = total.scal->x_split, w_split = total.scal->w_split;
   const int block = (int)blockIdx.x - totals;
   if (block < 0) {  // finishes the loss instead: nothing else in this launch needs it
     double* d = reinterpret_cast<double*>(lds);
     total_loss(total, *reinterpret_cast<double(*)[4]>(d), *reinterpret_cast<double(*)[4]>(d + 4));
   } else if (block < dx_blocks) {
-    grad_tile<TX>(dx, block, lds, scal);
+    grad_tile<TX>(dx, block, lds, w_split, total.scal);
   } else {
-    grad_tile<TW>(dw, block - dx_blocks, lds, scal);
+    grad_tile<TW>(dw, block - dx_blocks, lds, x_split, total.scal);
   }
 }
 
